@@ -1,0 +1,253 @@
+"""Softmax cross entropy over many classes against its definition in 64 bits, element by element.
+
+Bounds.  A value rounded to a type is off by at most eps/2 of it (bf16 2^-8, fp16 2^-11, fp32 2^-24).  A sum on the tensor
+cores is cut to fp32 at each step of 16 elements, at most 2^-23 of the sum of the terms' magnitudes a step.
+  scores   16-bit operands: d/16 steps; fp32 operands: planes hold 22 bits each (2^-22 of either factor, 2^-22 for the
+           product that is left out), 48 steps in TMEM and d/256 sums in fp32.  e_s = that bound times the largest Σ_k |x_ik w_jk|
+           of the row, and 2^-22 of the largest score for the scaling by log2 e and its rounding.
+  softmax  relative error e_p = 2 e_s (score and log-sum-exp) + 2^-20 (2^x is off by 2^-22, sums over classes, the coefficient)
+  G        e_p of the softmax part, and its rounding to the operands' type (fp32: 2^-22 in two planes)
+  gx, gw   those errors times |w| or |x|, summed; the steps of that sum; the rounding of the result.  In fp16 a value below
+           2^-14 is rounded to 2^-25 at worst: G is scaled so that its largest possible value lies in [2^13, 2^14)."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _steps(k, dtype):
+    return (2.0 ** -23 * 48 + 2.0 ** -24 * (k / 256 + 1) + 3 * 2.0 ** -22) if dtype == torch.float32 else 2.0 ** -23 * (k / 16 + 1)
+
+
+def _reference(x, w, y, coef):
+    """loss, gx, gw in fp64 with their bounds; rows without a class take no part."""
+    dt = x.dtype
+    live = (y >= 0) & (y < w.shape[0])
+    X = torch.where(live[:, None], x.double(), 0.0)
+    W = w.double()
+    n, d = X.shape
+    V = W.shape[0]
+    s = X @ W.T
+    mag = X.abs() @ W.abs().T
+    lse = torch.logsumexp(s, 1)
+    at = torch.where(live, y, 0)
+    c = torch.where(live, torch.ones(n, dtype=torch.float64, device=x.device) if coef is None else coef.double(), 0.0)
+    loss = c * (lse - s.gather(1, at[:, None])[:, 0])
+    e_s = _steps(d, dt) * mag.max(1).values + 2.0 ** -22 * s.abs().max(1).values
+    loss_tol = c.abs() * (2 * e_s + 2.0 ** -20) + 2.0 ** -22 * loss.abs()
+    e_p = 2 * e_s + 2.0 ** -20
+    p = torch.exp(s - lse[:, None])
+    G = c[:, None] * p
+    eG = G.abs() * e_p[:, None]
+    G[torch.arange(n, device=x.device), at] -= c
+    eG += G.abs() * (2.0 ** -22 if dt == torch.float32 else HALF_STEP[dt])
+    if dt != torch.bfloat16:                    # below fp16's normal numbers, in the scaled value or its low plane
+        eG += 2.0 ** -24 * 2.0 ** -13 * c.abs().max()
+    out = []
+    for A, eA, B, k in ((G, eG, W, V), (G.T, eG.T, X, n)):
+        r = A @ B
+        tol = (eA + _steps(k, dt) * A.abs()) @ B.abs() + HALF_STEP[dt] * r.abs() * 1.01
+        out += [r, tol + (2.0 ** -25 if dt == torch.float16 else 1e-37)]
+    return loss, loss_tol + 1e-37, *out
+
+
+def _check(x, w, y, coef=None):
+    from parameter_server_b200.ops import dense, softmax
+
+    loss, gx, gw = softmax.softmax_loss(x, w, y, coef)
+    only, none_x, none_w = softmax.softmax_loss(x, w, y, coef, want_grad=False)
+    torch.cuda.synchronize()
+    dense.check_status(x.device)
+    assert none_x is None and none_w is None and torch.equal(only, loss)
+    assert loss.dtype == torch.float32 and gx.dtype == x.dtype and gw.dtype == w.dtype and gx.shape == x.shape and gw.shape == w.shape
+    want = _reference(x, w, y, coef)
+    for name, got, ref, tol in (("loss", loss, *want[:2]), ("gx", gx, *want[2:4]), ("gw", gw, *want[4:])):
+        off = (got.double() - ref).abs() / tol
+        assert bool((off <= 1).all()), (name, off.max().item())
+    return loss, gx, gw
+
+
+def _data(n, V, d, dtype, seed=0, scale=2.0):
+    g = torch.Generator(device="cuda").manual_seed(seed + n + V + d)
+    x = torch.randn(n, d, generator=g, device="cuda")
+    w = torch.randn(V, d, generator=g, device="cuda") * scale / d ** 0.5
+    y = torch.randint(0, V, (n,), generator=g, device="cuda")
+    return x.to(dtype), w.to(dtype), y
+
+
+@pytest.mark.parametrize("n,V,d", [
+    (1, 1, 1), (1, 2, 3), (3, 7, 8), (16, 100, 64), (127, 129, 65), (128, 64, 64), (129, 63, 63), (64, 1000, 200), (300, 257, 1),
+    (1, 50_000, 96), (2, 5_001, 1030), (1000, 1, 40), (513, 2049, 130), (4100, 300, 24), (2500, 3000, 72), (4096, 257, 260)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_loss_and_gradients(n, V, d, dtype):
+    _check(*_data(n, V, d, dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_without_a_class_hold_anything(dtype):
+    """A padded batch: what lies in rows with label -1 (NaN, infinities, the type's extremes) and in their coefficients is
+    not looked at; a batch of such rows alone has no gradient."""
+    x, w, y = _data(200, 90, 48, dtype, 1)
+    coef = torch.rand(200, device="cuda") + 0.5
+    gone = torch.arange(200, device="cuda") % 3 == 0
+    y[gone] = -1
+    clean = x.clone()
+    clean[gone] = 0
+    want = _check(clean, w, y, coef)
+    dirty, dirty_coef = x.clone(), coef.clone()
+    fills = [float("nan"), float("inf"), -float("inf"), torch.finfo(dtype).min, torch.finfo(dtype).max]
+    for i, r in enumerate(gone.nonzero()[:, 0].tolist()):
+        dirty[r] = fills[i % 5]
+        dirty_coef[r] = fills[(i + 1) % 5]
+    from parameter_server_b200.ops import softmax
+
+    got = softmax.softmax_loss(dirty, w, y, dirty_coef)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert not got[0][gone].any() and not got[1][gone].any()
+    for t in softmax.softmax_loss(dirty, w, torch.full_like(y, -1), dirty_coef):
+        assert not t.any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["small", "large", "negative", "zero"])
+def test_coefficients(dtype, kind):
+    x, w, y = _data(150, 333, 56, dtype, 2)
+    c = torch.rand(150, device="cuda") + 0.5
+    c = {"small": c * 1e-4, "large": c * 100, "negative": -c, "zero": c * 0}[kind]
+    _check(x, w, y, c)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_confident_and_far_scores(dtype):
+    """Scores of some hundreds: no overflow, and the loss of a row whose class is certain is not negative."""
+    x, w, y = _data(130, 500, 64, dtype, 3, scale=60.0)
+    y[:65] = (x.float() @ w.float().T).argmax(1)[:65]
+    loss, _, _ = _check(x, w, y)
+    assert bool((loss >= 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_and_alignment(dtype):
+    """Rows with a stride, from any offset, one row for all: as from a contiguous copy."""
+    from parameter_server_b200.ops import softmax
+
+    big = torch.randn(140, 300, device="cuda").to(dtype)
+    wig = torch.randn(210, 310, device="cuda").to(dtype)
+    y = torch.randint(0, 200, (140,), device="cuda")
+    for a, b in ((big[:, 3:103], wig[:200, 5:105]), (big[:, 8:108], wig[5:205, 16:116]), (big[:1].expand(140, 300)[:, 1:101], wig[1:201, :100])):
+        got = softmax.softmax_loss(a, b, y)
+        want = softmax.softmax_loss(a.contiguous(), b.contiguous(), y)
+        for g, t in zip(got, want):
+            assert torch.equal(g, t)
+    yy = torch.stack([y, y], 1)[:, 0]
+    assert torch.equal(softmax.softmax_loss(big, wig[:200, :300], yy, want_grad=False)[0], softmax.softmax_loss(big, wig[:200, :300], y, want_grad=False)[0])
+
+
+def test_gradients_against_differences():
+    """(f(t + h) − f(t − h)) / 2h of the summed loss: with h = 2^-3 its own error is of order h²/6 of a third derivative
+    below |direction·w|³, which the directions keep under 1e-3; the losses' sum is off by 1e-4 at most."""
+    from parameter_server_b200.ops import softmax
+
+    x, w, y = _data(40, 60, 32, torch.float32, 4)
+    coef = torch.rand(40, device="cuda") + 0.5
+    _, gx, gw = softmax.softmax_loss(x, w, y, coef)
+    h = 2.0 ** -3
+    for t, g in ((x, gx), (w, gw)):
+        u = torch.randn_like(t)
+        u = u / u.norm()
+        f = [softmax.softmax_loss(*(a + s * h * u if a is t else a for a in (x, w)), y, coef, want_grad=False)[0].double().sum() for s in (1, -1)]
+        assert abs(((f[0] - f[1]) / (2 * h)).item() - (g.double() * u.double()).sum().item()) < 3e-3
+
+
+def test_labels_outside_the_classes():
+    from parameter_server_b200.ops import dense, softmax
+
+    x, w, y = _data(20, 30, 16, torch.bfloat16, 5)
+    dense.check_status(x.device)
+    bad = y.clone()
+    bad[3], bad[7], bad[9] = 30, -2, 1 << 40
+    got = softmax.softmax_loss(x, w, bad)
+    with pytest.raises(RuntimeError):
+        dense.check_status(x.device)
+    bad[[3, 7, 9]] = -1
+    for a, b in zip(got, softmax.softmax_loss(x, w, bad)):
+        assert torch.equal(a, b)
+    dense.check_status(x.device)
+
+
+def test_nan_and_infinity_in_rows_with_a_class():
+    """They reach the loss and the gradient of their own row, and no other row's loss."""
+    from parameter_server_b200.ops import softmax
+
+    for dtype in TYPES:
+        x, w, y = _data(50, 70, 32, dtype, 6)
+        x[4, 5], x[9, 1] = float("nan"), float("inf")
+        loss, gx, _ = softmax.softmax_loss(x, w, y)
+        bad = torch.zeros(50, dtype=torch.bool, device="cuda")
+        bad[4] = bad[9] = True
+        assert bool(torch.isnan(loss[bad]).all()) and bool(torch.isfinite(loss[~bad]).all())
+        assert bool(torch.isnan(gx[bad]).any(1).all()) and bool(torch.isfinite(gx[~bad]).all())
+
+
+def test_captured_replayed_and_on_another_stream():
+    from parameter_server_b200.ops import softmax
+
+    x, w, y = _data(300, 700, 72, torch.float32, 7)
+    want = softmax.softmax_loss(x, w, y)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = softmax.softmax_loss(x, w, y)
+    stream.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    graphs = []
+    for _ in range(2):                                   # two graphs alive at once, each with a workspace of its own
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = softmax.softmax_loss(x, w, y)
+        graphs.append((graph, out))
+    x2 = torch.randn_like(x)
+    want2 = softmax.softmax_loss(x2, w, y)
+    x.copy_(x2)
+    for graph, _ in graphs:
+        graph.replay()
+    graphs[0][0].replay()
+    torch.cuda.synchronize()
+    for _, out in graphs:
+        for a, b in zip(out, want2):
+            assert torch.equal(a, b)
+
+
+def test_no_rows():
+    from parameter_server_b200.ops import softmax
+
+    w = torch.randn(5, 8, device="cuda")
+    loss, gx, gw = softmax.softmax_loss(torch.empty(0, 8, device="cuda"), w, torch.empty(0, dtype=torch.int64, device="cuda"))
+    assert loss.shape == (0,) and gx.shape == (0, 8) and not gw.any()
+
+
+def test_classes_in_several_pieces():
+    """More rows × classes than one piece of the softmax holds: 256 MB of fp16 planes are 22,000 classes of 3,050 rows."""
+    from parameter_server_b200.ops import dense, softmax
+
+    x, w, y = _data(3050, 50_001, 40, torch.float32, 8)
+    y[::7] = -1
+    loss, gx, gw = softmax.softmax_loss(x, w, y)
+    dense.check_status(x.device)
+    live = (y >= 0).nonzero()[:, 0]
+    s = x[live].double() @ w.double().T
+    p = torch.softmax(s, 1)
+    p[torch.arange(len(live), device="cuda"), y[live]] -= 1
+    ref = torch.zeros(3050, 40, dtype=torch.float64, device="cuda")
+    ref[live] = p @ w.double()
+    # 2-norms: the errors of elements are independent and far below their bounds above; 1e-5 is 84 fp32 half steps
+    assert ((gx.double() - ref).norm() / ref.norm()).item() < 1e-5
+    refw = p.T @ x[live].double()
+    assert ((gw.double() - refw).norm() / refw.norm()).item() < 1e-5
+    lse = torch.logsumexp(s, 1) - s.gather(1, y[live][:, None])[:, 0]
+    assert ((loss[live].double() - lse).norm() / lse.norm()).item() < 1e-5
