@@ -1,0 +1,80 @@
+"""Orthogonalised weight updates (``csrc/orthogonal.cu``): Newton-Schulz steps with the polynomial of the Muon optimiser on
+the tensor cores, alone and as an update rule next to :func:`dense.sgd_update`."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import _native as N
+from . import dense
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+EPS = 1e-7            # added to the Frobenius norm that the steps start from
+MAX_STEPS = 64
+
+
+class _Args(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("m", C.c_void_p), ("out", C.c_void_p), ("batch", C.c_int), ("rows", C.c_int), ("cols", C.c_int),
+                ("dtype", C.c_int), ("steps", C.c_int), ("nesterov", C.c_int), ("lr", C.c_float), ("momentum", C.c_float),
+                ("eps", C.c_float), ("pad", C.c_float), ("ws", C.c_void_p), ("ws_bytes", C.c_int64), ("status", C.c_void_p)]
+
+
+def _check(what: str, t: torch.Tensor, like: torch.Tensor, dtypes) -> None:
+    if not t.is_cuda or t.device != like.device:
+        raise ValueError(f"{what} has to be on the GPU of the first tensor")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{what} has to be {' or '.join(str(d) for d in dtypes)}: got {t.dtype}")
+    if t.dim() not in (2, 3) or t.shape != like.shape:
+        raise ValueError(f"{what}: matrices [rows, cols] or [batch, rows, cols] of one shape: got {tuple(t.shape)} and {tuple(like.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what} has to be contiguous")
+
+
+def _run(x, m, out, steps, lr, momentum, nesterov) -> None:
+    if not 1 <= steps <= MAX_STEPS:
+        raise ValueError(f"1 to {MAX_STEPS} steps: got {steps}")
+    batch, rows, cols = (1, *x.shape) if x.dim() == 2 else x.shape
+    if batch > 65535 or max(rows, cols) > 1 << 30:
+        raise ValueError("at most 65,535 matrices of at most 2^30 rows and columns")
+    if x.numel() == 0:
+        return
+    a = _Args(x.data_ptr(), None if m is None else m.data_ptr(), out.data_ptr(), batch, rows, cols, DTYPES[x.dtype], steps, int(nesterov),
+              lr, momentum, EPS, 0.0, None, 0, dense.status_ptr(x.device))
+    lib = N.lib()
+    lib.psb_orthogonal_workspace.restype = C.c_int64
+    size = lib.psb_orthogonal_workspace(C.byref(a))
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+    a.ws, a.ws_bytes = ws.data_ptr(), size
+    N.check(lib.psb_orthogonal(C.byref(a), N.stream_ptr()), "orthogonal")
+
+
+def orthogonalize(x: torch.Tensor, steps: int = 5) -> torch.Tensor:
+    """``steps`` Newton-Schulz steps on a contiguous matrix [rows, cols] or a batch [batch, rows, cols], fp32, bf16 or
+    fp16: ``X = x / (|x|_F + 1e-7)``, then ``X ← 3.4445 X − 4.7750 (X Xᵀ) X + 2.0315 (X Xᵀ)² X`` each, which brings singular
+    values into about [0.7, 1.2].  The result has the type of x; fp32 and fp16 results are computed with 22-bit operands, bf16 ones
+    with 22 bits up to the last two steps and 11 bits in those.  The workspace takes 8 bytes an element of x and 16 bytes
+    an element of the smaller square."""
+    _check("orthogonalize: x", x, x, tuple(DTYPES))
+    with torch.cuda.device(x.device):
+        out = torch.empty_like(x)
+        _run(x, None, out, steps, 0.0, 0.0, False)
+    return out
+
+
+def orthogonal_update(w: torch.Tensor, g: torch.Tensor, m: torch.Tensor, lr: float, momentum: float = 0.95, nesterov: bool = True,
+                      steps: int = 5) -> None:
+    """One update of fp32 weights ``w`` [rows, cols] or [batch, rows, cols] with their gradient ``g`` (fp32, bf16 or fp16) and
+    momentum ``m`` (fp32), in place: ``m ← momentum·m + g``, ``w ← w − lr·√max(1, rows/cols)·orthogonalize(u)`` with
+    ``u = g + momentum·m`` (``nesterov``) or ``m``, all contiguous and apart in memory."""
+    _check("orthogonal_update: w", w, w, (torch.float32,))
+    _check("orthogonal_update: g", g, w, tuple(DTYPES))
+    _check("orthogonal_update: m", m, w, (torch.float32,))
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (w, g, m))
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("orthogonal_update: w, g and m share memory")
+    with torch.cuda.device(w.device):
+        _run(g, m, w, steps, lr * math.sqrt(max(1.0, w.shape[-2] / max(w.shape[-1], 1))), momentum, nesterov)
+    dense._written(w)
+    dense._written(m)
