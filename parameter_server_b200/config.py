@@ -95,7 +95,8 @@ LMCall = Schema("LM.Call", F("cmd", LMCommand, "required"), F("key", PbRange), F
                 F("block_order", "int32", "repeated"), F("num_prior", "int32", default=0))
 
 # ---------------------------------------------------------------- neural_network.proto
-LayerType = Enum("LayerConfig.Type", NONE=0, FULLY_CONNECTED=1, DATA=2, LOGISTIC_LOSS=3, AUC=4, SPARSE_FULLY_CONNECTED=5)
+LayerType = Enum("LayerConfig.Type", NONE=0, FULLY_CONNECTED=1, DATA=2, LOGISTIC_LOSS=3, AUC=4, SPARSE_FULLY_CONNECTED=5,
+                 SOFTMAX_LOSS=6)
 ActivationType = Enum("ActivationConfig.Type", IDENTITY=0, SIGMOID=1, LOGISTIC=2, SOFTMAX=3, RELU=4, SCALED_TANH=5)
 ActivationConfig = Schema("ActivationConfig", F("type", ActivationType, "required"))
 LayerConfig = Schema("LayerConfig", F("type", LayerType, "required"), F("name", "string", "required"),
@@ -104,10 +105,11 @@ LayerConfig = Schema("LayerConfig", F("type", LayerType, "required"), F("name", 
                      F("lr_scale", "double", default=1.0), F("data", DataConfig), F("init", ParameterInitConfig))
 NetConfig = Schema("NetConfig", F("name", "string"), F("layer", LayerConfig, "repeated"))
 NNSolverType = Enum("NN.SolverConfig.Type", SGD=1)
-NNUpdate = Enum("NN.SolverConfig.Update", NORMAL=1, ADAGRAD=2)
+NNUpdate = Enum("NN.SolverConfig.Update", NORMAL=1, ADAGRAD=2, ORTHOGONAL=3)
 NNSolverConfig = Schema("NN.SolverConfig", F("type", NNSolverType, "required"), F("update", NNUpdate),
                         F("lr", LearningRateConfig), F("max_iteration", "int32", default=1000),
-                        F("display", "int32", default=100), F("validation", "int32", default=100))
+                        F("display", "int32", default=100), F("validation", "int32", default=100),
+                        F("momentum", "float", default=0.95))
 NNConfig = Schema("NN.Config", F("train", NetConfig), F("test", NetConfig), F("solver", NNSolverConfig))
 
 # ---------------------------------------------------------------- app.proto

@@ -474,7 +474,7 @@ LossPlan loss_plan(const LossArgs& a) {
     p.g = take(p.g_plane * 2 * p.planes);
     p.gx_splits = p.piece >= a.V ? split_count(a.n, a.d, a.V) : 1;
     p.gw_splits = p.piece >= a.V ? split_count(a.V, a.d, a.n) : 1;
-    if (p.gx_splits > 1 || p.piece < a.V) p.gx_acc = take((int64_t)p.gx_splits * a.n * a.d * 4);
+    if (a.gx != nullptr && (p.gx_splits > 1 || p.piece < a.V)) p.gx_acc = take((int64_t)p.gx_splits * a.n * a.d * 4);
     if (p.gw_splits > 1) p.gw_acc = take((int64_t)p.gw_splits * a.V * a.d * 4);
   }
   p.total = at;
@@ -577,6 +577,7 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
     if (r) return r;
     if (p.gw_splits > 1)
       k_loss_sum<<<blocks_for((int64_t)a.V * a.d), 256, 0, s>>>(eg.acc, p.gw_splits, eg.slot, (int64_t)a.V * a.d, a.gw, scal, a.dtype, 0);
+    if (a.gx == nullptr) continue;
     // gx += G w[v0.., :]
     Gemm16Args gx = g;
     const int vkb = (len + kG16K - 1) / kG16K;

@@ -1,5 +1,5 @@
-"""The neural-network application: a DAG of layers built from a ``NetConfig``, trained by SGD or
-AdaGrad, with the dense layers on the tcgen05 tensor cores.
+"""The neural-network application: a DAG of layers built from a ``NetConfig``, trained by SGD,
+AdaGrad or orthogonalised updates, with the dense layers on the tcgen05 tensor cores.
 
 Reference: ``Net`` (src/neural_network/net.h:34-65), ``Layer`` + factory
 (src/neural_network/layer.h:26-73, layer_inl.h:12-36), ``FullyConnectedLayer``
@@ -9,6 +9,9 @@ Reference: ``Net`` (src/neural_network/net.h:34-65), ``Layer`` + factory
 (sgd_solver.h:11-67).  The reference's solver never distributes (its ``process()`` is empty); here
 ranks train data-parallel: every rank draws its own minibatches and the weight gradients are
 all-reduced over NCCL before the update.
+
+Not in the reference: the loss over many classes (``SOFTMAX_LOSS``) and the orthogonalised update of weight
+matrices (``update: ORTHOGONAL``).
 
 Layout: activations are ``[batch, features]``, weights are stored ``[out, in]`` so that both GEMM
 operands of the forward pass are K-major; the two products of the backward pass read transposes
@@ -26,7 +29,7 @@ from typing import Dict, List, Optional
 import numpy as np
 import torch
 
-from ..ops import dense
+from ..ops import dense, orthogonal, softmax
 from ..parallel.peer import PeerGroup
 from ..config import data_files
 from ..runtime import host
@@ -34,11 +37,12 @@ from ..runtime import host
 
 @dataclass
 class Parameter:
-    """Edge or model tensor of the net: value, gradient, AdaGrad accumulator."""
+    """Edge or model tensor of the net: value, gradient, AdaGrad accumulator, momentum of the orthogonalised update."""
     name: str
     value: Optional[torch.Tensor] = None
     gradient: Optional[torch.Tensor] = None
     hession: Optional[torch.Tensor] = None
+    momentum: Optional[torch.Tensor] = None
 
 
 def init_tensor(shape, init, device, seed: int) -> torch.Tensor:
@@ -88,7 +92,10 @@ class DataLayer(Layer):
         X = torch.zeros(rows, cols)
         rr = np.repeat(np.arange(rows), np.diff(off))
         X[torch.from_numpy(rr), torch.from_numpy(idx)] = torch.from_numpy(val if len(val) else np.ones(len(idx), np.float32))
-        self.set_data(X, torch.from_numpy(np.where(r.value(0) > 0, 1.0, -1.0).astype(np.float32)))
+        labels = r.value(0)
+        if not any(lc.type == "SOFTMAX_LOSS" for lc in self.net.conf.layer):      # whose labels are the numbers of classes
+            labels = np.where(labels > 0, 1.0, -1.0)
+        self.set_data(X, torch.from_numpy(labels.astype(np.float32)))
 
     def set_data(self, X: torch.Tensor, y: torch.Tensor, normalize: bool = True) -> None:
         self.X = X.to(self.net.device).contiguous().float()
@@ -143,6 +150,16 @@ class DataLayer(Layer):
         return 0.0
 
 
+def shared_model(layer: Layer, shape) -> Parameter:
+    """The model of a layer: the one that a net of the same layer names made already (the test net shares the training
+    net's), or a new one, the same in every process."""
+    shared = layer.net.shared_models.get(layer.name)
+    if shared is None:
+        w = init_tensor(shape, layer.conf.init if layer.conf.has("init") else None, layer.net.device, seed=zlib.crc32(layer.name.encode()) % (1 << 30))
+        shared = layer.net.shared_models[layer.name] = Parameter(layer.name, w, torch.zeros_like(w), None)
+    return shared
+
+
 def _transposed(x: torch.Tensor) -> torch.Tensor:
     """``xᵀ``, contiguous and 16-byte aligned, to be read only: a single row or column is laid out like its transpose."""
     same = 1 in x.shape and x.numel() > 0 and x.is_contiguous() and x.data_ptr() % 16 == 0
@@ -162,14 +179,7 @@ class FullyConnectedLayer(Layer):
 
     def _ensure_model(self, in_dim: int) -> None:
         if self.model is None:
-            shared = self.net.shared_models.get(self.name)
-            if shared is not None:
-                self.model = shared                      # CLONE: the test net shares the training net's model
-                return
-            w = init_tensor((self.out_dim, in_dim), self.conf.init if self.conf.has("init") else None, self.net.device,
-                            seed=zlib.crc32(self.name.encode()) % (1 << 30))   # same weights in every process
-            self.model = Parameter(self.name, w, torch.zeros_like(w), None)
-            self.net.shared_models[self.name] = self.model
+            self.model = shared_model(self, (self.out_dim, in_dim))
 
     def forward(self) -> float:
         x = self.inputs[0].value
@@ -216,13 +226,7 @@ class SparseFullyConnectedLayer(Layer):
     def forward(self) -> float:
         off, idx, vals, in_dim = self.inputs[0].value
         if self.model is None:
-            shared = self.net.shared_models.get(self.name)
-            if shared is None:
-                w = init_tensor((in_dim, self.out_dim), self.conf.init if self.conf.has("init") else None, self.net.device,
-                                seed=zlib.crc32(self.name.encode()) % (1 << 30))
-                shared = Parameter(self.name, w, torch.zeros_like(w), None)
-                self.net.shared_models[self.name] = shared
-            self.model = shared
+            self.model = shared_model(self, (in_dim, self.out_dim))
         self.x = (off, idx, vals, in_dim)
         self.outputs[0].value = dense.sparse_fc_forward(off, idx, vals, self.model.value, self.act)
         return 0.0
@@ -244,6 +248,29 @@ class LogisticLossLayer(Layer):
         self.inputs[0].gradient = self.grad.reshape(self.inputs[0].value.shape)
 
 
+class SoftmaxLossLayer(Layer):
+    """Softmax cross entropy over ``size`` classes: the layer holds the classes' weights [size, in], so that the scores
+    need not be kept.  Labels are class numbers from 0 on, as floats or integers; -1 is a row without a class."""
+
+    def init(self) -> None:
+        self.classes = int(self.conf.size)
+        if self.classes <= 0:
+            raise ValueError("a softmax loss needs the number of classes (size)")
+
+    def forward(self) -> float:
+        x, y = self.inputs[0].value, self.inputs[1].value
+        if self.model is None:
+            self.model = shared_model(self, (self.classes, x.shape[1]))
+        losses, self.gx, self.gw = softmax.softmax_loss(x, self.model.value, y.reshape(-1).long(), want_grad=self.net.training,
+                                                        want_gx=self.inputs[0].needs_grad)
+        self.loss, self.n = losses.sum(dtype=torch.float64).reshape(1), y.numel()
+        return 0.0
+
+    def backward(self) -> None:
+        self.model.gradient = self.gw
+        self.inputs[0].gradient = self.gx
+
+
 class AUCLayer(Layer):
     def forward(self) -> float:
         x, y = self.inputs[0].value.reshape(-1), self.inputs[1].value
@@ -254,7 +281,8 @@ class AUCLayer(Layer):
 
 
 LAYERS = {"DATA": DataLayer, "FULLY_CONNECTED": FullyConnectedLayer, "SPARSE_FULLY_CONNECTED": SparseFullyConnectedLayer,
-          "LOGISTIC_LOSS": LogisticLossLayer, "AUC": AUCLayer}
+          "LOGISTIC_LOSS": LogisticLossLayer, "AUC": AUCLayer, "SOFTMAX_LOSS": SoftmaxLossLayer}
+LOSSES = (LogisticLossLayer, SoftmaxLossLayer)
 
 
 class Edge(Parameter):
@@ -336,7 +364,9 @@ class Net:
 
 
 class SGDSolver:
-    """w ← w − α·g/(β+√t) or AdaGrad w ← w − α·g/(β+√Σg²); periodic evaluation of the test net."""
+    """w ← w − α·g/(β+√t), AdaGrad w ← w − α·g/(β+√Σg²), or orthogonalised updates: the weight matrices between dense layers
+    by ``orthogonal_update`` with the step α/(β+√t), all other models (feature vectors, classes) by AdaGrad.  Periodic evaluation
+    of the test net."""
 
     def __init__(self, nn_conf, group: PeerGroup):
         self.conf, self.group = nn_conf, group
@@ -344,7 +374,8 @@ class SGDSolver:
         self.test = Net(nn_conf.test, group, self.train.shared_models, training=False) if nn_conf.has("test") else None
         s = nn_conf.solver
         self.alpha, self.beta = s.lr.alpha, s.lr.beta
-        self.adagrad = s.update == "ADAGRAD"
+        self.adagrad, self.orthogonal = s.update == "ADAGRAD", s.update == "ORTHOGONAL"
+        self.momentum = s.momentum
         self.history: List[dict] = []
 
     def step(self, it: int) -> float:
@@ -359,10 +390,17 @@ class SGDSolver:
 
                 dist.all_reduce(p.gradient, group=self.group.group)
                 p.gradient /= self.group.world
-            if self.adagrad and p.hession is None:
+            if self.orthogonal and isinstance(l, FullyConnectedLayer):
+                if p.momentum is None:
+                    p.momentum = torch.zeros_like(p.value)
+                orthogonal.orthogonal_update(p.value, p.gradient, p.momentum, self.alpha * l.lr_scale / (self.beta + math.sqrt(it + 1)),
+                                             momentum=self.momentum)
+                continue
+            adagrad = self.adagrad or self.orthogonal
+            if adagrad and p.hession is None:
                 p.hession = torch.zeros_like(p.value)
-            dense.sgd_update(p.value, p.gradient, p.hession if self.adagrad else None, self.alpha * l.lr_scale, self.beta, it + 1)
-        loss_layer = next((l for l in self.train.layers if isinstance(l, LogisticLossLayer)), None)
+            dense.sgd_update(p.value, p.gradient, p.hession if adagrad else None, self.alpha * l.lr_scale, self.beta, it + 1)
+        loss_layer = next((l for l in self.train.layers if isinstance(l, LOSSES)), None)
         return float(loss_layer.loss.item()) / max(loss_layer.n, 1) if loss_layer else 0.0
 
     def evaluate(self) -> Optional[float]:
@@ -372,6 +410,11 @@ class SGDSolver:
         auc_layer = next((l for l in self.test.layers if isinstance(l, AUCLayer)), None)
         return auc_layer.auc if auc_layer else None
 
+    def test_loss(self) -> Optional[float]:
+        """The mean softmax loss of the test net's last evaluation."""
+        l = next((l for l in self.test.layers if isinstance(l, SoftmaxLossLayer)), None) if self.test is not None else None
+        return float(l.loss.item()) / max(l.n, 1) if l else None
+
     def run(self, verbose: bool = True) -> List[dict]:
         s = self.conf.solver
         for it in range(s.max_iteration):
@@ -379,9 +422,11 @@ class SGDSolver:
             rec = {"iter": it, "loss": loss}
             if s.validation > 0 and (it + 1) % s.validation == 0:
                 rec["test_auc"] = self.evaluate()
+                if (test_loss := self.test_loss()) is not None:
+                    rec["test_loss"] = test_loss
             if verbose and self.group.rank == 0 and ((it + 1) % max(s.display, 1) == 0 or "test_auc" in rec):
-                print(f"iter {it + 1:6d}  loss {loss:.5f}" + (f"  test auc {rec['test_auc']:.5f}" if rec.get("test_auc") is not None else ""),
-                      file=sys.stderr)
+                print(f"iter {it + 1:6d}  loss {loss:.5f}" + (f"  test auc {rec['test_auc']:.5f}" if rec.get("test_auc") is not None else "")
+                      + (f"  test loss {rec['test_loss']:.5f}" if "test_loss" in rec else ""), file=sys.stderr)
             self.history.append(rec)
         dense.check_status(self.group.device)
         return self.history

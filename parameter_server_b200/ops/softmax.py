@@ -21,10 +21,10 @@ class _Args(C.Structure):
 
 
 def softmax_loss(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, coef: Optional[torch.Tensor] = None,
-                 want_grad: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+                 want_grad: bool = True, want_gx: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(loss, gx, gw) of rows ``x`` [n, d] against classes ``w`` [classes, d], both fp32, bf16 or fp16:
     ``loss[i] = coef[i]·(log Σ_j exp(x_i·w_j) − x_i·w_{y_i})`` in fp32 [n] and the gradients of its sum, in the type of the
-    operands (None without ``want_grad``).
+    operands (None without ``want_grad``; ``want_gx`` False leaves gx out, for rows that are data).
 
     ``y``: int64 [n], 0 ≤ y < classes; -1 is a row without a class: whatever x and coef hold there, its loss is 0 and it has
     no part in the gradients.  Another label counts as -1 and is reported by :func:`dense.check_status`.  ``coef``: fp32 [n]
@@ -50,13 +50,13 @@ def softmax_loss(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, coef: Option
         raise ValueError("softmax_loss takes labels int64 [n] and coefficients float32 [n]")
     with torch.cuda.device(x.device):
         loss = torch.empty(n, dtype=torch.float32, device=x.device)
-        gx = torch.empty((n, d), dtype=x.dtype, device=x.device) if want_grad else None
+        gx = torch.empty((n, d), dtype=x.dtype, device=x.device) if want_grad and want_gx else None
         gw = torch.empty((classes, d), dtype=w.dtype, device=x.device) if want_grad else None
         if n == 0:
             return loss, gx, gw.zero_() if want_grad else None
         y, coef = y.contiguous(), None if coef is None else coef.contiguous()
         a = _Args(x.data_ptr(), w.data_ptr(), y.data_ptr(), None if coef is None else coef.data_ptr(), loss.data_ptr(),
-                  gx.data_ptr() if want_grad else None, gw.data_ptr() if want_grad else None, x.stride(0), w.stride(0), n, classes, d,
+                  None if gx is None else gx.data_ptr(), gw.data_ptr() if want_grad else None, x.stride(0), w.stride(0), n, classes, d,
                   DTYPES[x.dtype], int(want_grad), 0, None, 0, dense.status_ptr(x.device))
         lib = N.lib()
         lib.psb_softmax_loss_workspace.restype = C.c_int64
