@@ -6,15 +6,20 @@
 // and lo·hi in one accumulator; what is left out, lo·lo, is below 2^-22 of the terms.  That costs three 16-bit products
 // where three tf32 products (11 bits as well) would cost six.  The tensor cores cut a sum to fp32 at every step of 16
 // elements instead of rounding it, an error that grows with the number of steps (K = 60,000: 6e-5 of a gradient); products
-// of planes are therefore summed in TMEM for 256 elements of K at a time (48 steps) and added up in the epilogue's
-// registers.  An operand may lie either way round in memory: K-major
+// of planes are therefore summed in TMEM for 128 elements of K at a time (24 steps) and added up in the epilogue's
+// registers.  (64 elements: 25 % slower; 256: 4 % faster, twice the error.)  An operand may lie either way round in memory: K-major
 // ([rows][k], k contiguous) or MN-major ([k][rows], rows contiguous); nothing is transposed in memory.
 //
 // Shape.  Persistent CTAs, or CTA pairs (cta_group::2) where the problem has enough tiles:
 //   warp 0, one lane    TMA producer, a ring of stages of 64 elements of K (128-byte swizzle rows)
 //   warp 1, one lane    tcgen05.mma; in a pair the leader issues for both CTAs
-//   warps 2-9           epilogue: warp w reads TMEM lanes 32(w % 4)..+31, half of the tile's columns; the accumulator is
+//   warps 4-11          epilogue: warp w reads TMEM lanes 32(w % 4)..+31, half of the tile's columns; the accumulator is
 //                       double-buffered, so a tile's epilogue runs under the next tile's products
+// Sums of planes need 128 registers of an epilogue thread: its warps take over registers of the other four.
+// 16-bit results leave through shared memory as TMA stores of 32 x 32 boxes: a lane holds a row, and stores of rows by
+// lanes touch 32 lines an instruction (4096 x 4096 Newton-Schulz step: 2.6 times the time).
+// Launches of one call overlap: a kernel sets itself up while the one before it drains (programmatic dependent launch) and
+// waits for it before it touches memory.
 // No load is a multicast.
 #pragma once
 #include <cuda_bf16.h>
@@ -24,22 +29,23 @@
 
 namespace psb {
 
-constexpr int kG16Threads = 320, kG16K = 64;
+constexpr int kG16Threads = 384, kG16K = 64;
+constexpr int kG16Epi = 4;                         // first warp of the epilogue, of eight
+constexpr int kStageOut = 4096;                   // bytes of shared memory of an epilogue warp
 constexpr int kG16Smem = 192 * 1024;              // of the stages
 
-template <int kCtas_, int kN_, int kPlanes_, bool kAMN_, bool kBMN_>
+template <int kCtas_, int kN_, int kPlanes_>
 struct Cfg16 {
   static constexpr int kCtas = kCtas_, kN = kN_, kPlanes = kPlanes_;
-  static constexpr bool kAMN = kAMN_, kBMN = kBMN_;
   static constexpr int kM = 128 * kCtas, kBRows = kN / kCtas;
   static constexpr int kABytes = 128 * 128, kBBytes = kBRows * 128;
   static constexpr int kStageBytes = kPlanes * (kABytes + kBBytes);
   static constexpr int kStages = kG16Smem / kStageBytes > 8 ? 8 : kG16Smem / kStageBytes;
-  static constexpr int kSmemBytes = kStages * kStageBytes + 1024 + 512;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 8 * kStageOut + 1024 + 256;
   static constexpr bool kPromote = kPlanes == 2;   // sums of kChunk blocks of K are added up in registers
-  static constexpr int kChunk = kPromote ? 4 : 1 << 30;
+  static constexpr int kChunk = kPromote ? 2 : 1 << 30;
   static constexpr uint32_t kTmem = 2 * kN < 32 ? 32 : 2 * kN;
-  static_assert(kStages >= 3 && kBRows % 64 == 0 && kTmem <= 512, "shape of a tile");
+  static_assert(kStages >= 3 && kBRows % 64 == 0 && kTmem <= 512 && kSmemBytes <= 232448, "shape of a tile");
 };
 
 struct Gemm16Args {
@@ -48,6 +54,7 @@ struct Gemm16Args {
   int a_z, b_z;                // matrices of a map per batch entry (planes that lie there, whether read or not); 0: one for all
   int a_m0, a_k0, b_n0, b_k0;  // where the problem starts in the maps
   int splits, kb_split;        // K blocks are dealt to `splits` pieces of kb_split; a piece is a tile of its own
+  int a_mn, b_mn;              // an operand is MN-major
   int sym;                     // square result that is symmetric: only tiles on and above the diagonal
   int bf16;                    // operands are bf16, else fp16
   uint32_t* status;
@@ -105,9 +112,9 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 }
 // rows r0.. of an operand, K block k0, into `rows` swizzled rows of 128 bytes (K-major) or into chunks of 64 rows, each
 // 64 k-lines of 128 bytes (MN-major)
-template <int kCtas, bool kMN, int kRows>
-__device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap* map, uint32_t bar, int k0, int r0, int z) {
-  if constexpr (kMN) {
+template <int kCtas, int kRows>
+__device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap* map, uint32_t bar, int k0, int r0, int z, bool mn) {
+  if (mn) {
 #pragma unroll
     for (int c = 0; c < kRows / 64; ++c) tma_load_3d<kCtas>(dst + c * 8192, map, bar, r0 + c * 64, k0, z);
   } else {
@@ -116,16 +123,13 @@ __device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap* ma
 }
 // MN-major, 128-byte swizzle: a chunk of 64 rows is 64 k-lines of 128 bytes, 8 lines are a swizzle atom.  Leading
 // byte offset (bits 16-29): from a chunk to the next, 8192; stride byte offset: from 8 k-lines to the next, 1024.
-template <bool kMN>
-__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
-  uint64_t d = make_smem_desc(addr);
-  if (kMN) d |= (uint64_t)(8192 >> 4) << 16;
-  return d;
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn) {
+  return make_smem_desc(addr) | (mn ? (uint64_t)(8192 >> 4) << 16 : 0ull);
 }
 // kind::f16: D fp32, A and B fp16 (0) or bf16 (1) at bits 7-9 and 10-12, bits 15 / 16: A / B is MN-major
 template <class C>
-__device__ __forceinline__ uint32_t idesc16(int bf16) {
-  return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | (C::kAMN ? 1u << 15 : 0u) | (C::kBMN ? 1u << 16 : 0u)
+__device__ __forceinline__ uint32_t idesc16(const Gemm16Args& g) {
+  return (1u << 4) | ((uint32_t)g.bf16 << 7) | ((uint32_t)g.bf16 << 10) | ((uint32_t)(g.a_mn != 0) << 15) | ((uint32_t)(g.b_mn != 0) << 16)
          | ((uint32_t)(C::kN >> 3) << 17) | ((uint32_t)(C::kM >> 4) << 24);
 }
 template <int kCtas>
@@ -144,15 +148,157 @@ __device__ __forceinline__ void commit16(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// An epilogue is a struct with Params, a constructor (params, args, tile, row, half) and
-//   chunk(v, col)   32 sums of the row, from column col of the result on (row and col may lie outside)
-//   end()           after the last chunk of the row's half tile
+// Wait until the launches before this one are complete and their writes visible, then let the next one start its set-up.
+__device__ __forceinline__ void pdl_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// hi and lo plane of a value that is scaled already
+__device__ __forceinline__ void split16(float v, __half& hi, __half& lo) {
+  hi = __float2half_rn(v);
+  lo = __float2half_rn(v - __half2float(hi));
+}
+__device__ __forceinline__ uint32_t pack_half2(__half a, __half b) {
+  return (uint32_t)__half_as_ushort(a) | ((uint32_t)__half_as_ushort(b) << 16);
+}
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+
+enum : int { kFmtF16 = 0, kFmtBF16 = 1, kFmtPlanes = 2 };      // fp16, bf16, hi and lo planes of fp16
+
+// An epilogue warp's way to global memory: its 4 KB of shared memory.  v: 32 columns from col on of this lane's row of the
+// 32 rows from row on.
+struct OutStage {
+  uint32_t addr;
+  float* f;
+  int lane;
+  uint32_t turn = 0;
+
+  // The buffer that the next store uses, free again: one of two for one plane, the whole for two.
+  __device__ __forceinline__ uint32_t acquire(bool two) {
+    if (lane == 0) {
+      if (two) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      else asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    }
+    __syncwarp();
+    const uint32_t a = two ? addr : addr + (turn & 1u) * 2048u;
+    ++turn;
+    return a;
+  }
+  __device__ __forceinline__ void store_box(uint32_t src, const CUtensorMap* map, int x, int y, int z, bool two) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane == 0) {
+      asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+                   ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(src) : "memory");
+      if (two)
+        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+                     ::"l"(map), "r"(x), "r"(y), "r"(z + 1), "r"(src + 2048u) : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+  }
+  // 32 x 32 box, rows of 64 bytes, 64-byte swizzle (16-byte piece j of row r lies at j ^ ((r / 2) % 4)): free of bank conflicts.
+  // What lies outside the map is not written.
+  template <int fmt>
+  __device__ __forceinline__ void store(const CUtensorMap* map, const float (&v)[32], int row, int col, int z, bool mirror) {
+    constexpr bool two = fmt == kFmtPlanes;
+    uint32_t a = acquire(two);
+    const uint32_t mine = a + (uint32_t)lane * 64u, sw = ((uint32_t)lane >> 1) & 3u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t h[4], l[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pair<fmt>(v[8 * j + 2 * i], v[8 * j + 2 * i + 1], h[i], l[i]);
+      const uint32_t to = mine + (((uint32_t)j ^ sw) << 4);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+      if (two) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 2048u), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]) : "memory");
+    }
+    store_box(a, map, col, row, z, two);
+    if (!mirror) return;
+    // the transposed box: row j holds column j, this lane's element
+    a = acquire(two);
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      uint32_t h, l;
+      pair<fmt>(v[j], v[j + 1], h, l);
+      const uint32_t to = a + (uint32_t)j * 64u + ((((uint32_t)lane >> 3) ^ (((uint32_t)j >> 1) & 3u)) << 4) + ((uint32_t)lane & 7u) * 2u;
+      asm volatile("st.shared.b16 [%0], %1;" ::"r"(to), "h"((uint16_t)h) : "memory");
+      asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + 64u), "h"((uint16_t)(h >> 16)) : "memory");
+      if (two) {
+        asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + 2048u), "h"((uint16_t)l) : "memory");
+        asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + 2112u), "h"((uint16_t)(l >> 16)) : "memory");
+      }
+    }
+    store_box(a, map, row, col, z, two);
+  }
+  // two neighbouring values in the format's halves, and their low planes
+  template <int fmt>
+  static __device__ __forceinline__ void pair(float x, float y, uint32_t& h, uint32_t& l) {
+    if constexpr (fmt == kFmtBF16) {
+      const __nv_bfloat162 t = __floats2bfloat162_rn(x, y);
+      h = *reinterpret_cast<const uint32_t*>(&t);
+      l = 0;
+    } else {
+      const __half2 t = __floats2half2_rn(x, y);
+      h = *reinterpret_cast<const uint32_t*>(&t);
+      l = 0;
+      if constexpr (fmt != kFmtPlanes) return;
+      const float2 b = __half22float2(t);
+      const __half2 u = __floats2half2_rn(x - b.x, y - b.y);
+      l = *reinterpret_cast<const uint32_t*>(&u);
+    }
+  }
+  // Results of any stride and alignment: f(r, v) for r = 0..31 with v = row r's value of column `lane`, so that a warp's
+  // accesses are pieces of one row.  The exclusive or keeps both directions free of bank conflicts.
+  template <class F>
+  __device__ __forceinline__ void by_rows(const float (&v)[32], F f) {
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) f32(lane, j) = v[j];
+    __syncwarp();
+    f([&](int r) { return f32(r, lane); });
+  }
+  __device__ __forceinline__ float& f32(int r, int c) { return f[r * 32 + (c ^ r)]; }
+  __device__ __forceinline__ void drain() {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+};
+
+// 32 sums of the half tile from column c on: from TMEM, or from the registers that they were added up in
+template <int kHalf>
+struct SumsInTmem {
+  uint32_t taddr;
+  __device__ __forceinline__ void load(int c, float (&v)[32]) const {
+    uint32_t r[32];
+    tmem_load_32x32(taddr + (uint32_t)c, r);
+    tmem_load_wait();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+  }
+};
+template <int kHalf>
+struct SumsInRegisters {
+  const float (&sum)[kHalf];
+  __device__ __forceinline__ void load(int c, float (&v)[32]) const {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      v[j] = sum[c + j];
+      asm volatile("" : "+f"(v[j]));       // what is made of these 32 is not begun before the 32 before them are out: registers
+    }
+  }
+};
+
+// An epilogue is a struct with Params and
+//   run<kPlanes, kHalf>(params, args, tile, row, col, half, stage, sums, done)
+// row: the first of the warp's 32 rows, col: the first of its kHalf columns (either may lie outside the result); done() is
+// called after the last load of sums.
 template <class C, class Epi>
 __global__ void __launch_bounds__(kG16Threads, 1)
 gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ typename Epi::Params ep) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(stages + C::kStages * C::kStageBytes);
+  uint8_t* outs = stages + C::kStages * C::kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(outs + 8 * kStageOut);
   uint64_t *empty = full + C::kStages, *tfull = empty + C::kStages, *tempty = tfull + 2;
   uint32_t* tmem_base = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile uint32_t* abort_flag = tmem_base + 1;
@@ -180,7 +326,10 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
   if (C::kCtas == 2) cluster_sync_all();       // the peer's barriers are ready before anything is signalled there
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tmem_base;
+  pdl_wait();
 
+  if (warp < kG16Epi) {
+  if constexpr (C::kPromote) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");    // 384 x 168 registers at launch = 128 x 56 + 256 x 224
   if (warp == 0 && lane == 0) {
     uint32_t it = 0;
     for (int t = first; t < ntiles && !*abort_flag; t += step) {
@@ -194,8 +343,8 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
         const uint32_t sa = smem_u32(stages + st * C::kStageBytes), sb = sa + C::kPlanes * C::kABytes;
 #pragma unroll
         for (int p = 0; p < C::kPlanes; ++p) {
-          load_operand<C::kCtas, C::kAMN, 128>(sa + p * C::kABytes, &g.a, bar, g.a_k0 + kb * kG16K, am, w.z * g.a_z + p);
-          load_operand<C::kCtas, C::kBMN, C::kBRows>(sb + p * C::kBBytes, &g.b, bar, g.b_k0 + kb * kG16K, bn, w.z * g.b_z + p);
+          load_operand<C::kCtas, 128>(sa + p * C::kABytes, &g.a, bar, g.a_k0 + kb * kG16K, am, w.z * g.a_z + p, g.a_mn);
+          load_operand<C::kCtas, C::kBRows>(sb + p * C::kBBytes, &g.b, bar, g.b_k0 + kb * kG16K, bn, w.z * g.b_z + p, g.b_mn);
         }
       }
     }
@@ -203,7 +352,9 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
     for (uint32_t u = it > (uint32_t)C::kStages ? it - C::kStages : 0; u < it && !*abort_flag; ++u)
       if (!mbar_wait(&empty[u % C::kStages], (u / C::kStages) & 1)) *abort_flag = 1;
   } else if (warp == 1 && lane == 0 && rank == 0) {
-    const uint32_t idesc = idesc16<C>(g.bf16);
+    const uint32_t idesc = idesc16<C>(g);
+    // 16 elements of K: 32 bytes of a K-major row, 16 lines of 128 bytes MN-major
+    const uint64_t ka = g.a_mn ? 2048 >> 4 : 32 >> 4, kb_ = g.b_mn ? 2048 >> 4 : 32 >> 4;
     uint32_t it = 0, n = 0;
     for (int t = first; t < ntiles && !*abort_flag; t += step) {
       const Tile16 w = tile16<C>(g, t);
@@ -221,11 +372,11 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
           const uint32_t sa = smem_u32(stages + st * C::kStageBytes), sb = sa + C::kPlanes * C::kABytes;
 #pragma unroll
           for (int q = 0; q < (C::kPlanes == 2 ? 3 : 1); ++q) {      // hi·lo, lo·hi, hi·hi
-            const uint64_t da = operand_desc<C::kAMN>(sa + (q == 1 ? C::kABytes : 0));
-            const uint64_t db = operand_desc<C::kBMN>(sb + (C::kPlanes == 2 && q == 0 ? C::kBBytes : 0));
+            const uint64_t da = operand_desc(sa + (q == 1 ? C::kABytes : 0), g.a_mn);
+            const uint64_t db = operand_desc(sb + (C::kPlanes == 2 && q == 0 ? C::kBBytes : 0), g.b_mn);
 #pragma unroll
-            for (int k = 0; k < kG16K / 16; ++k) {     // 16 elements of K: 32 bytes of a K-major row, 16 MN-major lines
-              mma16<C::kCtas>(d, da + (uint64_t)(k * (C::kAMN ? 2048 : 32) >> 4), db + (uint64_t)(k * (C::kBMN ? 2048 : 32) >> 4), idesc, accumulate);
+            for (int k = 0; k < kG16K / 16; ++k) {
+              mma16<C::kCtas>(d, da + k * ka, db + k * kb_, idesc, accumulate);
               accumulate = 1;
             }
           }
@@ -234,9 +385,13 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
         commit16<C::kCtas>(&tfull[acc]);
       }
     }
-  } else if (warp >= 2) {
+  }
+  } else {
+    if constexpr (C::kPromote) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     constexpr int kHalf = C::kN / 2;
-    const int q = warp & 3, half = (warp - 2) >> 2;
+    const int q = warp & 3, half = (warp - kG16Epi) >> 2;
+    uint8_t* mine = outs + (warp - kG16Epi) * kStageOut;
+    OutStage stage{smem_u32(mine), reinterpret_cast<float*>(mine), lane};
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * kHalf);
     uint32_t n = 0;
     // warp-uniform, as the TMEM loads are warp-collective
@@ -264,51 +419,35 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
     bool ok = true;
     for (int t = first; t < ntiles && ok; t += step) {
       const Tile16 w = tile16<C>(g, t);
-      const int row = w.m0 + rank * 128 + q * 32 + lane, col = w.n0 + half * kHalf;
+      const int row = w.m0 + rank * 128 + q * 32, col = w.n0 + half * kHalf;
       if constexpr (C::kPromote) {
         float sum[kHalf];
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j) sum[j] = 0.f;
         for (int kc = w.kb0; kc < w.kb1; kc += C::kChunk, ++n) {
           const uint32_t acc = n & 1u;
           if (!(ok = sums_ready(acc, (n >> 1) & 1))) break;
+uint32_t r[2][32];
+          tmem_load_32x32(lanes + acc * (uint32_t)C::kN, r[0]);
 #pragma unroll
-          for (int c = 0; c < kHalf; c += 32) {
-            uint32_t r[32];
-            tmem_load_32x32(lanes + acc * (uint32_t)C::kN + (uint32_t)c, r);
+          for (int c = 0; c < kHalf; c += 32) {      // the next load is on its way while these are added
             tmem_load_wait();
+            if (c + 32 < kHalf) tmem_load_32x32(lanes + acc * (uint32_t)C::kN + (uint32_t)c + 32u, r[(c / 32 + 1) & 1]);
+            else release(acc);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sum[c + j] = kc == w.kb0 ? __uint_as_float(r[j]) : sum[c + j] + __uint_as_float(r[j]);
+            for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(r[(c / 32) & 1][j]);
           }
-          release(acc);
         }
         if (!ok) break;
-        Epi epi(ep, g, w, row, half);
-#pragma unroll
-        for (int c = 0; c < kHalf; c += 32) {
-          float v[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = sum[c + j];
-          epi.chunk(v, col + c);
-        }
-        epi.end();
+        Epi::template run<C::kPlanes, kHalf>(ep, g, w, row, col, half, stage, SumsInRegisters<kHalf>{sum}, [] {});
       } else {
         const uint32_t acc = n & 1u;
         if (!(ok = sums_ready(acc, (n >> 1) & 1))) break;
         ++n;
-        Epi epi(ep, g, w, row, half);
-#pragma unroll 1
-        for (int c = 0; c < kHalf; c += 32) {
-          uint32_t r[32];
-          tmem_load_32x32(lanes + acc * (uint32_t)C::kN + (uint32_t)c, r);
-          tmem_load_wait();
-          if (c + 32 >= kHalf) release(acc);
-          float v[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-          epi.chunk(v, col + c);
-        }
-        epi.end();
+        Epi::template run<C::kPlanes, kHalf>(ep, g, w, row, col, half, stage, SumsInTmem<kHalf>{lanes + acc * (uint32_t)C::kN}, [&] { release(acc); });
       }
     }
+    stage.drain();
   }
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -327,16 +466,6 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
   }
 }
 
-// hi and lo plane of a value that is scaled already
-__device__ __forceinline__ void split16(float v, __half& hi, __half& lo) {
-  hi = __float2half_rn(v);
-  lo = __float2half_rn(v - __half2float(hi));
-}
-__device__ __forceinline__ uint32_t pack_half2(__half a, __half b) {
-  return (uint32_t)__half_as_ushort(a) | ((uint32_t)__half_as_ushort(b) << 16);
-}
-__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-
 }  // namespace psb
 
 namespace {
@@ -353,15 +482,16 @@ int sm_count(int* dev_out) {
 }
 
 // Map over `count` row-major 16-bit matrices of [rows][cols], row stride ld elements, matrix stride `stride` elements;
-// the box is 64 columns of box_rows rows.  0, a driver error, or -1 without the driver's entry point.
-int make_map16(CUtensorMap* map, const void* base, int bf16, int64_t rows, int64_t cols, int64_t ld, int64_t stride, int count, int box_rows) {
+// the box is 64 columns of box_rows rows, 32 of 32 for results (out).  0, a driver error, or -1 without the driver's entry point.
+int make_map16(CUtensorMap* map, const void* base, int bf16, int64_t rows, int64_t cols, int64_t ld, int64_t stride, int count, int box_rows,
+               bool out = false) {
   EncodeTiledFn enc = get_encode();
   if (!enc) return -1;
   const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)count};
   const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(count > 1 ? stride : ld * rows) * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, estr[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {out ? 32u : 64u, (cuuint32_t)box_rows, 1}, estr[3] = {1, 1, 1};
   return (int)enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box,
-                  estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  estr, CU_TENSOR_MAP_INTERLEAVE_NONE, out ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
@@ -372,13 +502,47 @@ struct Operand16 {
   int count;                          // matrices in the map
 };
 
+int make_out_map(CUtensorMap* map, const Operand16& o, int bf16) {
+  return make_map16(map, o.base, bf16, o.rows, o.cols, o.ld, o.stride, o.count, 32, true);
+}
+
+// A launch of a call: every one after the first may start its set-up before its predecessor is complete.
+struct Chain {
+  cudaStream_t stream;
+  bool started = false;
+  template <class... P, class... A>
+  int launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, int cluster, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[2];
+    int n = 0;
+    if (cluster > 1) {
+      at[n].id = cudaLaunchAttributeClusterDimension;
+      at[n].val.clusterDim.x = (unsigned)cluster; at[n].val.clusterDim.y = 1; at[n].val.clusterDim.z = 1;
+      ++n;
+    }
+    if (started) {
+      at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      at[n].val.programmaticStreamSerializationAllowed = 1;
+      ++n;
+    }
+    cfg.attrs = at;
+    cfg.numAttrs = (unsigned)n;
+    started = true;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, (P)args...);
+  }
+};
+
 template <class C, class Epi>
-int launch16(psb::Gemm16Args g, const Operand16& a, const Operand16& b, const typename Epi::Params& ep, cudaStream_t stream) {
+int launch16(Chain& chain, psb::Gemm16Args& g, const Operand16& a, const Operand16& b, const typename Epi::Params& ep) {
   int dev = 0;
   const int sms = sm_count(&dev);
   if (sms <= 0) return (int)cudaErrorInvalidDevice;
-  int r = make_map16(&g.a, a.base, g.bf16, a.rows, a.cols, a.ld, a.stride, a.count, C::kAMN ? 64 : 128);
-  if (r == 0) r = make_map16(&g.b, b.base, g.bf16, b.rows, b.cols, b.ld, b.stride, b.count, C::kBMN ? 64 : C::kBRows);
+  int r = make_map16(&g.a, a.base, g.bf16, a.rows, a.cols, a.ld, a.stride, a.count, g.a_mn ? 64 : 128);
+  if (r == 0) r = make_map16(&g.b, b.base, g.bf16, b.rows, b.cols, b.ld, b.stride, b.count, g.b_mn ? 64 : C::kBRows);
   if (r) return r;
   static bool attr[kMaxDevices] = {};
   if (!attr[dev]) {
@@ -387,17 +551,52 @@ int launch16(psb::Gemm16Args g, const Operand16& a, const Operand16& b, const ty
     attr[dev] = true;
   }
   const int tiles = psb::tiles16<C>(g), most = sms / C::kCtas;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((tiles < most ? tiles : most) * C::kCtas));
-  cfg.blockDim = dim3(psb::kG16Threads);
-  cfg.dynamicSmemBytes = C::kSmemBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = C::kCtas; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = C::kCtas == 2 ? 1 : 0;
-  return (int)cudaLaunchKernelEx(&cfg, psb::gemm16_kernel<C, Epi>, g, ep);
+  return chain.launch(psb::gemm16_kernel<C, Epi>, dim3((unsigned)((tiles < most ? tiles : most) * C::kCtas)), psb::kG16Threads, C::kSmemBytes, C::kCtas, g, ep);
+}
+
+// ---- which tiles, and in how many pieces K is taken
+enum : int { kPair256 = 0, kOne128 = 1, kOne64 = 2 };      // 256x256 on a pair, 128x128, 128x64
+struct Tiling { int kind, splits, kb_split; };
+
+inline int tiling_rows(int kind) { return kind == kPair256 ? 256 : 128; }
+inline int tiling_cols(int kind) { return kind == kPair256 ? 256 : kind == kOne128 ? 128 : 64; }
+
+// The cheapest by this estimate, in cycles of an SM: rounds of tiles, each its blocks of K at the slower of the tensor
+// cores (128 x N x 64 in 2N cycles a product, as a rule) and the loads (48 bytes a cycle from L2, as measured with all SMs
+// busy), plus what does not overlap in the last round, plus storing and adding up the pieces of K (at 3000 bytes a cycle).
+inline Tiling choose_tiling(int64_t batch, int64_t M, int64_t N, int64_t K, int planes, bool sym, int max_splits, int only = -1) {
+  const int64_t nkb = (K + psb::kG16K - 1) / psb::kG16K;
+  Tiling best = {kOne64, 1, (int)nkb};
+  double least = 1e300;
+  for (int kind = 0; kind < 3; ++kind) {
+    if ((only >= 0 && kind != only) || (sym && kind == kOne64)) continue;
+    const int64_t rows = tiling_rows(kind), cols = tiling_cols(kind);
+    const int64_t tm = (M + rows - 1) / rows, tn = (N + cols - 1) / cols, slots = kind == kPair256 ? 74 : 148;
+    const int64_t tiles = batch * (sym ? tm * (tm + 1) / 2 : tm * tn);
+    const double mma = 2.0 * cols * (planes == 2 ? 3 : 1);
+    const double load = planes * (kind == kPair256 ? 32768.0 : 16384.0 + 128.0 * cols) / 48.0;
+    for (int64_t s = 1; s <= max_splits && s <= nkb; ++s) {
+      const int64_t per = (nkb + s - 1) / s, real = (nkb + per - 1) / per;
+      if (real != s) continue;
+      if (s > 1 && per < 4) break;
+      const int64_t rounds = (tiles * s + slots - 1) / slots;
+      double t = (double)rounds * (double)per * (mma > load ? mma : load) + 12.0 * (double)cols + 600.0 * (double)rounds;
+      if (s > 1) t += 4500.0 + (double)batch * M * N * (8.0 * s + 4.0) / 3000.0;
+      if (t < least) { least = t; best = {kind, (int)s, (int)per}; }
+    }
+  }
+  return best;
+}
+
+template <int kPlanes, class Epi>
+int launch_tiled(Chain& chain, int kind, psb::Gemm16Args& g, const Operand16& a, const Operand16& b, const typename Epi::Params& ep) {
+  if (kind == kPair256) return launch16<psb::Cfg16<2, 256, kPlanes>, Epi>(chain, g, a, b, ep);
+  if (kind == kOne128) return launch16<psb::Cfg16<1, 128, kPlanes>, Epi>(chain, g, a, b, ep);
+  return launch16<psb::Cfg16<1, 64, kPlanes>, Epi>(chain, g, a, b, ep);
+}
+template <class Epi>
+int product16(Chain& chain, int planes, int kind, psb::Gemm16Args& g, const Operand16& a, const Operand16& b, const typename Epi::Params& ep) {
+  return planes == 2 ? launch_tiled<2, Epi>(chain, kind, g, a, b, ep) : launch_tiled<1, Epi>(chain, kind, g, a, b, ep);
 }
 
 }  // namespace

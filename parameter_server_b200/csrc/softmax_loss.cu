@@ -4,134 +4,158 @@
 //   G_ij = c_i (e^{s_ij − lse_i} − [j = y_i])        gx = G w        gw = Gᵀ x
 //
 // The scores are tiles of a product on the tensor cores (gemm16.cuh) and never leave the SM: its epilogue keeps each row's
-// running maximum m and sum Σ e^{s−m} over the tile's classes, and the score of the row's label; a second, small kernel
-// joins the tiles of a row.  The gradient takes the classes in pieces: the piece's scores are made again, turned into G
-// (which is kept for one piece only, in the type of the operands) and multiplied with the piece of w and with x.  gw of a
-// piece is complete, gx is summed over the pieces in fp32.  Sums have a fixed order: results do not vary from run to run.
+// maximum m and sum Σ e^{s−m} over half a tile's classes, and the score of the row's label.  A second kernel joins the
+// halves of a row to its log-sum-exp.
 //
-// Scores, maxima, sums and losses are fp32 (in units of log2 e: 2^x is the hardware's exponential).  G is rounded to the
-// operands' type: bf16 for bf16; fp16 for fp16, scaled by a power of two so that the largest coefficient is near 2^13;
-// two planes of fp16 for fp32, where x and w are such planes too (22 bits).
+// For the gradients the epilogue also writes e^{s−m} · 2^15 in fp16 (relative to the half tile's own maximum, which is all
+// that is known then), for as many classes as the workspace holds; the second kernel turns it into G in place, with one
+// factor a half tile.  Making the scores once costs 6nVd operations instead of 8nVd, for a pass over 2 bytes an element
+// (8192 rows, 131,072 classes, 2048 wide: 3.5 ms less for 0.7).  Classes beyond the workspace come in pieces, whose scores
+// are made again.  gw of a piece is complete, gx is summed over the pieces in fp32.  Sums have a fixed order: results do not
+// vary from run to run.
+//
+// Scores, maxima, sums and losses are fp32 (in units of log2 e: 2^x is the hardware's exponential).  The exponentials keep 11
+// bits (two planes for fp32: 22); the label's entry of G, where they would cancel, is made from the label's score in fp32.
+// G is rounded to the operands' type: bf16 for bf16; fp16 for fp16, scaled by a power of two so that the largest
+// coefficient is near 2^13; two planes of fp16 for fp32, where x and w are such planes too.
 #include "gemm16.cuh"
 
 namespace psb {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kExpScale = 15;                 // exponentials relative to their maximum are kept times 2^15
 
 enum : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
 
-// device scalars of a call: largest finite |x|, |w|, |c| as bits; then the exponents derived from them
-struct LossScal {
-  uint32_t max_x, max_w, max_c, pad;
+// Exponents of the operands' scales: x and w are multiplied by 2^x and 2^w, G by 2^g.
+struct Scales { int x, w, g; };
+// They are 0 for 16-bit operands and g is known where there are no coefficients; else the device finds them.
+struct ScaleRef {
+  Scales fixed;
+  const Scales* found;         // null: as fixed
+  __device__ __forceinline__ Scales get() const { return found != nullptr ? *found : fixed; }
 };
-// exponent that brings the largest finite magnitude into [2^top, 2^(top+1))
+// exponent that brings the magnitude with these bits into [2^top, 2^(top+1)); subnormals count as 2^-127, as the scale only
+// has to be representable
 __device__ __forceinline__ int scale_exp(uint32_t bits, int top) {
   if (bits == 0) return 0;
-  const int e = (int)(bits >> 23) - 127;             // subnormals count as 2^-127: the scale only has to be representable
-  const int k = top - e;
+  const int k = top - ((int)(bits >> 23) - 127);
   return k > 126 ? 126 : k;
 }
-__device__ __forceinline__ float pow2i(int e) {       // 2^e, kept finite and normal
+__device__ __forceinline__ float pow2i(int e) {       // 2^e, kept finite; 0 below the normal numbers
   e = e > 127 ? 127 : e;
   return e < -126 ? 0.f : __int_as_float((e + 127) << 23);
 }
-struct Scales { int x, w, g; };
-// fp32: planes use the whole range of fp16; 16-bit types are taken as they are, and fp16 gradients are scaled
-__device__ __forceinline__ Scales scales_of(const LossScal* s, int dtype) {
-  Scales k{0, 0, 0};
-  if (dtype == kF32) { k.x = scale_exp(s->max_x, 14); k.w = scale_exp(s->max_w, 14); }
-  if (dtype != kBF16) k.g = scale_exp(s->max_c, 13);
-  return k;
-}
+__device__ __forceinline__ float score_scale(const ScaleRef& r) { const Scales k = r.get(); return kLog2e * pow2i(-(k.x + k.w)); }
+__device__ __forceinline__ float grad_scale(const ScaleRef& r, int with_w) { const Scales k = r.get(); return pow2i(-(k.g + (with_w ? k.w : k.x))); }
+__device__ __forceinline__ bool has_class(int64_t y, int V) { return y >= 0 && y < V; }
 
 // ------------------------------------------------------------------ preparation
 __device__ __forceinline__ uint32_t finite_bits(float v) {
   const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
   return b < 0x7F800000u ? b : 0u;
 }
-__device__ __forceinline__ uint32_t block_max_u32(uint32_t v) {
-  __shared__ uint32_t sh[32];
+__device__ __forceinline__ uint32_t block_max_u32(uint32_t v) {       // of 256 threads, in all of them
+  __shared__ uint32_t sh[8];
   v = __reduce_max_sync(0xffffffffu, v);
+  __syncthreads();
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = threadIdx.x < (blockDim.x >> 5) ? sh[threadIdx.x] : 0u;
-  if (threadIdx.x < 32) v = __reduce_max_sync(0xffffffffu, v);
-  return v;
+  v = sh[threadIdx.x & 7];
+  return __reduce_max_sync(0xffffffffu, v);
 }
-__device__ __forceinline__ bool has_class(int64_t y, int V) { return y >= 0 && y < V; }
-
-// Labels as int32 (-1: none), coefficients (0 where there is no class), the largest coefficient.  A label outside the classes
-// is recorded in the status word and counts as none.
-__global__ void __launch_bounds__(256)
-k_loss_labels(const int64_t* __restrict__ y, const float* __restrict__ coef, int n, int V, int* __restrict__ label, float* __restrict__ c,
-              LossScal* scal, uint32_t* status) {
+__device__ __forceinline__ uint32_t coef_max(const float* coef, const int64_t* y, int n, int V) {
+  if (coef == nullptr) return __float_as_uint(1.f);
   uint32_t top = 0;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) {
-    const int64_t v = y[i];
-    const bool ok = has_class(v, V);
-    if (v != -1 && !ok) set_status(status, kBadIndex, (uint32_t)i, (uint32_t)v);
-    label[i] = ok ? (int)v : -1;
-    const float cv = ok ? (coef != nullptr ? coef[i] : 1.f) : 0.f;
-    c[i] = cv;
-    top = max(top, finite_bits(cv));
-  }
-  top = block_max_u32(top);
-  if (threadIdx.x == 0 && top != 0) atomicMax(&scal->max_c, top);
+  for (int i = threadIdx.x; i < n; i += 256)
+    if (has_class(y[i], V)) top = max(top, finite_bits(coef[i]));
+  return block_max_u32(top);
+}
+// fp16 with coefficients: the scale of G alone (one block)
+__global__ void __launch_bounds__(256)
+k_loss_coef(const float* __restrict__ coef, const int64_t* __restrict__ y, int n, int V, Scales* out) {
+  pdl_wait();
+  const uint32_t top = coef_max(coef, y, n, V);
+  if (threadIdx.x == 0) *out = Scales{0, 0, scale_exp(top, 13)};
 }
 
-// Largest finite magnitude of fp32 rows; rows without a class do not count (y null: all rows do).
+// Largest finite magnitudes of fp32 operands, a block's each: blocks 0..bx-1 take x (rows without a class do not count),
+// the others w.
 __global__ void __launch_bounds__(256)
-k_loss_absmax(const float* __restrict__ a, int64_t rows, int cols, int64_t ld, const int64_t* __restrict__ y, int V, uint32_t* out) {
+k_loss_absmax(const float* __restrict__ x, int64_t ldx, const float* __restrict__ w, int64_t ldw, int n, int V, int d,
+              const int64_t* __restrict__ y, int bx, uint32_t* __restrict__ out) {
+  pdl_wait();
+  const bool is_x = (int)blockIdx.x < bx;
+  const float* a = is_x ? x : w;
+  const int64_t ld = is_x ? ldx : ldw, rows = is_x ? n : V, nb = is_x ? bx : gridDim.x - bx, b = is_x ? blockIdx.x : blockIdx.x - bx;
   uint32_t top = 0;
   const bool vec = ((reinterpret_cast<uintptr_t>(a) & 15) | (ld & 3)) == 0;
-  const int per = (cols + 3) / 4;
+  const int per = (d + 3) / 4;
   const int64_t total = rows * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+  for (int64_t i = b * 256 + threadIdx.x; i < total; i += nb * 256) {
     const int64_t r = i / per;
     const int c = (int)(i - r * per) * 4;
-    if (y != nullptr && !has_class(y[r], V)) continue;
+    if (is_x && !has_class(y[r], V)) continue;
     const float* p = a + r * ld + c;
-    if (vec && c + 4 <= cols) {
+    if (vec && c + 4 <= d) {
       const float4 v = *reinterpret_cast<const float4*>(p);
       top = max(max(top, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
     } else {
-      for (int j = 0; j < 4 && c + j < cols; ++j) top = max(top, finite_bits(p[j]));
+      for (int j = 0; j < 4 && c + j < d; ++j) top = max(top, finite_bits(p[j]));
     }
   }
   top = block_max_u32(top);
-  if (threadIdx.x == 0 && top != 0) atomicMax(out, top);
+  if (threadIdx.x == 0) out[blockIdx.x] = top;
 }
 
-// Rows of any stride and alignment into operand planes [plane][row][ldo]; rows without a class become zeros, whatever they
-// held (y null: none do).  which: 0 = x, 1 = w, the exponent that scales fp32.
+struct PackArgs {
+  const void* a;               // rows of `cols` elements, any stride and alignment
+  int64_t rows, ld;
+  uint16_t* out;               // operand planes [plane][row][ldo]
+  int64_t ldo, plane;
+};
+// Operands into planes of their own: blocks 0..bx-1 pack x, the others w (either may have no blocks).  Rows of x without a
+// class become zeros, whatever they held.  fp32: the scales come from the blocks' maxima and are written for those who follow.
 template <typename T>
 __global__ void __launch_bounds__(256)
-k_loss_pack(const T* __restrict__ a, int64_t rows, int cols, int64_t ld, const int64_t* __restrict__ y, int V, uint16_t* __restrict__ out,
-            int64_t ldo, int64_t plane, const LossScal* scal, int which) {
-  const int per = (int)(ldo / 8);
-  const int64_t total = rows * per;
+k_loss_pack(PackArgs px, PackArgs pw, int cols, const int64_t* __restrict__ y, int n, int V, const float* __restrict__ coef, int bx,
+            const uint32_t* __restrict__ maxima, int mx, int mw, Scales* found) {
+  pdl_wait();
+  const bool is_x = (int)blockIdx.x < bx;
+  const PackArgs& p = is_x ? px : pw;
+  const int64_t nb = is_x ? bx : gridDim.x - bx, b = is_x ? blockIdx.x : blockIdx.x - bx;
   float s = 1.f;
   if (sizeof(T) == 4) {
-    const Scales k = scales_of(scal, kF32);
-    s = pow2i(which ? k.w : k.x);
+    uint32_t tx = 0, tw = 0;
+    if (is_x || blockIdx.x == gridDim.x - 1) for (int i = threadIdx.x; i < mx; i += 256) tx = max(tx, maxima[i]);
+    if (!is_x) for (int i = threadIdx.x; i < mw; i += 256) tw = max(tw, maxima[mx + i]);
+    const int kx = scale_exp(block_max_u32(tx), 14), kw = scale_exp(block_max_u32(tw), 14);
+    s = pow2i(is_x ? kx : kw);
+    if (blockIdx.x == gridDim.x - 1) {
+      const uint32_t tc = coef_max(coef, y, n, V);
+      if (threadIdx.x == 0) *found = Scales{kx, kw, scale_exp(tc, 13)};
+    }
   }
-  const bool vec = ((reinterpret_cast<uintptr_t>(a) & 15) | ((ld * sizeof(T)) & 15)) == 0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+  const T* a = reinterpret_cast<const T*>(p.a);
+  const int per = (int)(p.ldo / 8);
+  const int64_t total = p.rows * per;
+  const bool vec = ((reinterpret_cast<uintptr_t>(a) & 15) | ((p.ld * sizeof(T)) & 15)) == 0;
+  for (int64_t i = b * 256 + threadIdx.x; i < total; i += nb * 256) {
     const int64_t r = i / per;
     const int c = (int)(i - r * per) * 8;
-    const T* p = a + r * ld + c;
-    const bool none = y != nullptr && !has_class(y[r], V);
+    const T* src = a + r * p.ld + c;
     alignas(16) T v[8];
-    if (none) {
+    if (is_x && !has_class(y[r], V)) {
+#pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = T(0);
     } else if (vec && c + 8 <= cols) {
 #pragma unroll
-      for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(v)[j] = reinterpret_cast<const uint4*>(p)[j];
+      for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(v)[j] = reinterpret_cast<const uint4*>(src)[j];
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? p[j] : T(0);
+      for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? src[j] : T(0);
     }
-    uint16_t* dst = out + r * ldo + c;
+    uint16_t* dst = p.out + r * p.ldo + c;
     if constexpr (sizeof(T) == 4) {
       uint32_t h[4], l[4];
 #pragma unroll
@@ -142,7 +166,7 @@ k_loss_pack(const T* __restrict__ a, int64_t rows, int cols, int64_t ld, const i
         h[j] = pack_half2(h0, h1); l[j] = pack_half2(l0, l1);
       }
       *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
-      *reinterpret_cast<uint4*>(dst + plane) = make_uint4(l[0], l[1], l[2], l[3]);
+      *reinterpret_cast<uint4*>(dst + p.plane) = make_uint4(l[0], l[1], l[2], l[3]);
     } else {
       *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(v);
     }
@@ -150,114 +174,108 @@ k_loss_pack(const T* __restrict__ a, int64_t rows, int cols, int64_t ld, const i
 }
 
 // ------------------------------------------------------------------ epilogues
-// Each row's maximum and Σ 2^(s−m) over half a tile's classes, and the score of its label, in units of log2 e.
+// Each row's maximum and Σ 2^(s−m) over half a tile's classes, the score of its label, in units of log2 e, and the
+// exponentials that are kept.
 struct EpiScore {
   struct Params {
-    float2* part;              // [2 · class tiles][n]
+    CUtensorMap e;             // exponentials [plane][n][keep]
+    float2* part;              // [n][2 · class tiles]
     float* target;             // [n]
-    const int* label;
-    const LossScal* scal;
-    int n, V, dtype;
+    const int64_t* y;
+    ScaleRef scale;
+    int n, V, parts, keep;
   };
-  const Params& p;
-  float scale, m, s;
-  int row, lab;
-  int64_t at;
-  __device__ __forceinline__ EpiScore(const Params& p_, const Gemm16Args&, const Tile16& w, int row_, int half)
-      : p(p_), m(-INFINITY), s(0.f), row(row_), lab(-2) {
-    const Scales k = scales_of(p.scal, p.dtype);
-    scale = kLog2e * pow2i(-(k.x + k.w));
-    if (row < p.n) lab = p.label[row];
-    at = (int64_t)(w.tn * 2 + half) * p.n + row;
-  }
-  __device__ __forceinline__ void chunk(float (&v)[32], int col) {
-    if (col >= p.V) return;
+  template <int kPlanes, int kHalf, class Sums, class Done>
+  static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int half, OutStage& st,
+                                             const Sums& sums, Done done) {
+    const float scale = score_scale(p.scale);
+    const int row = row0 + st.lane;
+    int64_t lab = -1;
+    if (row < p.n) lab = p.y[row];
     float top = -INFINITY;
-    const int left = p.V - col;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      v[j] *= scale;
-      if (left < 32) v[j] = j < left ? v[j] : -INFINITY;
+    for (int c = 0; c < kHalf; c += 32) {
+      float v[32];
+      sums.load(c, v);
+      const int left = p.V - (col0 + c);
+      if (left >= 32) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) top = fmaxf(top, v[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) top = j < left ? fmaxf(top, v[j]) : top;
+      }
     }
-    if ((unsigned)(lab - col) < 32u) {
-      float t = 0.f;
+    // without a finite score the reference is 0: 2^(-inf) is 0 and nothing is subtracted from an infinity
+    const float m = __fmul_rn(top, scale), ref = top == -INFINITY ? 0.f : m;
+    float s = 0.f;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) t = j == lab - col ? v[j] : t;
-      p.target[row] = t;
+    for (int c = 0; c < kHalf; c += 32) {
+      float v[32];
+      sums.load(c, v);
+      if (c + 32 >= kHalf) done();
+      const int col = col0 + c, left = p.V - col;
+      if (left <= 0) continue;
+      if (lab >= col && lab < col + 32 && lab < p.V) {
+        const int at = (int)(lab - col);
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) t = j == at ? v[j] : t;
+        p.target[row] = __fmul_rn(t, scale);
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        // product and difference rounded apart, as those of the maximum and of the label are: a row whose class is certain has
+        // a loss of 0, not of a rounding
+        v[j] = ex2(__fsub_rn(__fmul_rn(v[j], scale), ref));
+        if (left < 32) v[j] = j < left ? v[j] : 0.f;
+        s += v[j];
+        v[j] *= (float)(1 << kExpScale);
+      }
+      if (col < p.keep) st.store<kPlanes == 2 ? kFmtPlanes : kFmtF16>(&p.e, v, row0, col, 0, false);
     }
-#pragma unroll
-    for (int j = 0; j < 32; ++j) top = fmaxf(top, v[j]);
-    // without a finite score yet the reference is 0: 2^(-inf) is 0 and nothing is subtracted from an infinity
-    const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.f : mn;
-    float sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) sum += ex2(v[j] - ref);
-    s = s * ex2(m - ref) + sum;
-    m = mn;
-  }
-  __device__ __forceinline__ void end() {
-    if (row < p.n) p.part[at] = make_float2(m, s);
+    if (row < p.n) p.part[(int64_t)row * p.parts + w.tn * 2 + half] = make_float2(top == -INFINITY ? top : m, s);
   }
 };
 
-// G of a piece of the classes, in the operands' type
+// G of a piece of the classes, in the operands' type, from scores made again
 struct EpiG {
   struct Params {
-    uint16_t* out;             // [plane][n][ldg]
-    int64_t ldg, plane;
+    CUtensorMap g;             // [plane][n][len]
     const float* lse;          // [n], log2
-    const float* c;
-    const int* label;
-    const LossScal* scal;
-    int n, len, v0, dtype;
+    const float* coef;
+    const int64_t* y;
+    ScaleRef scale;
+    int n, V, len, v0, dtype;
   };
-  const Params& p;
-  float scale, c, lse;
-  int row, lab;
-  __device__ __forceinline__ EpiG(const Params& p_, const Gemm16Args&, const Tile16&, int row_, int)
-      : p(p_), c(0.f), lse(0.f), row(row_), lab(-1) {
-    const Scales k = scales_of(p.scal, p.dtype);
-    scale = kLog2e * pow2i(-(k.x + k.w));
-    if (row < p.n) {
-      lab = p.label[row];
+  template <int kPlanes, int kHalf, class Sums, class Done>
+  static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16&, int row0, int col0, int, OutStage& st,
+                                             const Sums& sums, Done done) {
+    const float scale = score_scale(p.scale);
+    const int row = row0 + st.lane;
+    float c = 0.f, lse = 0.f;
+    int64_t lab = -1;
+    if (row < p.n && has_class(p.y[row], p.V)) {
+      lab = p.y[row] - p.v0;
+      c = (p.coef != nullptr ? p.coef[row] : 1.f) * pow2i(p.scale.get().g);
       lse = p.lse[row];
-      c = lab >= 0 ? p.c[row] * pow2i(k.g) : 0.f;
-      lab = lab >= 0 ? lab - p.v0 : -1;
-      if (lab < 0 && p.label[row] >= 0) lab = -2;         // the row's class lies in another piece
+    }
+    const bool none = row >= p.n || !has_class(p.y[row], p.V);
+#pragma unroll
+    for (int k = 0; k < kHalf; k += 32) {
+      float v[32];
+      sums.load(k, v);
+      if (k + 32 >= kHalf) done();
+      const int col = col0 + k;
+      if (col >= p.len) continue;
+      const int at = lab >= col && lab < col + 32 ? (int)(lab - col) : -1;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = none ? 0.f : c * (ex2(fmaf(v[j], scale, -lse)) - (at == j ? 1.f : 0.f));
+      if constexpr (kPlanes == 2) st.store<kFmtPlanes>(&p.g, v, row0, col, 0, false);
+      else if (p.dtype == kBF16) st.store<kFmtBF16>(&p.g, v, row0, col, 0, false);
+      else st.store<kFmtF16>(&p.g, v, row0, col, 0, false);
     }
   }
-  __device__ __forceinline__ void chunk(float (&v)[32], int col) {
-    if (row >= p.n || col >= p.ldg) return;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      v[j] = ex2(v[j] * scale - lse);
-      v[j] = lab == -1 ? 0.f : c * (v[j] - (j == lab - col ? 1.f : 0.f));
-    }
-    uint16_t* dst = p.out + (int64_t)row * p.ldg + col;
-    const int left = (int)p.ldg - col;                     // a multiple of 8; what lies behind the piece is not read
-#pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      if (j >= left) break;
-      uint32_t h[4], l[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = v[j + 2 * i], b = v[j + 2 * i + 1];
-        if (p.dtype == kBF16) {
-          const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-          h[i] = *reinterpret_cast<const uint32_t*>(&t);
-        } else {
-          __half h0, l0, h1, l1;
-          split16(a, h0, l0);
-          split16(b, h1, l1);
-          h[i] = pack_half2(h0, h1);
-          l[i] = pack_half2(l0, l1);
-        }
-      }
-      *reinterpret_cast<uint4*>(dst + j) = make_uint4(h[0], h[1], h[2], h[3]);
-      if (p.dtype == kF32) *reinterpret_cast<uint4*>(dst + p.plane + j) = make_uint4(l[0], l[1], l[2], l[3]);
-    }
-  }
-  __device__ __forceinline__ void end() {}
 };
 
 __device__ __forceinline__ void store_as(void* out, int64_t at, float v, int dtype) {
@@ -265,127 +283,176 @@ __device__ __forceinline__ void store_as(void* out, int64_t at, float v, int dty
   else if (dtype == kBF16) reinterpret_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
   else reinterpret_cast<__half*>(out)[at] = __float2half_rn(v);
 }
-// 1 / (scale of G times scale of the other operand)
-__device__ __forceinline__ float grad_scale(const LossScal* scal, int dtype, int with_w) {
-  const Scales k = scales_of(scal, dtype);
-  return pow2i(-(k.g + (with_w ? k.w : k.x)));
-}
 
 // A gradient: to the result, or raw fp32 sums to `acc` (piece by piece, or one slot per split of K)
 struct EpiGrad {
   struct Params {
+    CUtensorMap map;           // of the result, where it is 16-bit and aligned
     void* out;
     float* acc;
-    int64_t ldo, slot;
-    const LossScal* scal;
-    int M, N, dtype, with_w;
+    int64_t slot;
+    ScaleRef scale;
+    int M, N, dtype, with_w, by_map;
     int read, write;           // acc is added to the product; the sum goes to acc instead of the result
   };
-  const Params& p;
-  float scale;
-  int row;
-  float* acc;
-  __device__ __forceinline__ EpiGrad(const Params& p_, const Gemm16Args&, const Tile16& w, int row_, int)
-      : p(p_), row(row_) {
-    scale = grad_scale(p.scal, p.dtype, p.with_w);
-    acc = p.acc != nullptr ? p.acc + w.split * p.slot + (int64_t)row * p.N : nullptr;
-  }
-  __device__ __forceinline__ void chunk(float (&v)[32], int col) {
-    if (row >= p.M || col >= p.N) return;
-    const int left = p.N - col;
-    const bool vec = left >= 32 && (p.N & 3) == 0;         // acc is 16-byte aligned and its rows are N floats
-    if (p.read) {
-      if (vec) {
+  template <int kPlanes, int kHalf, class Sums, class Done>
+  static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int, OutStage& st,
+                                             const Sums& sums, Done done) {
+    const float scale = grad_scale(p.scale, p.with_w);
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 t = *reinterpret_cast<const float4*>(acc + col + j);
-          v[j] += t.x; v[j + 1] += t.y; v[j + 2] += t.z; v[j + 3] += t.w;
-        }
-      } else {
+    for (int k = 0; k < kHalf; k += 32) {
+      float v[32];
+      sums.load(k, v);
+      if (k + 32 >= kHalf) done();
+      const int col = col0 + k;
+      if (row0 >= p.M || col >= p.N) continue;
+      if (kPlanes == 1 && p.by_map) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) if (j < left) v[j] += acc[col + j];
+        for (int j = 0; j < 32; ++j) v[j] *= scale;
+        if (p.dtype == kBF16) st.store<kFmtBF16>(&p.map, v, row0, col, 0, false);
+        else st.store<kFmtF16>(&p.map, v, row0, col, 0, false);
+        continue;
       }
-    }
-    if (p.write) {
-      if (vec) {
+      const int rows = p.M - row0 < 32 ? p.M - row0 : 32, mine = col + st.lane;
+      const bool in = mine < p.N;
+      const int64_t at = (int64_t)row0 * p.N + mine;
+      float* acc = p.acc != nullptr ? p.acc + w.split * p.slot + at : nullptr;
+      st.by_rows(v, [&](auto value) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(acc + col + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-      } else {
+        for (int r0 = 0; r0 < 32; r0 += 8) {
+          float t[8];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) if (j < left) acc[col + j] = v[j];
-      }
-      return;
-    }
+          for (int i = 0; i < 8; ++i) t[i] = p.read && in && r0 + i < rows ? acc[(int64_t)(r0 + i) * p.N] : 0.f;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] *= scale;
-    const int64_t at = (int64_t)row * p.ldo + col;
-    if (left >= 32 && p.dtype == kF32 && ((reinterpret_cast<uintptr_t>(p.out) & 15) | (p.ldo & 3)) == 0) {
-      float* dst = reinterpret_cast<float*>(p.out) + at;
-#pragma unroll
-      for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(dst + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-    } else if (left >= 32 && p.dtype != kF32 && ((reinterpret_cast<uintptr_t>(p.out) & 15) | (p.ldo & 7)) == 0) {
-      uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + at;
-#pragma unroll
-      for (int j = 0; j < 32; j += 8) {
-        uint32_t h[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (p.dtype == kBF16) {
-            const __nv_bfloat162 t = __floats2bfloat162_rn(v[j + 2 * i], v[j + 2 * i + 1]);
-            h[i] = *reinterpret_cast<const uint32_t*>(&t);
-          } else {
-            h[i] = pack_half2(__float2half_rn(v[j + 2 * i]), __float2half_rn(v[j + 2 * i + 1]));
+          for (int i = 0; i < 8; ++i) {
+            t[i] += value(r0 + i);
+            if (!in || r0 + i >= rows) continue;
+            if (p.write) acc[(int64_t)(r0 + i) * p.N] = t[i];
+            else store_as(p.out, at + (int64_t)(r0 + i) * p.N, t[i] * scale, p.dtype);
           }
         }
-        *reinterpret_cast<uint4*>(dst + j) = make_uint4(h[0], h[1], h[2], h[3]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) if (j < left) store_as(p.out, at + j, v[j], p.dtype);
+      });
     }
   }
-  __device__ __forceinline__ void end() {}
 };
 
 // ------------------------------------------------------------------ joining
-// The halves of a row's tiles to its log-sum-exp (log2) and its loss.  kRows rows a block, the rest of its threads share
-// the tiles of a row.
-template <int kRows>
-__global__ void __launch_bounds__(256)
-k_loss_join(const float2* __restrict__ part, int parts, int n, const float* __restrict__ target, const int* __restrict__ label,
-            const float* __restrict__ c, float* __restrict__ lse, float* __restrict__ loss) {
-  constexpr int kLanes = 256 / kRows;
-  __shared__ float2 sh[kLanes][kRows];
-  const int rr = threadIdx.x % kRows, ln = threadIdx.x / kRows, row = blockIdx.x * kRows + rr;
-  float m = -INFINITY, s = 0.f;
-  if (row < n)
-    for (int q = ln; q < parts; q += kLanes) {
-      const float2 v = part[(int64_t)q * n + row];
-      const float mn = fmaxf(m, v.x), ref = mn == -INFINITY ? 0.f : mn;
-      s = s * ex2(m - ref) + v.y * ex2(v.x - ref);
-      m = mn;
-    }
-  sh[ln][rr] = make_float2(m, s);
-  for (int o = kLanes / 2; o > 0; o >>= 1) {
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x), ref = m == -INFINITY ? 0.f : m;
+  return make_float2(m, a.y * ex2(a.x - ref) + b.y * ex2(b.x - ref));
+}
+// the parts of a row, joined by kLanes threads of a block (a warp, or the block of 256), in all of them
+template <int kLanes>
+__device__ __forceinline__ float2 join_row(const float2* part, int parts, int ln) {
+  float2 a = make_float2(-INFINITY, 0.f);
+  for (int q = ln; q < parts; q += kLanes) a = join(a, part[q]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    a = join(a, make_float2(__shfl_xor_sync(0xffffffffu, a.x, o), __shfl_xor_sync(0xffffffffu, a.y, o)));
+  if (kLanes > 32) {
+    __shared__ float2 sh[8];
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
     __syncthreads();
-    if (ln < o) {
-      const float2 a = sh[ln][rr], b = sh[ln + o][rr];
-      const float mn = fmaxf(a.x, b.x), ref = mn == -INFINITY ? 0.f : mn;
-      sh[ln][rr] = make_float2(mn, a.y * ex2(a.x - ref) + b.y * ex2(b.x - ref));
+    a = sh[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) a = join(a, sh[i]);
+  }
+  return a;
+}
+
+struct JoinArgs {
+  const float2* part;
+  const float* target;
+  const int64_t* y;
+  const float* coef;
+  float* lse;
+  float* loss;
+  uint16_t* g;                 // exponentials that become G; null: the losses alone
+  int64_t ldg, plane;
+  const uint16_t* x;           // rows that are copied with zeros where there is no class; null: packed already
+  uint16_t* x_out;
+  int64_t ldx, ldxo;
+  ScaleRef scale;
+  int n, V, d, parts, width, keep, dtype;    // width: classes of a part
+  uint32_t* status;
+};
+// A row's log-sum-exp (log2) and loss and, in place, its kept exponentials to G.  kLanes threads a row; blockIdx.y shares
+// the classes of a row where there are few rows.  Bound by reading and writing G.
+template <int kLanes>
+__global__ void __launch_bounds__(256)
+k_loss_rows(const __grid_constant__ JoinArgs p) {
+  pdl_wait();
+  const int ln = threadIdx.x % kLanes, row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  if (kLanes == 32 && row >= p.n) return;
+  const float2* part = p.part + (int64_t)row * p.parts;
+  const float2 a = join_row<kLanes>(part, p.parts, ln);
+  const float l2 = log2f(a.y), lse = a.x + l2;
+  const int64_t lab = p.y[row];
+  const bool ok = has_class(lab, p.V);
+  const float c = ok ? (p.coef != nullptr ? p.coef[row] : 1.f) : 0.f;
+  const float target = ok ? p.target[row] : 0.f;
+  if (ln == 0 && blockIdx.y == 0) {
+    if (lab != -1 && !ok) set_status(p.status, kBadIndex, (uint32_t)row, (uint32_t)lab);
+    p.lse[row] = lse;
+    p.loss[row] = ok ? c * (kLn2 * ((a.x - target) + l2)) : 0.f;
+  }
+  if (p.g == nullptr) return;
+  if (p.x != nullptr && blockIdx.y == 0) {
+    // 16-byte aligned rows of any length: what lies between the end of a row and its stride is never read by a product
+    for (int i = ln * 8; i < p.d; i += kLanes * 8) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (ok) {
+        if (i + 8 <= p.d) {
+          v = *reinterpret_cast<const uint4*>(p.x + row * p.ldx + i);
+        } else {
+          uint16_t t[8] = {};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) if (i + j < p.d) t[j] = p.x[row * p.ldx + i + j];
+          v = make_uint4(t[0] | t[1] << 16, t[2] | t[3] << 16, t[4] | t[5] << 16, t[6] | t[7] << 16);
+        }
+      }
+      *reinterpret_cast<uint4*>(p.x_out + row * p.ldxo + i) = v;
     }
   }
-  if (ln == 0 && row < n) {
-    const float2 v = sh[0][rr];
-    const float l2 = log2f(v.y);
-    lse[row] = v.x + l2;
-    loss[row] = label[row] >= 0 ? c[row] * (kLn2 * ((v.x - target[row]) + l2)) : 0.f;
+  const int kg = p.scale.get().g;
+  const float cg = c * pow2i(kg), at_label = cg * (ex2((target - a.x) - l2) - 1.f);
+  const float shift = (float)kExpScale + l2;
+  uint16_t* g = p.g + (int64_t)row * p.ldg;
+  for (int col = (blockIdx.y * kLanes + ln) * 8; col < p.keep; col += gridDim.y * kLanes * 8) {
+    uint4 h = *reinterpret_cast<const uint4*>(g + col), l = make_uint4(0, 0, 0, 0);
+    if (p.dtype == kF32) l = *reinterpret_cast<const uint4*>(g + p.plane + col);
+    const float f = cg * ex2((part[col / p.width].x - a.x) - shift);
+    uint32_t hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hs[i]));
+      if (p.dtype == kF32) {
+        const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&ls[i]));
+        v.x += u.x; v.y += u.y;
+      }
+      v.x = ok ? (lab == col + 2 * i ? at_label : v.x * f) : 0.f;
+      v.y = ok ? (lab == col + 2 * i + 1 ? at_label : v.y * f) : 0.f;
+      if (p.dtype == kBF16) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(v.x, v.y);
+        hs[i] = *reinterpret_cast<const uint32_t*>(&t);
+      } else {
+        __half h0, l0, h1, l1;
+        split16(v.x, h0, l0);
+        split16(v.y, h1, l1);
+        hs[i] = pack_half2(h0, h1);
+        ls[i] = pack_half2(l0, l1);
+      }
+    }
+    *reinterpret_cast<uint4*>(g + col) = make_uint4(hs[0], hs[1], hs[2], hs[3]);
+    if (p.dtype == kF32) *reinterpret_cast<uint4*>(g + p.plane + col) = make_uint4(ls[0], ls[1], ls[2], ls[3]);
   }
 }
 
 // the splits of K to the result
 __global__ void __launch_bounds__(256)
-k_loss_sum(const float* __restrict__ acc, int splits, int64_t slot, int64_t numel, void* out, const LossScal* scal, int dtype, int with_w) {
-  const float scale = grad_scale(scal, dtype, with_w);
+k_loss_sum(const float* __restrict__ acc, int splits, int64_t slot, int64_t numel, void* out, ScaleRef scale_ref, int dtype, int with_w) {
+  pdl_wait();
+  const float scale = grad_scale(scale_ref, with_w);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < numel; i += (int64_t)gridDim.x * 256) {
     float v = 0.f;
     for (int q = 0; q < splits; ++q) v += acc[q * slot + i];
@@ -403,7 +470,7 @@ struct LossArgs {
   void* gx;
   void* gw;
   int64_t ldx, ldw;
-  int n, V, d, dtype, want_grad, pad;
+  int n, V, d, dtype, want_grad, keep_mb;     // keep_mb: megabytes of exponentials that are kept
   void* ws;
   int64_t ws_bytes;
   uint32_t* status;
@@ -415,101 +482,79 @@ using namespace psb;
 
 namespace {
 
+constexpr int kMaxBlocks = 296;               // of the pass that finds the largest magnitudes, for either operand
+
 // where things lie in the workspace; everything is 256-byte aligned
 struct LossPlan {
-  int planes, pack_w, piece, tile;            // tile: 0 = pairs 256x256, 1 = 128x128, 2 = 128x64, of the scores
-  int parts, gx_splits, gw_splits;
+  int planes, pack_x, pack_w, parts, keep, piece;
+  Tiling score, gx, gw;                       // gx, gw: of the kept classes, or of a piece
   int64_t dp, ldg, x_plane, w_plane, g_plane;
-  int64_t scal, label, c, lse, target, x, w, part, g, gx_acc, gw_acc, total;
+  int64_t scales, maxima, lse, target, x, w, part, g, gx_acc, gw_acc, total;
 };
-
-constexpr int64_t kPieceBytes = (int64_t)256 << 20;    // of G
-
-int tile_kind(int64_t M, int64_t N) {
-  // 256x256 tiles of pairs from 48 tiles on (two thirds of the pairs of SMs); below, 128x128 tiles, or 128x64 where
-  // those would leave more than half of the SMs idle
-  if (((M + 255) / 256) * ((N + 255) / 256) >= 48) return 0;
-  return ((M + 127) / 128) * ((N + 127) / 128) >= 74 ? 1 : 2;
-}
-int tile_cols(int kind) { return kind == 0 ? 256 : kind == 1 ? 128 : 64; }
-int64_t tiles_of(int kind, int64_t M, int64_t N) {
-  const int64_t m = kind == 0 ? 256 : 128, c = tile_cols(kind);
-  return ((M + m - 1) / m) * ((N + c - 1) / c);
-}
-// K in so many pieces that the SMs are busy, eight blocks of 64 a piece at least; pieces' sums are stored and added up
-int split_count(int64_t M, int64_t N, int64_t K) {
-  const int64_t tiles = tiles_of(tile_kind(M, N), M, N), nkb = (K + kG16K - 1) / kG16K;
-  int64_t s = 148 / (tiles < 1 ? 1 : tiles);
-  if (s > nkb / 8) s = nkb / 8;
-  if (s < 2) return 1;
-  const int64_t per = (nkb + s - 1) / s;
-  return (int)((nkb + per - 1) / per);
-}
 
 LossPlan loss_plan(const LossArgs& a) {
   LossPlan p = {};
   p.planes = a.dtype == kF32 ? 2 : 1;
-  p.dp = (a.d + 7) / 8 * 8;
-  p.pack_w = p.planes == 2 || (a.ldw & 7) || (reinterpret_cast<uintptr_t>(a.w) & 15) || a.ldw < a.d;
-  p.tile = tile_kind(a.n, a.V);
-  p.parts = 2 * (int)((a.V + tile_cols(p.tile) - 1) / tile_cols(p.tile));
+  p.dp = ((int64_t)a.d + 7) / 8 * 8;
+  auto direct = [&](const void* t, int64_t ld) { return p.planes == 1 && (ld & 7) == 0 && (reinterpret_cast<uintptr_t>(t) & 15) == 0 && ld >= a.d; };
+  p.pack_x = !direct(a.x, a.ldx);
+  p.pack_w = !direct(a.w, a.ldw);
+  p.score = choose_tiling(1, a.n, a.V, a.d, p.planes, false, 1);
+  const int cols = tiling_cols(p.score.kind);
+  p.parts = 2 * ((a.V + cols - 1) / cols);
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
-  p.scal = take(sizeof(LossScal));
-  p.label = take((int64_t)a.n * 4);
-  p.c = take((int64_t)a.n * 4);
+  p.scales = take(sizeof(Scales));
+  p.maxima = take(2 * kMaxBlocks * 4);
   p.lse = take((int64_t)a.n * 4);
   p.target = take((int64_t)a.n * 4);
   p.x_plane = (int64_t)a.n * p.dp;
-  p.x = take(p.x_plane * 2 * p.planes);
+  if (p.pack_x || a.want_grad) p.x = take(p.x_plane * 2 * p.planes);
   p.w_plane = (int64_t)a.V * p.dp;
   if (p.pack_w) p.w = take(p.w_plane * 2 * p.planes);
   p.part = take((int64_t)p.parts * a.n * 8);
   if (a.want_grad) {
-    int64_t len = kPieceBytes / ((int64_t)a.n * 2 * p.planes) / 256 * 256;
+    int64_t len = ((int64_t)a.keep_mb << 20) / ((int64_t)a.n * 2 * p.planes) / 256 * 256;
     if (len < 256) len = 256;
-    p.piece = (int)(len < a.V ? len : a.V);
-    p.ldg = (p.piece + 7) / 8 * 8;
+    p.keep = p.piece = (int)(len < a.V ? len : a.V);
+    p.ldg = ((int64_t)p.piece + 7) / 8 * 8;
     p.g_plane = (int64_t)a.n * p.ldg;
     p.g = take(p.g_plane * 2 * p.planes);
-    p.gx_splits = p.piece >= a.V ? split_count(a.n, a.d, a.V) : 1;
-    p.gw_splits = p.piece >= a.V ? split_count(a.V, a.d, a.n) : 1;
-    if (a.gx != nullptr && (p.gx_splits > 1 || p.piece < a.V)) p.gx_acc = take((int64_t)p.gx_splits * a.n * a.d * 4);
-    if (p.gw_splits > 1) p.gw_acc = take((int64_t)p.gw_splits * a.V * a.d * 4);
+    const bool pieces = p.piece < a.V;
+    p.gw = choose_tiling(1, p.piece, a.d, a.n, p.planes, false, pieces ? 1 : 16);
+    p.gx = choose_tiling(1, a.n, a.d, p.piece, p.planes, false, pieces ? 1 : 64);
+    if (a.gx != nullptr && (p.gx.splits > 1 || pieces)) p.gx_acc = take((int64_t)p.gx.splits * a.n * a.d * 4);
+    if (p.gw.splits > 1) p.gw_acc = take((int64_t)p.gw.splits * a.V * a.d * 4);
   }
   p.total = at;
   return p;
 }
 
-template <int kPlanes, bool kAMN, bool kBMN, class Epi>
-int by_tile(int kind, const Gemm16Args& g, const Operand16& a, const Operand16& b, const typename Epi::Params& ep, cudaStream_t s) {
-  if (kind == 0) return launch16<Cfg16<2, 256, kPlanes, kAMN, kBMN>, Epi>(g, a, b, ep, s);
-  if (kind == 1) return launch16<Cfg16<1, 128, kPlanes, kAMN, kBMN>, Epi>(g, a, b, ep, s);
-  return launch16<Cfg16<1, 64, kPlanes, kAMN, kBMN>, Epi>(g, a, b, ep, s);
-}
-template <bool kAMN, bool kBMN, class Epi>
-int by_planes(int planes, int kind, const Gemm16Args& g, const Operand16& a, const Operand16& b, const typename Epi::Params& ep, cudaStream_t s) {
-  return planes == 2 ? by_tile<2, kAMN, kBMN, Epi>(kind, g, a, b, ep, s) : by_tile<1, kAMN, kBMN, Epi>(kind, g, a, b, ep, s);
-}
-
-unsigned blocks_for(int64_t threads) {
+unsigned blocks_for(int64_t threads, int64_t most) {
   const int64_t b = (threads + 255) / 256;
-  return (unsigned)(b < 1 ? 1 : b > 148 * 8 ? 148 * 8 : b);
-}
-template <typename T>
-void pack(const void* a, int64_t rows, int cols, int64_t ld, const int64_t* y, int V, uint16_t* out, int64_t ldo, int64_t plane,
-          const LossScal* scal, int which, cudaStream_t s) {
-  k_loss_pack<T><<<blocks_for(rows * (ldo / 8)), 256, 0, s>>>(reinterpret_cast<const T*>(a), rows, cols, ld, y, V, out, ldo, plane, scal, which);
-}
-void pack_any(int dtype, const void* a, int64_t rows, int cols, int64_t ld, const int64_t* y, int V, uint16_t* out, int64_t ldo, int64_t plane,
-              const LossScal* scal, int which, cudaStream_t s) {
-  if (dtype == kF32) pack<float>(a, rows, cols, ld, y, V, out, ldo, plane, scal, which, s);
-  else if (dtype == kBF16) pack<__nv_bfloat16>(a, rows, cols, ld, y, V, out, ldo, plane, scal, which, s);
-  else pack<__half>(a, rows, cols, ld, y, V, out, ldo, plane, scal, which, s);
+  return (unsigned)(b < 1 ? 1 : b > most ? most : b);
 }
 
 bool loss_args_ok(const LossArgs& a) {
-  return a.n > 0 && a.V > 0 && a.d > 0 && a.dtype >= kF32 && a.dtype <= kF16 && a.V <= (1 << 30) && a.n <= (1 << 30) && a.d <= (1 << 30);
+  return a.n > 0 && a.V > 0 && a.d > 0 && a.dtype >= kF32 && a.dtype <= kF16 && a.V <= (1 << 30) && a.n <= (1 << 30) && a.d <= (1 << 30) &&
+         a.keep_mb >= 0;
+}
+
+// out [M, N], contiguous, from a product, whole or split
+int gradient(Chain& chain, const LossPlan& p, const Tiling& t, Gemm16Args g, const Operand16& A, const Operand16& B, EpiGrad::Params e) {
+  g.splits = t.splits;
+  g.kb_split = t.splits > 1 ? t.kb_split : (g.K + kG16K - 1) / kG16K;
+  e.M = g.M; e.N = g.N;
+  if (t.splits > 1) { e.slot = (int64_t)g.M * g.N; e.write = 1; e.read = 0; }
+  e.by_map = !e.write && !e.read && e.dtype != kF32 && (g.N & 7) == 0 && (reinterpret_cast<uintptr_t>(e.out) & 15) == 0;
+  if (e.by_map) {
+    const int r = make_out_map(&e.map, Operand16{e.out, g.M, g.N, g.N, 0, 1}, e.dtype == kBF16);
+    if (r) return r;
+  }
+  int r = product16<EpiGrad>(chain, p.planes, t.kind, g, A, B, e);
+  if (r == 0 && t.splits > 1)
+    r = chain.launch(k_loss_sum, dim3(blocks_for(e.slot, 148 * 8)), 256, 0, 1, e.acc, t.splits, e.slot, e.slot, e.out, e.scale, e.dtype, e.with_w);
+  return r;
 }
 
 }  // namespace
@@ -526,76 +571,94 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
   const LossPlan p = loss_plan(a);
   if (p.total > a.ws_bytes || (reinterpret_cast<uintptr_t>(a.ws) & 255)) return (int)cudaErrorInvalidValue;
   uint8_t* ws = reinterpret_cast<uint8_t*>(a.ws);
-  LossScal* scal = reinterpret_cast<LossScal*>(ws + p.scal);
-  int* label = reinterpret_cast<int*>(ws + p.label);
-  float *c = reinterpret_cast<float*>(ws + p.c), *lse = reinterpret_cast<float*>(ws + p.lse), *target = reinterpret_cast<float*>(ws + p.target);
+  Scales* found = reinterpret_cast<Scales*>(ws + p.scales);
+  uint32_t* maxima = reinterpret_cast<uint32_t*>(ws + p.maxima);
+  float *lse = reinterpret_cast<float*>(ws + p.lse), *target = reinterpret_cast<float*>(ws + p.target);
   uint16_t *xb = reinterpret_cast<uint16_t*>(ws + p.x), *wb = reinterpret_cast<uint16_t*>(ws + p.w), *gb = reinterpret_cast<uint16_t*>(ws + p.g);
   float2* part = reinterpret_cast<float2*>(ws + p.part);
-  const int bf16 = a.dtype == kBF16;
+  Chain chain{s};
+  int r = 0;
 
-  cudaError_t e = cudaMemsetAsync(scal, 0, sizeof(LossScal), s);
-  if (e != cudaSuccess) return (int)e;
-  k_loss_labels<<<blocks_for(a.n), 256, 0, s>>>(a.y, a.coef, a.n, a.V, label, c, scal, a.status);
+  ScaleRef scale{{0, 0, a.dtype == kBF16 ? 0 : 13}, nullptr};       // without coefficients the largest is 1
+  if (a.dtype == kF32 || (a.dtype == kF16 && a.coef != nullptr && a.want_grad)) scale.found = found;
+  if (scale.found != nullptr && a.dtype == kF16) r = chain.launch(k_loss_coef, dim3(1), 256, 0, 1, a.coef, a.y, a.n, a.V, found);
+  unsigned mx = 0, mw = 0;
   if (a.dtype == kF32) {
-    k_loss_absmax<<<blocks_for((int64_t)a.n * ((a.d + 3) / 4)), 256, 0, s>>>((const float*)a.x, a.n, a.d, a.ldx, a.y, a.V, &scal->max_x);
-    k_loss_absmax<<<blocks_for((int64_t)a.V * ((a.d + 3) / 4)), 256, 0, s>>>((const float*)a.w, a.V, a.d, a.ldw, nullptr, a.V, &scal->max_w);
+    mx = blocks_for((int64_t)a.n * ((a.d + 3) / 4), kMaxBlocks);
+    mw = blocks_for((int64_t)a.V * ((a.d + 3) / 4), kMaxBlocks);
+    r = chain.launch(k_loss_absmax, dim3(mx + mw), 256, 0, 1, (const float*)a.x, a.ldx, (const float*)a.w, a.ldw, a.n, a.V, a.d, a.y, (int)mx, maxima);
   }
-  pack_any(a.dtype, a.x, a.n, a.d, a.ldx, a.y, a.V, xb, p.dp, p.x_plane, scal, 0, s);
-  if (p.pack_w) pack_any(a.dtype, a.w, a.V, a.d, a.ldw, nullptr, a.V, wb, p.dp, p.w_plane, scal, 1, s);
-  if ((e = cudaGetLastError()) != cudaSuccess) return (int)e;
+  if (r) return r;
+  if (p.pack_x || p.pack_w) {
+    const PackArgs px{a.x, a.n, a.ldx, xb, p.dp, p.x_plane}, pw{a.w, a.V, a.ldw, wb, p.dp, p.w_plane};
+    const unsigned bx = p.pack_x ? blocks_for((int64_t)a.n * (p.dp / 8), 148 * 8) : 0, bw = p.pack_w ? blocks_for((int64_t)a.V * (p.dp / 8), 148 * 8) : 0;
+    auto pack = [&](auto kernel) {
+      return chain.launch(kernel, dim3(bx + bw), 256, 0, 1, px, pw, a.d, a.y, a.n, a.V, a.coef, (int)bx, maxima, (int)mx, (int)mw, found);
+    };
+    r = a.dtype == kF32 ? pack(k_loss_pack<float>) : a.dtype == kBF16 ? pack(k_loss_pack<__nv_bfloat16>) : pack(k_loss_pack<__half>);
+    if (r) return r;
+  }
 
-  const Operand16 x{xb, a.n, a.d, p.dp, p.x_plane, p.planes};
+  // scores
+  const Operand16 x = p.pack_x ? Operand16{xb, a.n, a.d, p.dp, p.x_plane, p.planes} : Operand16{a.x, a.n, a.d, a.ldx, 0, 1};
   const Operand16 w = p.pack_w ? Operand16{wb, a.V, a.d, p.dp, p.w_plane, p.planes} : Operand16{a.w, a.V, a.d, a.ldw, 0, 1};
   Gemm16Args g = {};
-  g.batch = 1; g.splits = 1; g.bf16 = bf16; g.status = a.status;
+  g.batch = 1; g.splits = 1; g.bf16 = a.dtype == kBF16; g.status = a.status;
   g.M = a.n; g.N = a.V; g.K = a.d;
   g.kb_split = (a.d + kG16K - 1) / kG16K;
-  int r = by_planes<false, false, EpiScore>(p.planes, p.tile, g, x, w, EpiScore::Params{part, target, label, scal, a.n, a.V, a.dtype}, s);
-  if (r) return r;
-  if (a.n >= 256) k_loss_join<32><<<(a.n + 31) / 32, 256, 0, s>>>(part, p.parts, a.n, target, label, c, lse, a.loss);
-  else k_loss_join<1><<<a.n, 256, 0, s>>>(part, p.parts, a.n, target, label, c, lse, a.loss);
-  if ((e = cudaGetLastError()) != cudaSuccess || !a.want_grad) return (int)e;
+  EpiScore::Params es = {};
+  es.part = part; es.target = target; es.y = a.y; es.scale = scale; es.n = a.n; es.V = a.V; es.parts = p.parts; es.keep = p.keep;
+  if (a.want_grad && (r = make_out_map(&es.e, Operand16{gb, a.n, p.keep, p.ldg, p.g_plane, p.planes}, 0)) != 0) return r;
+  if ((r = product16<EpiScore>(chain, p.planes, p.score.kind, g, x, w, es)) != 0) return r;
 
+  // losses, and G of the kept classes
+  JoinArgs j = {};
+  j.part = part; j.target = target; j.y = a.y; j.coef = a.coef; j.lse = lse; j.loss = a.loss; j.scale = scale;
+  j.n = a.n; j.V = a.V; j.d = a.d; j.parts = p.parts; j.width = tiling_cols(p.score.kind) / 2; j.keep = p.keep; j.dtype = a.dtype; j.status = a.status;
+  if (a.want_grad) {
+    j.g = gb; j.ldg = p.ldg; j.plane = p.g_plane;
+    if (!p.pack_x) { j.x = reinterpret_cast<const uint16_t*>(a.x); j.x_out = xb; j.ldx = a.ldx; j.ldxo = p.dp; }
+  }
+  if (p.parts <= 64 && a.V <= 2048) {           // a warp a row; with and without gradients alike, so that losses are the same
+    r = chain.launch(k_loss_rows<32>, dim3((unsigned)(a.n + 7) / 8, 1), 256, 0, 1, j);
+  } else {
+    int64_t share = a.want_grad ? (148 * 4 + a.n - 1) / a.n : 1, most = ((int64_t)p.keep + 2047) / 2048;
+    if (share > most) share = most < 1 ? 1 : most;
+    r = chain.launch(k_loss_rows<256>, dim3((unsigned)a.n, (unsigned)share), 256, 0, 1, j);
+  }
+  if (r || !a.want_grad) return r;
+
+  const Operand16 xz{xb, a.n, a.d, p.dp, p.x_plane, p.planes};      // rows without a class are zeros
+  const int64_t es_out = a.dtype == kF32 ? 4 : 2;
   for (int v0 = 0; v0 < a.V; v0 += p.piece) {
     const int len = a.V - v0 < p.piece ? a.V - v0 : p.piece;
     const Operand16 gop{gb, a.n, len, p.ldg, p.g_plane, p.planes};
-    Gemm16Args gs = g;
-    gs.N = len; gs.b_n0 = v0;
-    r = by_planes<false, false, EpiG>(p.planes, tile_kind(a.n, len), gs, x, w,
-                                      EpiG::Params{gb, p.ldg, p.g_plane, lse, c, label, scal, a.n, len, v0, a.dtype}, s);
-    if (r) return r;
+    if (v0 > 0) {                              // beyond the kept classes: scores once more
+      Gemm16Args gs = g;
+      gs.N = len; gs.b_n0 = v0;
+      EpiG::Params eg = {};
+      if ((r = make_out_map(&eg.g, gop, a.dtype == kBF16)) != 0) return r;
+      eg.lse = lse; eg.coef = a.coef; eg.y = a.y; eg.scale = scale; eg.n = a.n; eg.V = a.V; eg.len = len; eg.v0 = v0; eg.dtype = a.dtype;
+      if ((r = product16<EpiG>(chain, p.planes, choose_tiling(1, a.n, len, a.d, p.planes, false, 1).kind, gs, x, w, eg)) != 0) return r;
+    }
+    EpiGrad::Params e = {};
+    e.scale = scale; e.dtype = a.dtype;
     // gw[v0.., :] = Gᵀ x
     Gemm16Args gg = g;
-    const int nkb = (a.n + kG16K - 1) / kG16K;
-    gg.M = len; gg.N = a.d; gg.K = a.n; gg.splits = p.gw_splits; gg.kb_split = (nkb + p.gw_splits - 1) / p.gw_splits;
-    const int64_t es = a.dtype == kF32 ? 4 : 2;
-    EpiGrad::Params eg = {};
-    eg.out = reinterpret_cast<uint8_t*>(a.gw) + (int64_t)v0 * a.d * es;
-    eg.ldo = a.d; eg.scal = scal; eg.M = len; eg.N = a.d; eg.dtype = a.dtype; eg.with_w = 0;
-    if (p.gw_splits > 1) { eg.acc = reinterpret_cast<float*>(ws + p.gw_acc); eg.slot = (int64_t)a.V * a.d; eg.write = 1; }
-    r = by_planes<true, true, EpiGrad>(p.planes, tile_kind(len, a.d), gg, gop, x, eg, s);
-    if (r) return r;
-    if (p.gw_splits > 1)
-      k_loss_sum<<<blocks_for((int64_t)a.V * a.d), 256, 0, s>>>(eg.acc, p.gw_splits, eg.slot, (int64_t)a.V * a.d, a.gw, scal, a.dtype, 0);
+    gg.M = len; gg.N = a.d; gg.K = a.n; gg.a_mn = gg.b_mn = 1;
+    EpiGrad::Params ew = e;
+    ew.out = reinterpret_cast<uint8_t*>(a.gw) + (int64_t)v0 * a.d * es_out;
+    if (p.gw.splits > 1) ew.acc = reinterpret_cast<float*>(ws + p.gw_acc);
+    if ((r = gradient(chain, p, p.gw, gg, gop, xz, ew)) != 0) return r;
     if (a.gx == nullptr) continue;
     // gx += G w[v0.., :]
     Gemm16Args gx = g;
-    const int vkb = (len + kG16K - 1) / kG16K;
-    gx.M = a.n; gx.N = a.d; gx.K = len; gx.b_k0 = v0; gx.splits = p.gx_splits; gx.kb_split = (vkb + p.gx_splits - 1) / p.gx_splits;
-    EpiGrad::Params ex = {};
-    ex.out = a.gx; ex.ldo = a.d; ex.scal = scal; ex.M = a.n; ex.N = a.d; ex.dtype = a.dtype; ex.with_w = 1;
-    const bool pieces = p.piece < a.V, last = v0 + len >= a.V;
-    if (pieces || p.gx_splits > 1) {
-      ex.acc = reinterpret_cast<float*>(ws + p.gx_acc);
-      ex.slot = (int64_t)a.n * a.d;
-      ex.read = v0 > 0;
-      ex.write = p.gx_splits > 1 || !last;
-    }
-    r = by_planes<false, true, EpiGrad>(p.planes, tile_kind(a.n, a.d), gx, gop, w, ex, s);
-    if (r) return r;
-    if (p.gx_splits > 1)
-      k_loss_sum<<<blocks_for((int64_t)a.n * a.d), 256, 0, s>>>(ex.acc, p.gx_splits, ex.slot, (int64_t)a.n * a.d, a.gx, scal, a.dtype, 1);
-    if ((e = cudaGetLastError()) != cudaSuccess) return (int)e;
+    gx.M = a.n; gx.N = a.d; gx.K = len; gx.b_k0 = v0; gx.b_mn = 1;
+    EpiGrad::Params ex = e;
+    ex.out = a.gx; ex.with_w = 1;
+    if (p.gx.splits > 1 || p.piece < a.V) ex.acc = reinterpret_cast<float*>(ws + p.gx_acc);
+    if (p.piece < a.V) { ex.read = v0 > 0; ex.write = v0 + len < a.V; }
+    if ((r = gradient(chain, p, p.gx, gx, gop, w, ex)) != 0) return r;
   }
   return 0;
 }

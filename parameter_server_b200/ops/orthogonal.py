@@ -54,8 +54,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5) -> torch.Tensor:
     """``steps`` Newton-Schulz steps on a contiguous matrix [rows, cols] or a batch [batch, rows, cols], fp32, bf16 or
     fp16: ``X = x / (|x|_F + 1e-7)``, then ``X ← 3.4445 X − 4.7750 (X Xᵀ) X + 2.0315 (X Xᵀ)² X`` each, which brings singular
     values into about [0.7, 1.2].  The result has the type of x; fp32 and fp16 results are computed with 22-bit operands, bf16 ones
-    with 22 bits up to the last two steps and 11 bits in those.  The workspace takes 8 bytes an element of x and 16 bytes
-    an element of the smaller square."""
+    with 22 bits up to the last step and 11 bits in that.  The workspace takes 8 bytes an element of x and 12 bytes or more an
+    element of the smaller square."""
     _check("orthogonalize: x", x, x, tuple(DTYPES))
     with torch.cuda.device(x.device):
         out = torch.empty_like(x)

@@ -12,11 +12,13 @@ from . import dense
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
+KEEP_MB = 2048      # of exponentials that the forward pass leaves for the gradients; the scores of further classes are made again
+
 
 class _Args(C.Structure):
     _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("y", C.c_void_p), ("coef", C.c_void_p), ("loss", C.c_void_p), ("gx", C.c_void_p),
                 ("gw", C.c_void_p), ("ldx", C.c_int64), ("ldw", C.c_int64), ("n", C.c_int), ("V", C.c_int), ("d", C.c_int),
-                ("dtype", C.c_int), ("want_grad", C.c_int), ("pad", C.c_int), ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
+                ("dtype", C.c_int), ("want_grad", C.c_int), ("keep_mb", C.c_int), ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
                 ("status", C.c_void_p)]
 
 
@@ -29,8 +31,8 @@ def softmax_loss(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, coef: Option
     ``y``: int64 [n], 0 ≤ y < classes; -1 is a row without a class: whatever x and coef hold there, its loss is 0 and it has
     no part in the gradients.  Another label counts as -1 and is reported by :func:`dense.check_status`.  ``coef``: fp32 [n]
     (None: ones).  Rows of x and w are contiguous, their strides are free.  fp32 operands are multiplied with 22 bits
-    (three fp16 products), 16-bit ones as they are; sums are fp32.  The gradients need a workspace of 256 MB for the
-    softmax of a piece of the classes, and n·d floats where the classes take more than one piece."""
+    (three fp16 products), 16-bit ones as they are; sums are fp32.  The gradients need a workspace of 2 bytes (fp32: 4) for
+    each row and class, at most 2 GB: beyond it the classes come in pieces, whose scores are made twice, and n·d floats."""
     for name, t in (("x", x), ("w", w), ("y", y), ("coef", coef)):
         if t is not None and (not t.is_cuda or t.device != x.device):
             raise ValueError(f"softmax_loss: {name} has to be on the GPU of x")
@@ -57,7 +59,7 @@ def softmax_loss(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, coef: Option
         y, coef = y.contiguous(), None if coef is None else coef.contiguous()
         a = _Args(x.data_ptr(), w.data_ptr(), y.data_ptr(), None if coef is None else coef.data_ptr(), loss.data_ptr(),
                   None if gx is None else gx.data_ptr(), gw.data_ptr() if want_grad else None, x.stride(0), w.stride(0), n, classes, d,
-                  DTYPES[x.dtype], int(want_grad), 0, None, 0, dense.status_ptr(x.device))
+                  DTYPES[x.dtype], int(want_grad), KEEP_MB, None, 0, dense.status_ptr(x.device))
         lib = N.lib()
         lib.psb_softmax_loss_workspace.restype = C.c_int64
         size = lib.psb_softmax_loss_workspace(C.byref(a))

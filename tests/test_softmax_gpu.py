@@ -3,10 +3,12 @@
 Bounds.  A value rounded to a type is off by at most eps/2 of it (bf16 2^-8, fp16 2^-11, fp32 2^-24).  A sum on the tensor
 cores is cut to fp32 at each step of 16 elements, at most 2^-23 of the sum of the terms' magnitudes a step.
   scores   16-bit operands: d/16 steps; fp32 operands: planes hold 22 bits each (2^-22 of either factor, 2^-22 for the
-           product that is left out), 48 steps in TMEM and d/256 sums in fp32.  e_s = that bound times the largest Σ_k |x_ik w_jk|
+           product that is left out), 24 steps in TMEM and d/128 sums in fp32.  e_s = that bound times the largest Σ_k |x_ik w_jk|
            of the row, and 2^-22 of the largest score for the scaling by log2 e and its rounding.
   softmax  relative error e_p = 2 e_s (score and log-sum-exp) + 2^-20 (2^x is off by 2^-22, sums over classes, the coefficient)
-  G        e_p of the softmax part, and its rounding to the operands' type (fp32: 2^-22 in two planes)
+  G        e_p of the softmax part; except at the label, 2^-11 of it for the exponential, which is kept in fp16 relative to the
+           largest of its tile (fp32: two planes, 2^-22) and times 2^15 (a unit of 2^-24 there is 2^-39 of the largest, at
+           most of c); the rounding of G to the operands' type (fp32: 2^-22 in two planes)
   gx, gw   those errors times |w| or |x|, summed; the steps of that sum; the rounding of the result.  In fp16 a value below
            2^-14 is rounded to 2^-25 at worst: G is scaled so that its largest possible value lies in [2^13, 2^14)."""
 import pytest
@@ -19,7 +21,7 @@ TYPES = [torch.float32, torch.bfloat16, torch.float16]
 
 
 def _steps(k, dtype):
-    return (2.0 ** -23 * 48 + 2.0 ** -24 * (k / 256 + 1) + 3 * 2.0 ** -22) if dtype == torch.float32 else 2.0 ** -23 * (k / 16 + 1)
+    return (2.0 ** -23 * 24 + 2.0 ** -24 * (k / 128 + 1) + 3 * 2.0 ** -22) if dtype == torch.float32 else 2.0 ** -23 * (k / 16 + 1)
 
 
 def _reference(x, w, y, coef):
@@ -41,7 +43,9 @@ def _reference(x, w, y, coef):
     e_p = 2 * e_s + 2.0 ** -20
     p = torch.exp(s - lse[:, None])
     G = c[:, None] * p
-    eG = G.abs() * e_p[:, None]
+    kept = G.abs() * (2.0 ** -22 if dt == torch.float32 else 2.0 ** -11) + 2.0 ** -39 * c.abs()[:, None]
+    kept[torch.arange(n, device=x.device), at] = 0
+    eG = G.abs() * e_p[:, None] + kept
     G[torch.arange(n, device=x.device), at] -= c
     eG += G.abs() * (2.0 ** -22 if dt == torch.float32 else HALF_STEP[dt])
     if dt != torch.bfloat16:                    # below fp16's normal numbers, in the scaled value or its low plane
@@ -231,10 +235,11 @@ def test_no_rows():
     assert loss.shape == (0,) and gx.shape == (0, 8) and not gw.any()
 
 
-def test_classes_in_several_pieces():
-    """More rows × classes than one piece of the softmax holds: 256 MB of fp16 planes are 22,000 classes of 3,050 rows."""
+def test_classes_in_several_pieces(monkeypatch):
+    """More rows × classes than are kept for the gradients: 256 MB of fp16 planes are 22,000 classes of 3,050 rows."""
     from parameter_server_b200.ops import dense, softmax
 
+    monkeypatch.setattr(softmax, "KEEP_MB", 256)
     x, w, y = _data(3050, 50_001, 40, torch.float32, 8)
     y[::7] = -1
     loss, gx, gw = softmax.softmax_loss(x, w, y)
@@ -251,3 +256,17 @@ def test_classes_in_several_pieces():
     assert ((gw.double() - refw).norm() / refw.norm()).item() < 1e-5
     lse = torch.logsumexp(s, 1) - s.gather(1, y[live][:, None])[:, 0]
     assert ((loss[live].double() - lse).norm() / lse.norm()).item() < 1e-5
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_small_pieces(dtype, monkeypatch):
+    """The smallest pieces, 256 classes: kept ones, scores made again, a last piece of one class."""
+    from parameter_server_b200.ops import softmax
+
+    x, w, y = _data(300, 1025, 72, dtype, 9)
+    y[::5] = -1
+    coef = torch.rand(300, device="cuda") + 0.5
+    whole = softmax.softmax_loss(x, w, y, coef)
+    monkeypatch.setattr(softmax, "KEEP_MB", 0)
+    got = _check(x, w, y, coef)
+    assert torch.equal(got[0], whole[0])
