@@ -203,6 +203,337 @@ k_orth_sum(const float* __restrict__ slots, int splits, int batch, int n, int ti
   }
 }
 
+// ------------------------------------------------------------------ matrices that fit into shared memory
+// A matrix whose shorter side is at most 128 stays on the SMs for all of its steps: a cluster of CTAs holds it, each a slice
+// of the longer side, and each the whole of the small squares.  One launch instead of 17, of which each costs 6 us however
+// small it is (64x64: 107 -> 18 us).  Operands lie in shared memory as the tensor cores read them: X [lo][slice] in swizzled rows
+// of 64 columns, which is K-major for X Xᵀ and, the same bytes, MN-major for B X.
+//   X Xᵀ of the slice -> fp32 sums; a share of them is added up over the CTAs (in their order) and sent to all, as planes
+//   B = A (b I + c A) + a I by every CTA for itself; X = B X of the slice
+// Two planes throughout.  Sums over more than 128 columns have an accumulator for each 128.
+struct SmallArgs {
+  OrthArgs o;
+  int lo, hi, tall, lop, hs, cl;               // lop: lo in 16s, hs: width of a slice in 64s, cl: CTAs of a cluster
+  int a_off, a2_off, p_off;
+};
+constexpr int kSmallThreads = 256;
+
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, int rank, int cl) { return cl > 1 ? mapa_u32(addr, (uint32_t)rank) : addr; }
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint4 v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void planes8(const float (&v)[8], uint4& h, uint4& l) {
+  uint32_t hs[4], ls[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) OutStage::pair<kFmtPlanes>(v[2 * i], v[2 * i + 1], hs[i], ls[i]);
+  h = make_uint4(hs[0], hs[1], hs[2], hs[3]);
+  l = make_uint4(ls[0], ls[1], ls[2], ls[3]);
+}
+// byte offset of eight columns (the c8-th eight) of a row in an operand of `rows` rows
+__device__ __forceinline__ int tile_at(int row, int c8, int rows) { return (c8 >> 3) * rows * 128 + row * 128 + (((c8 & 7) ^ (row & 7)) << 4); }
+
+__global__ void __launch_bounds__(kSmallThreads, 1)
+k_orth_small(const __grid_constant__ SmallArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ __align__(8) uint64_t done;
+  __shared__ uint32_t tmem_base, abort_flag;
+  __shared__ double sums[16], shared_sum[8];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = warp & 3, half = warp >> 2;
+  const int rank = p.cl > 1 ? (int)cluster_rank() : 0, z = blockIdx.x / p.cl;
+  const int lo = p.lo, lop = p.lop, hs = p.hs, c0 = rank * hs, width = p.hi - c0 < 0 ? 0 : p.hi - c0 < hs ? p.hi - c0 : hs;
+  const uint32_t X = smem_u32(base), A = smem_u32(base + p.a_off), A2 = smem_u32(base + p.a2_off), P = smem_u32(base + p.p_off);
+  const uint32_t xlo = (uint32_t)(hs / 64 * lop * 128), alo = (uint32_t)((lop + 63) / 64 * lop * 128);    // from a hi to its lo plane
+
+  if (tid == 0) {
+    mbar_init(&done, 1);
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+
+  // momentum and norm
+  const int64_t at0 = (int64_t)z * p.o.rows * p.o.cols;
+  double acc = 0.0;
+  for (int i = tid; i < lo * width; i += kSmallThreads) {
+    const int64_t at = at0 + (p.tall ? (int64_t)c0 * lo + i : (int64_t)(i / width) * p.hi + c0 + i % width);
+    float u = load_as(p.o.x, at, p.o.dtype);
+    if (p.o.m != nullptr) {
+      const float mv = p.o.momentum * p.o.m[at] + u;
+      p.o.m[at] = mv;
+      u = update_direction(u, mv, p.o.momentum, p.o.nesterov);
+    }
+    acc += (double)u * u;
+  }
+  acc = warp_sum_d(acc);
+  if (lane == 0) shared_sum[warp] = acc;
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_base;
+  double total = 0.0;
+  for (int i = 0; i < 8; ++i) total += shared_sum[i];
+  if (p.cl > 1) {
+    cluster_sync_all();                                   // every CTA runs
+    if (tid < p.cl)
+      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_u32(smem_u32(&sums[rank]), (uint32_t)tid)), "d"(total) : "memory");
+    cluster_sync_all();
+    total = 0.0;
+    for (int i = 0; i < p.cl; ++i) total += sums[i];
+  }
+  const double f = (double)kNsScale / (sqrt(total) + (double)p.o.eps);
+
+  // X: eight columns of a row at a time, consecutive threads along what is contiguous in memory
+  for (int i = tid; i < lop * (hs / 8); i += kSmallThreads) {
+    const int r = p.tall ? i % lop : i / (hs / 8), c8 = p.tall ? i / lop : i % (hs / 8);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = c8 * 8 + j;
+      v[j] = 0.f;
+      if (r < lo && c < width) {
+        const int64_t at = at0 + (p.tall ? (int64_t)(c0 + c) * lo + r : (int64_t)r * p.hi + c0 + c);
+        float u = load_as(p.o.x, at, p.o.dtype);
+        if (p.o.m != nullptr) u = update_direction(u, p.o.m[at], p.o.momentum, p.o.nesterov);
+        v[j] = (float)((double)u * f);
+      }
+    }
+    uint4 h, l;
+    planes8(v, h, l);
+    const uint32_t to = X + (uint32_t)tile_at(r, c8, lop);
+    st_cluster_v4(to, h);
+    st_cluster_v4(to + xlo, l);
+  }
+  asm volatile("fence.proxy.async;" ::: "memory");
+  __syncthreads();
+
+  uint32_t phase = 0;
+  auto finish_products = [&] {                             // the issuing thread, after its products
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&done)) : "memory");
+  };
+  auto wait_products = [&] {
+    if (lane == 0 && abort_flag == 0 && !mbar_wait(&done, phase & 1)) abort_flag = 1;
+    ++phase;
+    __syncwarp();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  };
+  auto operands_ready = [&] {                              // written by all threads, read by the tensor cores next
+    asm volatile("fence.proxy.async;" ::: "memory");
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  };
+  const uint32_t idesc_sq = (1u << 4) | ((uint32_t)(lop >> 3) << 17) | (8u << 24);
+  const int row = q * 32 + lane, groups = (hs + 127) / 128;
+  const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
+
+  for (int step = 0; step < p.o.steps; ++step) {
+    // ---- X Xᵀ of the slice, an accumulator for each 128 columns
+    if (tid == 0) {
+      for (int g = 0; g < groups; ++g) {
+        uint32_t accumulate = 0;
+        for (int pr = 0; pr < 3; ++pr)                     // hi·lo, lo·hi, hi·hi
+          for (int ch = 2 * g; ch < 2 * g + 2 && ch * 64 < hs; ++ch) {
+            const uint32_t at = X + (uint32_t)(ch * lop * 128);
+            const uint64_t da = make_smem_desc(at + (pr == 1 ? xlo : 0)), db = make_smem_desc(at + (pr == 0 ? xlo : 0));
+            for (int k = 0; k < 4; ++k) {
+              mma16<1>(tmem + (uint32_t)(g * lop), da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc_sq, accumulate);
+              accumulate = 1;
+            }
+          }
+      }
+      finish_products();
+    }
+    __syncwarp();
+    wait_products();
+    if (q * 32 < lop) {
+      for (int u = half; u < lop / 16; u += 2) {
+        float v[16] = {};
+        for (int g = 0; g < groups; ++g) {
+          uint32_t r[16];
+          tmem_load_32x16(lanes + (uint32_t)(g * lop + u * 16), r);
+          tmem_load_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(r[j]);
+        }
+        if (row >= lop) continue;
+        if (p.cl > 1) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            st_cluster_v4(P + (uint32_t)(row * lop * 4 + (((u * 4 + j) ^ (row & 3)) << 4)),
+                          make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])));
+          continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float a[8], b[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            a[j] = kNsInv * v[e * 8 + j];
+            b[j] = kNsC * a[j] + (row == u * 16 + e * 8 + j ? kNsB * kNsScale : 0.f);
+          }
+          uint4 h, l;
+          const uint32_t at = (uint32_t)tile_at(row, u * 2 + e, lop);
+          planes8(a, h, l);
+          st_cluster_v4(A + at, h);
+          st_cluster_v4(A + at + alo, l);
+          planes8(b, h, l);
+          st_cluster_v4(A2 + at, h);
+          st_cluster_v4(A2 + at + alo, l);
+        }
+      }
+    }
+    if (p.cl > 1) {
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      cluster_sync_all();
+      const int units = lop * lop / 8, per = (units + p.cl - 1) / p.cl;
+      for (int i = rank * per + tid; i < (rank + 1) * per && i < units; i += kSmallThreads) {
+        const int r = i / (lop / 8), c8 = i % (lop / 8);
+        float v[8] = {};
+        for (int s = 0; s < p.cl; ++s)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float4 t = ld_cluster_v4(mapa_u32(P + (uint32_t)(r * lop * 4 + (((c8 * 2 + e) ^ (r & 3)) << 4)), (uint32_t)s));
+            v[4 * e] += t.x; v[4 * e + 1] += t.y; v[4 * e + 2] += t.z; v[4 * e + 3] += t.w;
+          }
+        float b[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[j] *= kNsInv;
+          b[j] = kNsC * v[j] + (r == c8 * 8 + j ? kNsB * kNsScale : 0.f);
+        }
+        uint4 ah, al, bh, bl;
+        planes8(v, ah, al);
+        planes8(b, bh, bl);
+        const uint32_t at = (uint32_t)tile_at(r, c8, lop);
+        for (int s = 0; s < p.cl; ++s) {
+          const uint32_t to = mapa_u32(A + at, (uint32_t)s), to2 = mapa_u32(A2 + at, (uint32_t)s);
+          st_cluster_v4(to, ah);
+          st_cluster_v4(to + alo, al);
+          st_cluster_v4(to2, bh);
+          st_cluster_v4(to2 + alo, bl);
+        }
+      }
+      asm volatile("fence.proxy.async;" ::: "memory");
+      cluster_sync_all();
+    }
+    operands_ready();
+
+    // ---- B = A (b I + c A) + a I, into A's place
+    if (tid == 0) {
+      uint32_t accumulate = 0;
+      for (int pr = 0; pr < 3; ++pr)
+        for (int k = 0; k < lop / 16; ++k) {
+          const uint32_t off = (uint32_t)((k >> 2) * lop * 128 + (k & 3) * 32);
+          mma16<1>(tmem, make_smem_desc(A + (pr == 1 ? alo : 0) + off), make_smem_desc(A2 + (pr == 0 ? alo : 0) + off), idesc_sq, accumulate);
+          accumulate = 1;
+        }
+      finish_products();
+    }
+    __syncwarp();
+    wait_products();
+    if (q * 32 < lop) {
+      for (int u = half; u < lop / 16; u += 2) {
+        uint32_t r[16];
+        tmem_load_32x16(lanes + (uint32_t)(u * 16), r);
+        tmem_load_wait();
+        if (row >= lop) continue;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float b[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) b[j] = kNsInv * __uint_as_float(r[e * 8 + j]) + (row == u * 16 + e * 8 + j ? kNsA * kNsScale : 0.f);
+          uint4 h, l;
+          const uint32_t at = (uint32_t)tile_at(row, u * 2 + e, lop);
+          planes8(b, h, l);
+          st_cluster_v4(A + at, h);
+          st_cluster_v4(A + at + alo, l);
+        }
+      }
+    }
+    operands_ready();
+
+    // ---- X = B X of the slice; X is MN-major here: chunks of 64 columns, lop lines each
+    if (tid == 0) {
+      for (int n0 = 0; n0 < hs; n0 += 256) {
+        const int n = hs - n0 < 256 ? hs - n0 : 256;
+        const uint32_t idesc = (1u << 4) | (1u << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+        const uint64_t lead = (uint64_t)((lop * 128) >> 4) << 16;
+        uint32_t accumulate = 0;
+        for (int pr = 0; pr < 3; ++pr)
+          for (int k = 0; k < lop / 16; ++k) {
+            const uint32_t off = (uint32_t)((k >> 2) * lop * 128 + (k & 3) * 32);
+            mma16<1>(tmem + (uint32_t)n0, make_smem_desc(A + (pr == 1 ? alo : 0) + off),
+                     make_smem_desc(X + (pr == 0 ? xlo : 0) + (uint32_t)(n0 / 64 * lop * 128 + k * 2048)) | lead, idesc, accumulate);
+            accumulate = 1;
+          }
+      }
+      finish_products();
+    }
+    __syncwarp();
+    wait_products();
+    const bool last = step + 1 == p.o.steps;
+    if (q * 32 < lop && !last) {
+      for (int u = half; u < hs / 16; u += 2) {
+        uint32_t r[16];
+        tmem_load_32x16(lanes + (uint32_t)(u * 16), r);
+        tmem_load_wait();
+        if (row >= lop) continue;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = kNsInv * __uint_as_float(r[e * 8 + j]);
+          uint4 h, l;
+          const uint32_t at = (uint32_t)tile_at(row, u * 2 + e, lop);
+          planes8(x, h, l);
+          st_cluster_v4(X + at, h);
+          st_cluster_v4(X + at + xlo, l);
+        }
+      }
+    } else if (q * 32 < lop) {
+      auto put = [&](int64_t at, float x) {
+        if (p.o.m != nullptr) reinterpret_cast<float*>(p.o.out)[at] -= p.o.lr * x;
+        else if (p.o.dtype == kOrthF32) reinterpret_cast<float*>(p.o.out)[at] = x;
+        else if (p.o.dtype == kOrthBF16) reinterpret_cast<__nv_bfloat16*>(p.o.out)[at] = __float2bfloat16_rn(x);
+        else reinterpret_cast<__half*>(p.o.out)[at] = __float2half_rn(x);
+      };
+      float* st = reinterpret_cast<float*>(base + p.p_off + warp * 4096);
+      for (int c = half * 32; c < hs; c += 64) {
+        uint32_t r[32];
+        tmem_load_32x32(lanes + (uint32_t)c, r);
+        tmem_load_wait();
+        if (p.tall) {                                      // lanes are neighbours in memory
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (row < lo && c + j < width) put(at0 + (int64_t)(c0 + c + j) * lo + row, kNsInv * kNsInv * __uint_as_float(r[j]));
+          continue;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) st[lane * 32 + (j ^ lane)] = kNsInv * kNsInv * __uint_as_float(r[j]);
+        __syncwarp();
+#pragma unroll 8
+        for (int i = 0; i < 32; ++i)
+          if (q * 32 + i < lo && c + lane < width) put(at0 + (int64_t)(q * 32 + i) * p.hi + c0 + c + lane, st[i * 32 + (lane ^ i)]);
+      }
+    }
+    operands_ready();
+  }
+  if (tid == 0 && abort_flag != 0) set_status(p.o.status, kWaitTimeout, blockIdx.x, 500);
+  if (p.cl > 1) cluster_sync_all();
+  if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
 }  // namespace psb
 
 using namespace psb;
@@ -214,18 +545,46 @@ struct OrthPlan {
   Tiling gram[2], square[2], step[2];         // with one plane, with two
   int64_t ldx, xplane, ldl, lplane;
   int64_t part, x0, x1, a, a2, b, slots, total;
+  int small, lop, hs, cl, a_off, a2_off, p_off, smem;      // small: a cluster of cl CTAs holds the matrix
 };
+
+constexpr int kSmallSmem = 226 * 1024;      // of 227 KB
+// The fewest CTAs that hold a matrix with a short side of at most 128, if 16 do.
+bool small_plan(OrthPlan& p) {
+  if (p.lo > 128) return false;
+  p.lop = (p.lo + 15) / 16 * 16;
+  const int square = 4 * p.lop * ((p.lop + 63) / 64 * 64);
+  for (int cl = 1; cl <= 16; cl *= 2) {
+    const int64_t hs = (((int64_t)p.hi + cl - 1) / cl + 63) / 64 * 64;
+    if (hs > 512 || (hs + 127) / 128 * p.lop > 512) continue;
+    const int sums = cl > 1 ? 4 * p.lop * p.lop : 0, stage = sums > 32768 ? sums : 32768;      // 4 KB a warp for the result
+    const int bytes = 4 * p.lop * (int)hs + 2 * square + stage + (128 - p.lop) * 128;       // tiles are read as 128 rows
+    if (bytes + 1024 > kSmallSmem) continue;
+    p.hs = (int)hs; p.cl = cl;
+    p.a_off = 4 * p.lop * p.hs; p.a2_off = p.a_off + square; p.p_off = p.a2_off + square;
+    // more than half of an SM's shared memory, so that no two CTAs of a cluster meet on an SM: each takes all of its TMEM
+    p.smem = bytes + 1024 < 120 * 1024 ? 120 * 1024 : bytes + 1024;
+    return true;
+  }
+  return false;
+}
 
 bool orth_args_ok(const OrthArgs& a) {
   return a.batch > 0 && a.rows > 0 && a.cols > 0 && a.batch <= 65535 && a.rows <= (1 << 30) && a.cols <= (1 << 30) && a.steps > 0 &&
          a.dtype >= kOrthF32 && a.dtype <= kOrthF16;
 }
 
-OrthPlan orth_plan(const OrthArgs& a) {
+struct OrthKey {
+  int batch, rows, cols;
+  bool operator==(const OrthKey& o) const { return batch == o.batch && rows == o.rows && cols == o.cols; }
+};
+
+OrthPlan make_orth_plan(const OrthKey& a) {
   OrthPlan p = {};
   p.tall = a.rows > a.cols;
   p.lo = p.tall ? a.cols : a.rows;
   p.hi = p.tall ? a.rows : a.cols;
+  if ((int64_t)a.batch * 16 < (1 << 30) && small_plan(p)) { p.small = 1; return p; }
   int64_t slots = 0;
   for (int k = 0; k < 2; ++k) {
     p.gram[k] = choose_tiling(a.batch, p.lo, p.lo, p.hi, k + 1, true, 32);
@@ -250,6 +609,16 @@ OrthPlan orth_plan(const OrthArgs& a) {
   return p;
 }
 
+// a thread keeps the plans of the sizes that it met last: the search for tiles takes microseconds
+OrthPlan orth_plan(const OrthArgs& a) {
+  struct Entry { OrthKey key; OrthPlan plan; bool used; };
+  static thread_local Entry kept[16] = {};
+  const OrthKey k{a.batch, a.rows, a.cols};
+  Entry& e = kept[((unsigned)k.batch * 31u + (unsigned)k.rows * 7u + (unsigned)k.cols * 13u) % 16u];
+  if (!e.used || !(e.key == k)) e = Entry{k, make_orth_plan(k), true};
+  return e.plan;
+}
+
 }  // namespace
 
 extern "C" {
@@ -262,6 +631,20 @@ int psb_orthogonal(const OrthArgs* ap, cudaStream_t s) {
   const OrthArgs& a = *ap;
   if (!orth_args_ok(a)) return (int)cudaErrorInvalidValue;
   const OrthPlan p = orth_plan(a);
+  if (p.small) {
+    Chain chain{s};
+    int dev = 0;
+    if (sm_count(&dev) <= 0) return (int)cudaErrorInvalidDevice;
+    static bool attr[kMaxDevices] = {};
+    if (!attr[dev]) {
+      cudaError_t e = cudaFuncSetAttribute(k_orth_small, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmallSmem);
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(k_orth_small, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return (int)e;
+      attr[dev] = true;
+    }
+    const SmallArgs q{a, p.lo, p.hi, p.tall, p.lop, p.hs, p.cl, p.a_off, p.a2_off, p.p_off};
+    return chain.launch(k_orth_small, dim3((unsigned)(a.batch * p.cl)), kSmallThreads, p.smem, p.cl, q);
+  }
   if (p.total > a.ws_bytes || (reinterpret_cast<uintptr_t>(a.ws) & 255)) return (int)cudaErrorInvalidValue;
   uint8_t* ws = reinterpret_cast<uint8_t*>(a.ws);
   double* part = reinterpret_cast<double*>(ws + p.part);

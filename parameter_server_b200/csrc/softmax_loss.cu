@@ -79,33 +79,38 @@ k_loss_coef(const float* __restrict__ coef, const int64_t* __restrict__ y, int n
   if (threadIdx.x == 0) *out = Scales{0, 0, scale_exp(top, 13)};
 }
 
+// the largest finite magnitude that a thread finds, taking each step-th four columns from the first on (y null: all rows count)
+__device__ __forceinline__ uint32_t thread_absmax(const float* a, int64_t ld, int64_t rows, int cols, const int64_t* y, int V, int64_t first,
+                                                  int64_t step) {
+  uint32_t top = 0;
+  const bool vec = ((reinterpret_cast<uintptr_t>(a) & 15) | (ld & 3)) == 0;
+  const int per = (cols + 3) / 4;
+  const int64_t total = rows * per;
+  for (int64_t i = first; i < total; i += step) {
+    const int64_t r = i / per;
+    const int c = (int)(i - r * per) * 4;
+    if (y != nullptr && !has_class(y[r], V)) continue;
+    const float* p = a + r * ld + c;
+    if (vec && c + 4 <= cols) {
+      const float4 v = *reinterpret_cast<const float4*>(p);
+      top = max(max(top, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
+    } else {
+      for (int j = 0; j < 4 && c + j < cols; ++j) top = max(top, finite_bits(p[j]));
+    }
+  }
+  return top;
+}
 // Largest finite magnitudes of fp32 operands, a block's each: blocks 0..bx-1 take x (rows without a class do not count),
 // the others w.
 __global__ void __launch_bounds__(256)
 k_loss_absmax(const float* __restrict__ x, int64_t ldx, const float* __restrict__ w, int64_t ldw, int n, int V, int d,
               const int64_t* __restrict__ y, int bx, uint32_t* __restrict__ out) {
   pdl_wait();
-  const bool is_x = (int)blockIdx.x < bx;
-  const float* a = is_x ? x : w;
-  const int64_t ld = is_x ? ldx : ldw, rows = is_x ? n : V, nb = is_x ? bx : gridDim.x - bx, b = is_x ? blockIdx.x : blockIdx.x - bx;
-  uint32_t top = 0;
-  const bool vec = ((reinterpret_cast<uintptr_t>(a) & 15) | (ld & 3)) == 0;
-  const int per = (d + 3) / 4;
-  const int64_t total = rows * per;
-  for (int64_t i = b * 256 + threadIdx.x; i < total; i += nb * 256) {
-    const int64_t r = i / per;
-    const int c = (int)(i - r * per) * 4;
-    if (is_x && !has_class(y[r], V)) continue;
-    const float* p = a + r * ld + c;
-    if (vec && c + 4 <= d) {
-      const float4 v = *reinterpret_cast<const float4*>(p);
-      top = max(max(top, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
-    } else {
-      for (int j = 0; j < 4 && c + j < d; ++j) top = max(top, finite_bits(p[j]));
-    }
-  }
-  top = block_max_u32(top);
-  if (threadIdx.x == 0) out[blockIdx.x] = top;
+  const int b = (int)blockIdx.x;
+  const uint32_t top = block_max_u32(b < bx ? thread_absmax(x, ldx, n, d, y, V, (int64_t)b * 256 + threadIdx.x, (int64_t)bx * 256)
+                                            : thread_absmax(w, ldw, V, d, nullptr, V, (int64_t)(b - bx) * 256 + threadIdx.x,
+                                                            (int64_t)(gridDim.x - bx) * 256));
+  if (threadIdx.x == 0) out[b] = top;
 }
 
 struct PackArgs {
@@ -127,11 +132,17 @@ k_loss_pack(PackArgs px, PackArgs pw, int cols, const int64_t* __restrict__ y, i
   float s = 1.f;
   if (sizeof(T) == 4) {
     uint32_t tx = 0, tw = 0;
-    if (is_x || blockIdx.x == gridDim.x - 1) for (int i = threadIdx.x; i < mx; i += 256) tx = max(tx, maxima[i]);
-    if (!is_x) for (int i = threadIdx.x; i < mw; i += 256) tw = max(tw, maxima[mx + i]);
+    const bool last = blockIdx.x == gridDim.x - 1;
+    if (maxima == nullptr) {                 // small operands: every block looks through them itself
+      if (is_x || last) tx = thread_absmax(reinterpret_cast<const float*>(px.a), px.ld, px.rows, cols, y, V, threadIdx.x, 256);
+      if (!is_x) tw = thread_absmax(reinterpret_cast<const float*>(pw.a), pw.ld, pw.rows, cols, nullptr, V, threadIdx.x, 256);
+    } else {
+      if (is_x || last) for (int i = threadIdx.x; i < mx; i += 256) tx = max(tx, maxima[i]);
+      if (!is_x) for (int i = threadIdx.x; i < mw; i += 256) tw = max(tw, maxima[mx + i]);
+    }
     const int kx = scale_exp(block_max_u32(tx), 14), kw = scale_exp(block_max_u32(tw), 14);
     s = pow2i(is_x ? kx : kw);
-    if (blockIdx.x == gridDim.x - 1) {
+    if (last) {
       const uint32_t tc = coef_max(coef, y, n, V);
       if (threadIdx.x == 0) *found = Scales{kx, kw, scale_exp(tc, 13)};
     }
@@ -492,13 +503,27 @@ struct LossPlan {
   int64_t scales, maxima, lse, target, x, w, part, g, gx_acc, gw_acc, total;
 };
 
-LossPlan loss_plan(const LossArgs& a) {
+// what a plan depends on: sizes, types and alignment
+struct LossKey {
+  int n, V, d, dtype, want_grad, want_gx, keep_mb, pack_x, pack_w;
+  bool operator==(const LossKey& o) const {
+    return n == o.n && V == o.V && d == o.d && dtype == o.dtype && want_grad == o.want_grad && want_gx == o.want_gx && keep_mb == o.keep_mb &&
+           pack_x == o.pack_x && pack_w == o.pack_w;
+  }
+};
+LossKey loss_key(const LossArgs& a) {
+  auto direct = [&](const void* t, int64_t ld) {
+    return a.dtype != kF32 && (ld & 7) == 0 && (reinterpret_cast<uintptr_t>(t) & 15) == 0 && ld >= a.d;
+  };
+  return LossKey{a.n, a.V, a.d, a.dtype, a.want_grad, a.gx != nullptr, a.keep_mb, !direct(a.x, a.ldx), !direct(a.w, a.ldw)};
+}
+
+LossPlan make_loss_plan(const LossKey& a) {
   LossPlan p = {};
   p.planes = a.dtype == kF32 ? 2 : 1;
   p.dp = ((int64_t)a.d + 7) / 8 * 8;
-  auto direct = [&](const void* t, int64_t ld) { return p.planes == 1 && (ld & 7) == 0 && (reinterpret_cast<uintptr_t>(t) & 15) == 0 && ld >= a.d; };
-  p.pack_x = !direct(a.x, a.ldx);
-  p.pack_w = !direct(a.w, a.ldw);
+  p.pack_x = a.pack_x;
+  p.pack_w = a.pack_w;
   p.score = choose_tiling(1, a.n, a.V, a.d, p.planes, false, 1);
   const int cols = tiling_cols(p.score.kind);
   p.parts = 2 * ((a.V + cols - 1) / cols);
@@ -523,11 +548,21 @@ LossPlan loss_plan(const LossArgs& a) {
     const bool pieces = p.piece < a.V;
     p.gw = choose_tiling(1, p.piece, a.d, a.n, p.planes, false, pieces ? 1 : 16);
     p.gx = choose_tiling(1, a.n, a.d, p.piece, p.planes, false, pieces ? 1 : 64);
-    if (a.gx != nullptr && (p.gx.splits > 1 || pieces)) p.gx_acc = take((int64_t)p.gx.splits * a.n * a.d * 4);
+    if (a.want_gx && (p.gx.splits > 1 || pieces)) p.gx_acc = take((int64_t)p.gx.splits * a.n * a.d * 4);
     if (p.gw.splits > 1) p.gw_acc = take((int64_t)p.gw.splits * a.V * a.d * 4);
   }
   p.total = at;
   return p;
+}
+
+// The search for tiles takes microseconds, twice a call: a thread keeps the plans of the sizes that it met last.
+LossPlan loss_plan(const LossArgs& a) {
+  struct Entry { LossKey key; LossPlan plan; bool used; };
+  static thread_local Entry kept[16] = {};
+  const LossKey k = loss_key(a);
+  Entry& e = kept[((unsigned)k.n * 31u + (unsigned)k.V * 7u + (unsigned)k.d * 13u + (unsigned)k.want_grad) % 16u];
+  if (!e.used || !(e.key == k)) e = Entry{k, make_loss_plan(k), true};
+  return e.plan;
 }
 
 unsigned blocks_for(int64_t threads, int64_t most) {
@@ -583,7 +618,8 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
   if (a.dtype == kF32 || (a.dtype == kF16 && a.coef != nullptr && a.want_grad)) scale.found = found;
   if (scale.found != nullptr && a.dtype == kF16) r = chain.launch(k_loss_coef, dim3(1), 256, 0, 1, a.coef, a.y, a.n, a.V, found);
   unsigned mx = 0, mw = 0;
-  if (a.dtype == kF32) {
+  const bool small = (int64_t)(a.n + a.V) * a.d <= 32768;      // 128 KB: 32 values a thread, less than a launch
+  if (a.dtype == kF32 && !small) {
     mx = blocks_for((int64_t)a.n * ((a.d + 3) / 4), kMaxBlocks);
     mw = blocks_for((int64_t)a.V * ((a.d + 3) / 4), kMaxBlocks);
     r = chain.launch(k_loss_absmax, dim3(mx + mw), 256, 0, 1, (const float*)a.x, a.ldx, (const float*)a.w, a.ldw, a.n, a.V, a.d, a.y, (int)mx, maxima);
@@ -593,7 +629,7 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
     const PackArgs px{a.x, a.n, a.ldx, xb, p.dp, p.x_plane}, pw{a.w, a.V, a.ldw, wb, p.dp, p.w_plane};
     const unsigned bx = p.pack_x ? blocks_for((int64_t)a.n * (p.dp / 8), 148 * 8) : 0, bw = p.pack_w ? blocks_for((int64_t)a.V * (p.dp / 8), 148 * 8) : 0;
     auto pack = [&](auto kernel) {
-      return chain.launch(kernel, dim3(bx + bw), 256, 0, 1, px, pw, a.d, a.y, a.n, a.V, a.coef, (int)bx, maxima, (int)mx, (int)mw, found);
+      return chain.launch(kernel, dim3(bx + bw), 256, 0, 1, px, pw, a.d, a.y, a.n, a.V, a.coef, (int)bx, small ? nullptr : maxima, (int)mx, (int)mw, found);
     };
     r = a.dtype == kF32 ? pack(k_loss_pack<float>) : a.dtype == kBF16 ? pack(k_loss_pack<__nv_bfloat16>) : pack(k_loss_pack<__half>);
     if (r) return r;

@@ -24,9 +24,12 @@ def _status_for(dev) -> torch.Tensor:
 def status_ptr(dev) -> int:
     """Address of the status words of a GPU for operators that may be captured: the words are made and zeroed outside of a
     graph, whose replays would zero them again."""
-    if (dev.type, dev.index) not in _status and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("run the operator, or dense.check_status(device), once on this GPU before it is captured")
-    return _status_for(dev).data_ptr()
+    st = _status.get((dev.type, dev.index))
+    if st is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("run the operator, or dense.check_status(device), once on this GPU before it is captured")
+        st = _status_for(dev)
+    return st.data_ptr()
 
 
 def check_status(dev) -> None:

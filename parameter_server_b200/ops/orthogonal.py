@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
 import torch
 
@@ -15,10 +16,9 @@ EPS = 1e-7            # added to the Frobenius norm that the steps start from
 MAX_STEPS = 64
 
 
-class _Args(C.Structure):
-    _fields_ = [("x", C.c_void_p), ("m", C.c_void_p), ("out", C.c_void_p), ("batch", C.c_int), ("rows", C.c_int), ("cols", C.c_int),
-                ("dtype", C.c_int), ("steps", C.c_int), ("nesterov", C.c_int), ("lr", C.c_float), ("momentum", C.c_float),
-                ("eps", C.c_float), ("pad", C.c_float), ("ws", C.c_void_p), ("ws_bytes", C.c_int64), ("status", C.c_void_p)]
+# the arguments of a call as csrc/orthogonal.cu has them: x or the gradient, momentum, result or weights; batch, rows, cols, type,
+# steps, nesterov; lr, momentum, eps; workspace and its bytes; status words
+_ARGS = struct.Struct("3Q6i4fQqQ")
 
 
 def _check(what: str, t: torch.Tensor, like: torch.Tensor, dtypes) -> None:
@@ -40,14 +40,20 @@ def _run(x, m, out, steps, lr, momentum, nesterov) -> None:
         raise ValueError("at most 65,535 matrices of at most 2^30 rows and columns")
     if x.numel() == 0:
         return
-    a = _Args(x.data_ptr(), None if m is None else m.data_ptr(), out.data_ptr(), batch, rows, cols, DTYPES[x.dtype], steps, int(nesterov),
-              lr, momentum, EPS, 0.0, None, 0, dense.status_ptr(x.device))
+    dev = x.device
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _run(x, m, out, steps, lr, momentum, nesterov)
+
+    def args(ws, size):
+        return _ARGS.pack(x.data_ptr(), 0 if m is None else m.data_ptr(), out.data_ptr(), batch, rows, cols, DTYPES[x.dtype], steps,
+                          1 if nesterov else 0, lr, momentum, EPS, 0.0, ws, size, dense.status_ptr(dev))
+
     lib = N.lib()
     lib.psb_orthogonal_workspace.restype = C.c_int64
-    size = lib.psb_orthogonal_workspace(C.byref(a))
-    ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-    a.ws, a.ws_bytes = ws.data_ptr(), size
-    N.check(lib.psb_orthogonal(C.byref(a), N.stream_ptr()), "orthogonal")
+    size = lib.psb_orthogonal_workspace(args(0, 0))
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    N.check(lib.psb_orthogonal(args(ws.data_ptr(), size), N.raw_stream(dev.index)), "orthogonal")
 
 
 def orthogonalize(x: torch.Tensor, steps: int = 5) -> torch.Tensor:
@@ -57,9 +63,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5) -> torch.Tensor:
     with 22 bits up to the last step and 11 bits in that.  The workspace takes 8 bytes an element of x and 12 bytes or more an
     element of the smaller square."""
     _check("orthogonalize: x", x, x, tuple(DTYPES))
-    with torch.cuda.device(x.device):
-        out = torch.empty_like(x)
-        _run(x, None, out, steps, 0.0, 0.0, False)
+    out = torch.empty_like(x)
+    _run(x, None, out, steps, 0.0, 0.0, False)
     return out
 
 
@@ -74,7 +79,6 @@ def orthogonal_update(w: torch.Tensor, g: torch.Tensor, m: torch.Tensor, lr: flo
     spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (w, g, m))
     if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
         raise ValueError("orthogonal_update: w, g and m share memory")
-    with torch.cuda.device(w.device):
-        _run(g, m, w, steps, lr * math.sqrt(max(1.0, w.shape[-2] / max(w.shape[-1], 1))), momentum, nesterov)
+    _run(g, m, w, steps, lr * math.sqrt(max(1.0, w.shape[-2] / max(w.shape[-1], 1))), momentum, nesterov)
     dense._written(w)
     dense._written(m)

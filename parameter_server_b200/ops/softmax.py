@@ -3,7 +3,8 @@ classes are tiles of a tensor-core product that are reduced where they are made,
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Tuple
+import struct
+from typing import Dict, Optional, Tuple
 
 import torch
 
@@ -15,11 +16,10 @@ DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 KEEP_MB = 2048      # of exponentials that the forward pass leaves for the gradients; the scores of further classes are made again
 
 
-class _Args(C.Structure):
-    _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("y", C.c_void_p), ("coef", C.c_void_p), ("loss", C.c_void_p), ("gx", C.c_void_p),
-                ("gw", C.c_void_p), ("ldx", C.c_int64), ("ldw", C.c_int64), ("n", C.c_int), ("V", C.c_int), ("d", C.c_int),
-                ("dtype", C.c_int), ("want_grad", C.c_int), ("keep_mb", C.c_int), ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
-                ("status", C.c_void_p)]
+# the arguments of a call as csrc/softmax_loss.cu has them: x, w, y, coef, loss, gx, gw; strides of x and w; n, classes, d, type,
+# want_grad, keep_mb; workspace and its bytes; status words.  A small call is host time: a packed struct is quicker than ctypes'.
+_ARGS = struct.Struct("7Q2q6iQqQ")
+_sizes: Dict[tuple, int] = {}
 
 
 def softmax_loss(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, coef: Optional[torch.Tensor] = None,
@@ -33,10 +33,12 @@ def softmax_loss(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, coef: Option
     (None: ones).  Rows of x and w are contiguous, their strides are free.  fp32 operands are multiplied with 22 bits
     (three fp16 products), 16-bit ones as they are; sums are fp32.  The gradients need a workspace of 2 bytes (fp32: 4) for
     each row and class, at most 2 GB: beyond it the classes come in pieces, whose scores are made twice, and n·d floats."""
+    gpu = x.get_device()
     for name, t in (("x", x), ("w", w), ("y", y), ("coef", coef)):
-        if t is not None and (not t.is_cuda or t.device != x.device):
+        if t is not None and (t.get_device() != gpu or gpu < 0):
             raise ValueError(f"softmax_loss: {name} has to be on the GPU of x")
-    if x.dtype not in DTYPES or w.dtype != x.dtype:
+    dtype = DTYPES.get(x.dtype)
+    if dtype is None or w.dtype != x.dtype:
         raise ValueError(f"softmax_loss takes x and w of one type, fp32, bf16 or fp16: got {x.dtype} and {w.dtype}")
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"softmax_loss takes x [n, d] and w [classes, d]: got {tuple(x.shape)} and {tuple(w.shape)}")
@@ -46,24 +48,35 @@ def softmax_loss(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, coef: Option
         raise ValueError("softmax_loss needs at least one class and one column")
     if max(n, d, classes) > 1 << 30:
         raise ValueError("softmax_loss takes at most 2^30 rows, classes and columns")
-    if (n > 0 and d > 1 and x.stride(1) != 1) or (d > 1 and w.stride(1) != 1):
+    (ldx, sx), (ldw, sw) = x.stride(), w.stride()
+    if d > 1 and ((n > 0 and sx != 1) or sw != 1):
         raise ValueError("softmax_loss: rows of x and w have to be contiguous")
-    if y.dtype != torch.int64 or y.shape != (n,) or (coef is not None and (coef.dtype != torch.float32 or coef.shape != (n,))):
+    if y.dtype != torch.int64 or y.dim() != 1 or y.shape[0] != n or (coef is not None and (coef.dtype != torch.float32 or coef.shape != (n,))):
         raise ValueError("softmax_loss takes labels int64 [n] and coefficients float32 [n]")
-    with torch.cuda.device(x.device):
-        loss = torch.empty(n, dtype=torch.float32, device=x.device)
-        gx = torch.empty((n, d), dtype=x.dtype, device=x.device) if want_grad and want_gx else None
-        gw = torch.empty((classes, d), dtype=w.dtype, device=x.device) if want_grad else None
-        if n == 0:
-            return loss, gx, gw.zero_() if want_grad else None
-        y, coef = y.contiguous(), None if coef is None else coef.contiguous()
-        a = _Args(x.data_ptr(), w.data_ptr(), y.data_ptr(), None if coef is None else coef.data_ptr(), loss.data_ptr(),
-                  None if gx is None else gx.data_ptr(), gw.data_ptr() if want_grad else None, x.stride(0), w.stride(0), n, classes, d,
-                  DTYPES[x.dtype], int(want_grad), KEEP_MB, None, 0, dense.status_ptr(x.device))
-        lib = N.lib()
+    if torch.cuda.current_device() != gpu:
+        with torch.cuda.device(gpu):
+            return softmax_loss(x, w, y, coef, want_grad, want_gx)
+    dev = x.device
+    loss = torch.empty(n, dtype=torch.float32, device=dev)
+    gx = torch.empty((n, d), dtype=x.dtype, device=dev) if want_grad and want_gx else None
+    gw = torch.empty((classes, d), dtype=w.dtype, device=dev) if want_grad else None
+    if n == 0:
+        return loss, gx, gw.zero_() if want_grad else None
+    y, coef = y.contiguous(), None if coef is None else coef.contiguous()
+    px, pw, pgx, pgw = x.data_ptr(), w.data_ptr(), 0 if gx is None else gx.data_ptr(), 0 if gw is None else gw.data_ptr()
+    want = 1 if want_grad else 0
+    lib = N.lib()
+    # the workspace depends on sizes, types and alignment alone
+    key = (n, classes, d, dtype, want, pgx == 0, KEEP_MB, ldx, ldw, px & 15, pw & 15)
+    size = _sizes.get(key)
+    if size is None:
         lib.psb_softmax_loss_workspace.restype = C.c_int64
-        size = lib.psb_softmax_loss_workspace(C.byref(a))
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
-        a.ws, a.ws_bytes = ws.data_ptr(), size
-        N.check(lib.psb_softmax_loss(C.byref(a), N.stream_ptr()), "softmax_loss")
+        size = lib.psb_softmax_loss_workspace(_ARGS.pack(px, pw, 0, 0, 0, pgx, pgw, ldx, ldw, n, classes, d, dtype, want, KEEP_MB, 0, 0, 0))
+        if len(_sizes) >= 1024:
+            _sizes.clear()
+        _sizes[key] = size
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    args = _ARGS.pack(px, pw, y.data_ptr(), 0 if coef is None else coef.data_ptr(), loss.data_ptr(), pgx, pgw, ldx, ldw, n, classes, d,
+                      dtype, want, KEEP_MB, ws.data_ptr(), size, dense.status_ptr(dev))
+    N.check(lib.psb_softmax_loss(args, N.raw_stream(gpu)), "softmax_loss")
     return loss, gx, gw
