@@ -302,7 +302,7 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
   uint64_t *empty = full + C::kStages, *tfull = empty + C::kStages, *tempty = tfull + 2;
   uint32_t* tmem_base = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile uint32_t* abort_flag = tmem_base + 1;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = C::kCtas == 2 ? (int)cluster_rank() : 0;
   const int ntiles = tiles16<C>(g), first = blockIdx.x / C::kCtas, step = gridDim.x / C::kCtas;
 
@@ -325,66 +325,75 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
   __syncthreads();
   if (C::kCtas == 2) cluster_sync_all();       // the peer's barriers are ready before anything is signalled there
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = *tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_base, 0);
   pdl_wait();
 
   if (warp < kG16Epi) {
   if constexpr (C::kPromote) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");    // 384 x 168 registers at launch = 128 x 56 + 256 x 224
-  if (warp == 0 && lane == 0) {
+  bool ok = true;                       // the same in all lanes of a warp
+  if (warp == 0) {
     uint32_t it = 0;
-    for (int t = first; t < ntiles && !*abort_flag; t += step) {
+    for (int t = first; t < ntiles && ok; t += step) {
       const Tile16 w = tile16<C>(g, t);
       const int am = g.a_m0 + w.m0 + rank * 128, bn = g.b_n0 + w.n0 + rank * C::kBRows;
       for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
         const int st = it % C::kStages;
-        if (it >= (uint32_t)C::kStages && !mbar_wait(&empty[st], ((it / C::kStages) - 1) & 1)) { *abort_flag = 1; break; }
-        if (rank == 0) mbar_expect_tx(&full[st], C::kCtas * C::kStageBytes);
+        if (it >= (uint32_t)C::kStages && !(ok = mbar_wait_warp(&empty[st], ((it / C::kStages) - 1) & 1))) break;
         const uint32_t bar = C::kCtas == 2 ? mapa_u32(smem_u32(&full[st]), 0) : smem_u32(&full[st]);
-        const uint32_t sa = smem_u32(stages + st * C::kStageBytes), sb = sa + C::kPlanes * C::kABytes;
+        const uint32_t sa = smem_u32(stages) + st * C::kStageBytes, sb = sa + C::kPlanes * C::kABytes;
+        if (elect_one()) {
+          if (rank == 0) mbar_expect_tx(&full[st], C::kCtas * C::kStageBytes);
 #pragma unroll
-        for (int p = 0; p < C::kPlanes; ++p) {
-          load_operand<C::kCtas, 128>(sa + p * C::kABytes, &g.a, bar, g.a_k0 + kb * kG16K, am, w.z * g.a_z + p, g.a_mn);
-          load_operand<C::kCtas, C::kBRows>(sb + p * C::kBBytes, &g.b, bar, g.b_k0 + kb * kG16K, bn, w.z * g.b_z + p, g.b_mn);
+          for (int p = 0; p < C::kPlanes; ++p) {
+            load_operand<C::kCtas, 128>(sa + p * C::kABytes, &g.a, bar, g.a_k0 + kb * kG16K, am, w.z * g.a_z + p, g.a_mn);
+            load_operand<C::kCtas, C::kBRows>(sb + p * C::kBBytes, &g.b, bar, g.b_k0 + kb * kG16K, bn, w.z * g.b_z + p, g.b_mn);
+          }
         }
+        __syncwarp();
       }
+      ok = ok && __all_sync(0xffffffffu, *abort_flag == 0);
     }
     // the last releases must have landed here before this CTA's shared memory may go away
-    for (uint32_t u = it > (uint32_t)C::kStages ? it - C::kStages : 0; u < it && !*abort_flag; ++u)
-      if (!mbar_wait(&empty[u % C::kStages], (u / C::kStages) & 1)) *abort_flag = 1;
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+    for (uint32_t u = it > (uint32_t)C::kStages ? it - C::kStages : 0; u < it && ok; ++u) ok = mbar_wait_warp(&empty[u % C::kStages], (u / C::kStages) & 1);
+    if (!ok) *abort_flag = 1;
+  } else if (warp == 1 && rank == 0) {
     const uint32_t idesc = idesc16<C>(g);
     // 16 elements of K: 32 bytes of a K-major row, 16 lines of 128 bytes MN-major
     const uint64_t ka = g.a_mn ? 2048 >> 4 : 32 >> 4, kb_ = g.b_mn ? 2048 >> 4 : 32 >> 4;
+    const uint64_t base_a = operand_desc(smem_u32(stages), g.a_mn), base_b = operand_desc(smem_u32(stages) + C::kPlanes * C::kABytes, g.b_mn);
     uint32_t it = 0, n = 0;
-    for (int t = first; t < ntiles && !*abort_flag; t += step) {
+    for (int t = first; t < ntiles && ok; t += step) {
       const Tile16 w = tile16<C>(g, t);
-      for (int kc = w.kb0; kc < w.kb1 && !*abort_flag; kc += C::kChunk, ++n) {
+      for (int kc = w.kb0; kc < w.kb1 && ok; kc += C::kChunk, ++n) {
         const uint32_t acc = n & 1u;
-        if (n >= 2 && !mbar_wait(&tempty[acc], ((n >> 1) - 1) & 1)) { *abort_flag = 1; break; }
+        if (n >= 2 && !(ok = mbar_wait_warp(&tempty[acc], ((n >> 1) - 1) & 1))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t d = tmem + acc * (uint32_t)C::kN;
         const int ke = w.kb1 - kc < C::kChunk ? w.kb1 : kc + C::kChunk;
         uint32_t accumulate = 0;
         for (int kb = kc; kb < ke; ++kb, ++it) {
           const int st = it % C::kStages;
-          if (!mbar_wait(&full[st], (it / C::kStages) & 1)) { *abort_flag = 1; break; }
+          if (!(ok = mbar_wait_warp(&full[st], (it / C::kStages) & 1))) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t sa = smem_u32(stages + st * C::kStageBytes), sb = sa + C::kPlanes * C::kABytes;
+          const uint64_t sa = base_a + (uint32_t)(st * (C::kStageBytes >> 4)), sb = base_b + (uint32_t)(st * (C::kStageBytes >> 4));
+          if (elect_one()) {
 #pragma unroll
-          for (int q = 0; q < (C::kPlanes == 2 ? 3 : 1); ++q) {      // hi·lo, lo·hi, hi·hi
-            const uint64_t da = operand_desc(sa + (q == 1 ? C::kABytes : 0), g.a_mn);
-            const uint64_t db = operand_desc(sb + (C::kPlanes == 2 && q == 0 ? C::kBBytes : 0), g.b_mn);
+            for (int q = 0; q < (C::kPlanes == 2 ? 3 : 1); ++q) {      // hi·lo, lo·hi, hi·hi
+              const uint64_t da = sa + (q == 1 ? C::kABytes >> 4 : 0), db = sb + (C::kPlanes == 2 && q == 0 ? C::kBBytes >> 4 : 0);
 #pragma unroll
-            for (int k = 0; k < kG16K / 16; ++k) {
-              mma16<C::kCtas>(d, da + k * ka, db + k * kb_, idesc, accumulate);
-              accumulate = 1;
+              for (int k = 0; k < kG16K / 16; ++k) mma16<C::kCtas>(d, da + k * ka, db + k * kb_, idesc, q == 0 && k == 0 ? accumulate : 1u);
             }
+            commit16<C::kCtas>(&empty[st]);
           }
-          commit16<C::kCtas>(&empty[st]);
+          __syncwarp();
+          accumulate = 1;
         }
-        commit16<C::kCtas>(&tfull[acc]);
+        if (ok && elect_one()) commit16<C::kCtas>(&tfull[acc]);
+        __syncwarp();
       }
+      ok = ok && __all_sync(0xffffffffu, *abort_flag == 0);
     }
+    if (!ok) *abort_flag = 1;
   }
   } else {
     if constexpr (C::kPromote) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");

@@ -206,19 +206,20 @@ k_orth_sum(const float* __restrict__ slots, int splits, int batch, int n, int ti
 // ------------------------------------------------------------------ matrices that fit into shared memory
 // A matrix whose shorter side is at most 128 stays on the SMs for all of its steps: a cluster of CTAs holds it, each a slice
 // of the longer side, and each the whole of the small squares.  One launch instead of 17, of which each costs 6 us however
-// small it is (64x64: 107 -> 18 us).  Operands lie in shared memory as the tensor cores read them: X [lo][slice] in swizzled rows
-// of 64 columns, which is K-major for X Xᵀ and, the same bytes, MN-major for B X.
+// small it is.  Operands lie in shared memory as the tensor cores read them: X [lo][slice] in swizzled rows of 64 columns,
+// which is K-major for X Xᵀ and, the same bytes, MN-major for B X.
 //   X Xᵀ of the slice -> fp32 sums; a share of them is added up over the CTAs (in their order) and sent to all, as planes
 //   B = A (b I + c A) + a I by every CTA for itself; X = B X of the slice
-// Two planes throughout.  Sums over more than 128 columns have an accumulator for each 128.
+// Two planes throughout.  A product this small takes the tensor cores some 80 cycles whatever its width, so hi·hi and
+// hi·lo are one product: the planes of 64 columns lie behind one another, and rows of both are the N of one instruction.
+// Sums over more than 128 columns have an accumulator for each 128.
 struct SmallArgs {
   OrthArgs o;
   int lo, hi, tall, lop, hs, cl;               // lop: lo in 16s, hs: width of a slice in 64s, cl: CTAs of a cluster
   int a_off, a2_off, p_off;
 };
-constexpr int kSmallThreads = 256;
+constexpr int kSmallThreads = 512, kSmallParts = kSmallThreads / 128;
 
-__device__ __forceinline__ uint32_t mapa(uint32_t addr, int rank, int cl) { return cl > 1 ? mapa_u32(addr, (uint32_t)rank) : addr; }
 __device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint4 v) {
   asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -227,15 +228,26 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ void planes8(const float (&v)[8], uint4& h, uint4& l) {
+__device__ __forceinline__ void st_own_v4(uint32_t addr, uint4 v) {
+  asm volatile("st.shared::cta.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ float4 ld_own_v4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cta.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void planes8(const float* v, uint4& h, uint4& l) {
   uint32_t hs[4], ls[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) OutStage::pair<kFmtPlanes>(v[2 * i], v[2 * i + 1], hs[i], ls[i]);
   h = make_uint4(hs[0], hs[1], hs[2], hs[3]);
   l = make_uint4(ls[0], ls[1], ls[2], ls[3]);
 }
-// byte offset of eight columns (the c8-th eight) of a row in an operand of `rows` rows
-__device__ __forceinline__ int tile_at(int row, int c8, int rows) { return (c8 >> 3) * rows * 128 + row * 128 + (((c8 & 7) ^ (row & 7)) << 4); }
+// Byte offset of eight columns (the c8-th eight) of a row in an operand of `rows` rows: blocks of 64 columns, the hi and then
+// the lo plane of each.
+__device__ __forceinline__ uint32_t tile_at(int row, int c8, int rows) {
+  return (uint32_t)((c8 >> 3) * rows * 256 + row * 128 + (((c8 & 7) ^ (row & 7)) << 4));
+}
 
 __global__ void __launch_bounds__(kSmallThreads, 1)
 k_orth_small(const __grid_constant__ SmallArgs p) {
@@ -243,12 +255,12 @@ k_orth_small(const __grid_constant__ SmallArgs p) {
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ __align__(8) uint64_t done;
   __shared__ uint32_t tmem_base, abort_flag;
-  __shared__ double sums[16], shared_sum[8];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = warp & 3, half = warp >> 2;
+  __shared__ double sums[16], shared_sum[kSmallThreads / 32];
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, q = warp & 3, part = warp >> 2;
   const int rank = p.cl > 1 ? (int)cluster_rank() : 0, z = blockIdx.x / p.cl;
   const int lo = p.lo, lop = p.lop, hs = p.hs, c0 = rank * hs, width = p.hi - c0 < 0 ? 0 : p.hi - c0 < hs ? p.hi - c0 : hs;
   const uint32_t X = smem_u32(base), A = smem_u32(base + p.a_off), A2 = smem_u32(base + p.a2_off), P = smem_u32(base + p.p_off);
-  const uint32_t xlo = (uint32_t)(hs / 64 * lop * 128), alo = (uint32_t)((lop + 63) / 64 * lop * 128);    // from a hi to its lo plane
+  const uint32_t lo_plane = (uint32_t)(lop * 128);          // from a hi to its lo plane
 
   if (tid == 0) {
     mbar_init(&done, 1);
@@ -261,27 +273,69 @@ k_orth_small(const __grid_constant__ SmallArgs p) {
   }
   pdl_wait();
 
-  // momentum and norm
+  // Momentum, norm, and U in fp32 at X's place: eight columns of a row take the bytes of their two planes.  Consecutive
+  // threads go along what is contiguous in memory; the next eight are on their way while these are worked on.
   const int64_t at0 = (int64_t)z * p.o.rows * p.o.cols;
-  double acc = 0.0;
-  for (int i = tid; i < lo * width; i += kSmallThreads) {
-    const int64_t at = at0 + (p.tall ? (int64_t)c0 * lo + i : (int64_t)(i / width) * p.hi + c0 + i % width);
-    float u = load_as(p.o.x, at, p.o.dtype);
-    if (p.o.m != nullptr) {
-      const float mv = p.o.momentum * p.o.m[at] + u;
-      p.o.m[at] = mv;
-      u = update_direction(u, mv, p.o.momentum, p.o.nesterov);
+  const int per_row = hs / 8, eights = lop * per_row;
+  const bool moving = p.o.m != nullptr;
+  const uintptr_t all = reinterpret_cast<uintptr_t>(p.o.x) | reinterpret_cast<uintptr_t>(p.o.m);
+  const bool vec = !p.tall && p.o.dtype == kOrthF32 && (p.hi & 3) == 0 && (all & 15) == 0;
+  struct Eight { int r, c8, left; int64_t at; float u[8], m[8]; };
+  const int64_t by = p.tall ? lo : 1;
+  auto fetch = [&](int i, Eight& e) {
+    e.r = p.tall ? i % lop : i / per_row;
+    e.c8 = p.tall ? i / lop : i % per_row;
+    e.left = i < eights && e.r < lo ? width - e.c8 * 8 : 0;
+    e.at = at0 + (p.tall ? (int64_t)(c0 + e.c8 * 8) * lo + e.r : (int64_t)e.r * p.hi + c0 + e.c8 * 8);
+    if (vec && e.left >= 8) {
+      const float4* xs = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.o.x) + e.at);
+      *reinterpret_cast<float4*>(e.u) = xs[0];
+      *reinterpret_cast<float4*>(e.u + 4) = xs[1];
+      if (moving) {
+        *reinterpret_cast<float4*>(e.m) = *reinterpret_cast<const float4*>(p.o.m + e.at);
+        *reinterpret_cast<float4*>(e.m + 4) = *reinterpret_cast<const float4*>(p.o.m + e.at + 4);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e.u[j] = j < e.left ? load_as(p.o.x, e.at + j * by, p.o.dtype) : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e.m[j] = moving && j < e.left ? p.o.m[e.at + j * by] : 0.f;
     }
-    acc += (double)u * u;
+  };
+  double acc = 0.0;
+  Eight next;
+  fetch(tid, next);
+  for (int i = tid; i < eights; i += kSmallThreads) {
+    Eight e = next;
+    fetch(i + kSmallThreads, next);
+    if (moving) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        e.m[j] = p.o.momentum * e.m[j] + e.u[j];
+        e.u[j] = update_direction(e.u[j], e.m[j], p.o.momentum, p.o.nesterov);
+      }
+      if (vec && e.left >= 8) {
+        *reinterpret_cast<float4*>(p.o.m + e.at) = *reinterpret_cast<float4*>(e.m);
+        *reinterpret_cast<float4*>(p.o.m + e.at + 4) = *reinterpret_cast<float4*>(e.m + 4);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) if (j < e.left) p.o.m[e.at + j * by] = e.m[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc += (double)e.u[j] * e.u[j];
+    const uint32_t to = X + tile_at(e.r, e.c8, lop);
+    st_own_v4(to, *reinterpret_cast<uint4*>(e.u));
+    st_own_v4(to + lo_plane, *reinterpret_cast<uint4*>(e.u + 4));
   }
   acc = warp_sum_d(acc);
   if (lane == 0) shared_sum[warp] = acc;
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
   double total = 0.0;
-  for (int i = 0; i < 8; ++i) total += shared_sum[i];
+  for (int i = 0; i < kSmallThreads / 32; ++i) total += shared_sum[i];
   if (p.cl > 1) {
     cluster_sync_all();                                   // every CTA runs
     if (tid < p.cl)
@@ -291,34 +345,22 @@ k_orth_small(const __grid_constant__ SmallArgs p) {
     for (int i = 0; i < p.cl; ++i) total += sums[i];
   }
   const double f = (double)kNsScale / (sqrt(total) + (double)p.o.eps);
-
-  // X: eight columns of a row at a time, consecutive threads along what is contiguous in memory
-  for (int i = tid; i < lop * (hs / 8); i += kSmallThreads) {
-    const int r = p.tall ? i % lop : i / (hs / 8), c8 = p.tall ? i / lop : i % (hs / 8);
+  for (int i = tid; i < eights; i += kSmallThreads) {      // this thread's own
+    const uint32_t to = X + (p.tall ? tile_at(i % lop, i / lop, lop) : tile_at(i / per_row, i % per_row, lop));
+    const float4 a = ld_own_v4(to), b = ld_own_v4(to + lo_plane);
+    const float u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int c = c8 * 8 + j;
-      v[j] = 0.f;
-      if (r < lo && c < width) {
-        const int64_t at = at0 + (p.tall ? (int64_t)(c0 + c) * lo + r : (int64_t)r * p.hi + c0 + c);
-        float u = load_as(p.o.x, at, p.o.dtype);
-        if (p.o.m != nullptr) u = update_direction(u, p.o.m[at], p.o.momentum, p.o.nesterov);
-        v[j] = (float)((double)u * f);
-      }
-    }
+    for (int j = 0; j < 8; ++j) v[j] = (float)((double)u[j] * f);      // f may lie outside fp32 where U is tiny or huge
     uint4 h, l;
     planes8(v, h, l);
-    const uint32_t to = X + (uint32_t)tile_at(r, c8, lop);
-    st_cluster_v4(to, h);
-    st_cluster_v4(to + xlo, l);
+    st_own_v4(to, h);
+    st_own_v4(to + lo_plane, l);
   }
-  asm volatile("fence.proxy.async;" ::: "memory");
-  __syncthreads();
 
   uint32_t phase = 0;
-  auto finish_products = [&] {                             // the issuing thread, after its products
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&done)) : "memory");
+  auto finish_products = [&] {                             // by warp 0, which issues the products
+    if (elect_one()) asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&done)) : "memory");
   };
   auto wait_products = [&] {
     if (lane == 0 && abort_flag == 0 && !mbar_wait(&done, phase & 1)) abort_flag = 1;
@@ -327,85 +369,90 @@ k_orth_small(const __grid_constant__ SmallArgs p) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   };
   auto operands_ready = [&] {                              // written by all threads, read by the tensor cores next
-    asm volatile("fence.proxy.async;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   };
-  const uint32_t idesc_sq = (1u << 4) | ((uint32_t)(lop >> 3) << 17) | (8u << 24);
-  const int row = q * 32 + lane, groups = (hs + 127) / 128;
+  // 16 sums of this lane's row from a column on, from two accumulators, or more where stride is given
   const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
+  auto add16 = [&](float (&v)[16], uint32_t column) {
+    uint32_t r[16];
+    tmem_load_32x16(lanes + column, r);
+    tmem_load_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(r[j]);
+  };
+  // N = rows of both planes, or of one
+  const uint32_t idesc_both = (1u << 4) | ((uint32_t)(2 * lop >> 3) << 17) | (8u << 24), idesc_one = (1u << 4) | ((uint32_t)(lop >> 3) << 17) | (8u << 24);
+  const uint64_t lo_off = (uint64_t)(lo_plane >> 4), block = (uint64_t)(uint32_t)(lop * 16);      // in units of 16 bytes
+  const int row = q * 32 + lane, groups = (hs + 127) / 128;
+  const bool busy = q * 32 < lop;                          // this warp's lanes hold rows
+  operands_ready();
 
   for (int step = 0; step < p.o.steps; ++step) {
-    // ---- X Xᵀ of the slice, an accumulator for each 128 columns
-    if (tid == 0) {
+    // ---- X Xᵀ of the slice, for each 128 columns: hi·hi in lop columns of TMEM, hi·lo + lo·hi in the next lop
+    if (warp == 0) {
+      const uint64_t x = make_smem_desc(X);
       for (int g = 0; g < groups; ++g) {
+        const uint32_t d = tmem + (uint32_t)(g * 2 * lop);
         uint32_t accumulate = 0;
-        for (int pr = 0; pr < 3; ++pr)                     // hi·lo, lo·hi, hi·hi
-          for (int ch = 2 * g; ch < 2 * g + 2 && ch * 64 < hs; ++ch) {
-            const uint32_t at = X + (uint32_t)(ch * lop * 128);
-            const uint64_t da = make_smem_desc(at + (pr == 1 ? xlo : 0)), db = make_smem_desc(at + (pr == 0 ? xlo : 0));
-            for (int k = 0; k < 4; ++k) {
-              mma16<1>(tmem + (uint32_t)(g * lop), da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc_sq, accumulate);
-              accumulate = 1;
-            }
+        for (int ch = 2 * g; ch < 2 * g + 2 && ch * 64 < hs; ++ch) {
+          const uint64_t at = x + (uint64_t)(uint32_t)ch * block;
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma16<1>(d, at + 2 * k, at + 2 * k, idesc_both, k == 0 ? accumulate : 1u);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma16<1>(d + (uint32_t)lop, at + lo_off + 2 * k, at + 2 * k, idesc_one, 1u);
           }
+          accumulate = 1;
+        }
       }
       finish_products();
     }
     __syncwarp();
     wait_products();
-    if (q * 32 < lop) {
-      for (int u = half; u < lop / 16; u += 2) {
+    if (busy)
+      for (int u = part; u < lop / 16; u += kSmallParts) {
         float v[16] = {};
-        for (int g = 0; g < groups; ++g) {
-          uint32_t r[16];
-          tmem_load_32x16(lanes + (uint32_t)(g * lop + u * 16), r);
-          tmem_load_wait();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(r[j]);
-        }
+        for (int g = 0; g < 2 * groups; ++g) add16(v, (uint32_t)(g * lop + u * 16));
         if (row >= lop) continue;
         if (p.cl > 1) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            st_cluster_v4(P + (uint32_t)(row * lop * 4 + (((u * 4 + j) ^ (row & 3)) << 4)),
-                          make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3])));
+          for (int j = 0; j < 4; ++j) st_own_v4(P + (uint32_t)(row * lop * 4 + (((u * 4 + j) ^ (row & 3)) << 4)), *reinterpret_cast<uint4*>(v + 4 * j));
           continue;
+        }
+        float b[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          v[j] *= kNsInv;
+          b[j] = kNsC * v[j] + (row == u * 16 + j ? kNsB * kNsScale : 0.f);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float a[8], b[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            a[j] = kNsInv * v[e * 8 + j];
-            b[j] = kNsC * a[j] + (row == u * 16 + e * 8 + j ? kNsB * kNsScale : 0.f);
-          }
           uint4 h, l;
-          const uint32_t at = (uint32_t)tile_at(row, u * 2 + e, lop);
-          planes8(a, h, l);
-          st_cluster_v4(A + at, h);
-          st_cluster_v4(A + at + alo, l);
-          planes8(b, h, l);
-          st_cluster_v4(A2 + at, h);
-          st_cluster_v4(A2 + at + alo, l);
+          const uint32_t at = tile_at(row, u * 2 + e, lop);
+          planes8(v + 8 * e, h, l);
+          st_own_v4(A + at, h);
+          st_own_v4(A + at + lo_plane, l);
+          planes8(b + 8 * e, h, l);
+          st_own_v4(A2 + at, h);
+          st_own_v4(A2 + at + lo_plane, l);
         }
       }
-    }
     if (p.cl > 1) {
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       cluster_sync_all();
       const int units = lop * lop / 8, per = (units + p.cl - 1) / p.cl;
       for (int i = rank * per + tid; i < (rank + 1) * per && i < units; i += kSmallThreads) {
         const int r = i / (lop / 8), c8 = i % (lop / 8);
-        float v[8] = {};
+        float v[8] = {}, b[8];
         for (int s = 0; s < p.cl; ++s)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float4 t = ld_cluster_v4(mapa_u32(P + (uint32_t)(r * lop * 4 + (((c8 * 2 + e) ^ (r & 3)) << 4)), (uint32_t)s));
             v[4 * e] += t.x; v[4 * e + 1] += t.y; v[4 * e + 2] += t.z; v[4 * e + 3] += t.w;
           }
-        float b[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           v[j] *= kNsInv;
@@ -414,13 +461,13 @@ k_orth_small(const __grid_constant__ SmallArgs p) {
         uint4 ah, al, bh, bl;
         planes8(v, ah, al);
         planes8(b, bh, bl);
-        const uint32_t at = (uint32_t)tile_at(r, c8, lop);
+        const uint32_t at = tile_at(r, c8, lop);
         for (int s = 0; s < p.cl; ++s) {
           const uint32_t to = mapa_u32(A + at, (uint32_t)s), to2 = mapa_u32(A2 + at, (uint32_t)s);
           st_cluster_v4(to, ah);
-          st_cluster_v4(to + alo, al);
+          st_cluster_v4(to + lo_plane, al);
           st_cluster_v4(to2, bh);
-          st_cluster_v4(to2 + alo, bl);
+          st_cluster_v4(to2 + lo_plane, bl);
         }
       }
       asm volatile("fence.proxy.async;" ::: "memory");
@@ -429,105 +476,169 @@ k_orth_small(const __grid_constant__ SmallArgs p) {
     operands_ready();
 
     // ---- B = A (b I + c A) + a I, into A's place
-    if (tid == 0) {
-      uint32_t accumulate = 0;
-      for (int pr = 0; pr < 3; ++pr)
-        for (int k = 0; k < lop / 16; ++k) {
-          const uint32_t off = (uint32_t)((k >> 2) * lop * 128 + (k & 3) * 32);
-          mma16<1>(tmem, make_smem_desc(A + (pr == 1 ? alo : 0) + off), make_smem_desc(A2 + (pr == 0 ? alo : 0) + off), idesc_sq, accumulate);
-          accumulate = 1;
+    if (warp == 0) {
+      const uint64_t a = make_smem_desc(A), a2 = make_smem_desc(A2);
+      for (int ch = 0; ch * 64 < lop; ++ch) {
+        const uint64_t off = (uint64_t)(uint32_t)ch * block;
+        const int ks = lop - ch * 64 < 64 ? (lop - ch * 64) / 16 : 4;
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < ks) mma16<1>(tmem, a + off + 2 * k, a2 + off + 2 * k, idesc_both, ch > 0 || k > 0 ? 1u : 0u);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < ks) mma16<1>(tmem + (uint32_t)lop, a + off + lo_off + 2 * k, a2 + off + 2 * k, idesc_one, 1u);
         }
+      }
       finish_products();
     }
     __syncwarp();
     wait_products();
-    if (q * 32 < lop) {
-      for (int u = half; u < lop / 16; u += 2) {
-        uint32_t r[16];
-        tmem_load_32x16(lanes + (uint32_t)(u * 16), r);
-        tmem_load_wait();
+    if (busy)
+      for (int u = part; u < lop / 16; u += kSmallParts) {
+        float v[16] = {};
+        add16(v, (uint32_t)(u * 16));
+        add16(v, (uint32_t)(lop + u * 16));
         if (row >= lop) continue;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float b[8];
+        for (int j = 0; j < 16; ++j) v[j] = kNsInv * v[j] + (row == u * 16 + j ? kNsA * kNsScale : 0.f);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) b[j] = kNsInv * __uint_as_float(r[e * 8 + j]) + (row == u * 16 + e * 8 + j ? kNsA * kNsScale : 0.f);
+        for (int e = 0; e < 2; ++e) {
           uint4 h, l;
-          const uint32_t at = (uint32_t)tile_at(row, u * 2 + e, lop);
-          planes8(b, h, l);
-          st_cluster_v4(A + at, h);
-          st_cluster_v4(A + at + alo, l);
+          const uint32_t at = tile_at(row, u * 2 + e, lop);
+          planes8(v + 8 * e, h, l);
+          st_own_v4(A + at, h);
+          st_own_v4(A + at + lo_plane, l);
         }
       }
-    }
     operands_ready();
 
-    // ---- X = B X of the slice; X is MN-major here: chunks of 64 columns, lop lines each
-    if (tid == 0) {
+    // ---- X = B X of the slice; X is MN-major here: blocks of 64 columns, lop lines of the hi plane and as many of the lo.
+    // Up to 128 columns both planes are one N (their blocks take turns in TMEM), beyond that N is wide enough.
+    const bool both = hs <= 128;
+    if (warp == 0) {
+      const uint64_t b = make_smem_desc(A), x = make_smem_desc(X), plane_lead = (uint64_t)((lop * 128) >> 4) << 16, block_lead = plane_lead << 1;
       for (int n0 = 0; n0 < hs; n0 += 256) {
         const int n = hs - n0 < 256 ? hs - n0 : 256;
-        const uint32_t idesc = (1u << 4) | (1u << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
-        const uint64_t lead = (uint64_t)((lop * 128) >> 4) << 16;
-        uint32_t accumulate = 0;
-        for (int pr = 0; pr < 3; ++pr)
-          for (int k = 0; k < lop / 16; ++k) {
-            const uint32_t off = (uint32_t)((k >> 2) * lop * 128 + (k & 3) * 32);
-            mma16<1>(tmem + (uint32_t)n0, make_smem_desc(A + (pr == 1 ? alo : 0) + off),
-                     make_smem_desc(X + (pr == 0 ? xlo : 0) + (uint32_t)(n0 / 64 * lop * 128 + k * 2048)) | lead, idesc, accumulate);
-            accumulate = 1;
+        const uint32_t mn = (1u << 4) | (1u << 16) | (8u << 24), one = mn | ((uint32_t)(n >> 3) << 17), two = mn | ((uint32_t)(2 * n >> 3) << 17);
+        const uint64_t at = x + (uint64_t)(uint32_t)(n0 / 64) * block;
+        for (int ch = 0; ch * 64 < lop; ++ch) {
+          const uint64_t off = b + (uint64_t)(uint32_t)ch * block, lines = (uint64_t)(uint32_t)(ch * 512);       // 64 lines
+          const int ks = lop - ch * 64 < 64 ? (lop - ch * 64) / 16 : 4;
+          if (elect_one()) {
+            if (both) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (k < ks) mma16<1>(tmem, off + 2 * k, (at + lines + 128 * k) | plane_lead, two, ch > 0 || k > 0 ? 1u : 0u);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (k < ks) mma16<1>(tmem + (uint32_t)(2 * hs), off + lo_off + 2 * k, (at + lines + 128 * k) | block_lead, one, ch > 0 || k > 0 ? 1u : 0u);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (k < ks) mma16<1>(tmem + (uint32_t)n0, off + 2 * k, (at + lo_off + lines + 128 * k) | block_lead, one, ch > 0 || k > 0 ? 1u : 0u);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (k < ks) mma16<1>(tmem + (uint32_t)n0, off + lo_off + 2 * k, (at + lines + 128 * k) | block_lead, one, 1u);
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (k < ks) mma16<1>(tmem + (uint32_t)n0, off + 2 * k, (at + lines + 128 * k) | block_lead, one, 1u);
+            }
           }
+        }
       }
       finish_products();
     }
     __syncwarp();
     wait_products();
     const bool last = step + 1 == p.o.steps;
-    if (q * 32 < lop && !last) {
-      for (int u = half; u < hs / 16; u += 2) {
-        uint32_t r[16];
-        tmem_load_32x16(lanes + (uint32_t)(u * 16), r);
-        tmem_load_wait();
-        if (row >= lop) continue;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = kNsInv * __uint_as_float(r[e * 8 + j]);
-          uint4 h, l;
-          const uint32_t at = (uint32_t)tile_at(row, u * 2 + e, lop);
-          planes8(x, h, l);
-          st_cluster_v4(X + at, h);
-          st_cluster_v4(X + at + xlo, l);
+    if (busy)
+      for (int u = part; u < hs / 16; u += kSmallParts) {
+        float v[16] = {};
+        if (both) {
+          const uint32_t at = (uint32_t)((u >> 2) * 128 + (u & 3) * 16);
+          add16(v, at);
+          add16(v, at + 64);
+          add16(v, (uint32_t)(2 * hs + u * 16));
+        } else {
+          add16(v, (uint32_t)(u * 16));
         }
-      }
-    } else if (q * 32 < lop) {
-      auto put = [&](int64_t at, float x) {
-        if (p.o.m != nullptr) reinterpret_cast<float*>(p.o.out)[at] -= p.o.lr * x;
-        else if (p.o.dtype == kOrthF32) reinterpret_cast<float*>(p.o.out)[at] = x;
-        else if (p.o.dtype == kOrthBF16) reinterpret_cast<__nv_bfloat16*>(p.o.out)[at] = __float2bfloat16_rn(x);
-        else reinterpret_cast<__half*>(p.o.out)[at] = __float2half_rn(x);
-      };
-      float* st = reinterpret_cast<float*>(base + p.p_off + warp * 4096);
-      for (int c = half * 32; c < hs; c += 64) {
-        uint32_t r[32];
-        tmem_load_32x32(lanes + (uint32_t)c, r);
-        tmem_load_wait();
-        if (p.tall) {                                      // lanes are neighbours in memory
+        if (row >= lop) continue;
+        if (!last) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (row < lo && c + j < width) put(at0 + (int64_t)(c0 + c + j) * lo + row, kNsInv * kNsInv * __uint_as_float(r[j]));
+          for (int j = 0; j < 16; ++j) v[j] *= kNsInv;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint4 h, l;
+            const uint32_t at = tile_at(row, u * 2 + e, lop);
+            planes8(v + 8 * e, h, l);
+            st_own_v4(X + at, h);
+            st_own_v4(X + at + lo_plane, l);
+          }
           continue;
         }
-        __syncwarp();
+        // the result in fp32 over X (and, by a column of each row, A): as it lies in memory, for all threads to store
 #pragma unroll
-        for (int j = 0; j < 32; ++j) st[lane * 32 + (j ^ lane)] = kNsInv * kNsInv * __uint_as_float(r[j]);
-        __syncwarp();
-#pragma unroll 8
-        for (int i = 0; i < 32; ++i)
-          if (q * 32 + i < lo && c + lane < width) put(at0 + (int64_t)(q * 32 + i) * p.hi + c0 + c + lane, st[i * 32 + (lane ^ i)]);
+        for (int j = 0; j < 16; ++j) v[j] *= kNsInv * kNsInv;
+        if (p.tall) {
+          float* st = reinterpret_cast<float*>(base);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) st[(u * 16 + j) * (lop + 1) + row] = v[j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) st_own_v4(X + (uint32_t)(row * hs * 4 + (((u * 4 + j) ^ (row & 7)) << 4)), *reinterpret_cast<uint4*>(v + 4 * j));
+        }
+      }
+    operands_ready();
+  }
+
+  // four neighbours at a time; old weights of the next four are on their way while these are stored
+  {
+    const float* st = reinterpret_cast<const float*>(base);
+    float* wts = reinterpret_cast<float*>(p.o.out);
+    const int per = p.tall ? (lo * width + 3) / 4 : (width + 3) / 4, fours = p.tall ? per : per * lo;
+    const bool vec_out = p.o.dtype == kOrthF32 || moving ? (reinterpret_cast<uintptr_t>(p.o.out) & 15) == 0 && ((p.tall ? lo * (int64_t)c0 | (int64_t)p.o.rows * p.o.cols : p.hi) & 3) == 0 : false;
+    struct Four { int left, r, c; int64_t at; float w[4]; };
+    auto fetch4 = [&](int i, Four& t) {
+      t.r = p.tall ? 0 : i / per;
+      t.c = (p.tall ? i : i % per) * 4;
+      t.left = i < fours ? (p.tall ? lo * width : width) - t.c : 0;
+      t.at = at0 + (p.tall ? (int64_t)c0 * lo : (int64_t)t.r * p.hi + c0) + t.c;
+      if (!moving) return;
+      if (vec_out && t.left >= 4) *reinterpret_cast<float4*>(t.w) = *reinterpret_cast<const float4*>(wts + t.at);
+      else
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t.w[j] = j < t.left ? wts[t.at + j] : 0.f;
+    };
+    Four ahead[2];
+    fetch4(tid, ahead[0]);
+    fetch4(tid + kSmallThreads, ahead[1]);
+    for (int i = tid; i < fours; i += kSmallThreads) {
+      Four t = ahead[0];
+      ahead[0] = ahead[1];
+      fetch4(i + 2 * kSmallThreads, ahead[1]);
+      float v[4];
+      if (p.tall) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { const int e = t.c + j; v[j] = j < t.left ? st[e / lo * (lop + 1) + e % lo] : 0.f; }
+      } else {
+        *reinterpret_cast<float4*>(v) = ld_own_v4(X + (uint32_t)(t.r * hs * 4 + (((t.c >> 2) ^ (t.r & 7)) << 4)));
+      }
+      if (moving)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = t.w[j] - p.o.lr * v[j];
+      if (vec_out && t.left >= 4) {
+        *reinterpret_cast<float4*>(wts + t.at) = *reinterpret_cast<float4*>(v);
+        continue;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (j >= t.left) continue;
+        if (moving || p.o.dtype == kOrthF32) wts[t.at + j] = v[j];
+        else if (p.o.dtype == kOrthBF16) reinterpret_cast<__nv_bfloat16*>(p.o.out)[t.at + j] = __float2bfloat16_rn(v[j]);
+        else reinterpret_cast<__half*>(p.o.out)[t.at + j] = __float2half_rn(v[j]);
       }
     }
-    operands_ready();
   }
   if (tid == 0 && abort_flag != 0) set_status(p.o.status, kWaitTimeout, blockIdx.x, 500);
   if (p.cl > 1) cluster_sync_all();
@@ -549,24 +660,29 @@ struct OrthPlan {
 };
 
 constexpr int kSmallSmem = 226 * 1024;      // of 227 KB
-// The fewest CTAs that hold a matrix with a short side of at most 128, if 16 do.
-bool small_plan(OrthPlan& p) {
+// How many CTAs hold a matrix with a short side of at most 128: the cheapest number by this estimate of a step's cycles,
+// which follows clock readings of 64x64 (5.4 k, one CTA), 128x128 (18 k, one) and 64x2048 (17.8 k on 4 CTAs).
+bool small_plan(OrthPlan& p, int batch) {
   if (p.lo > 128) return false;
   p.lop = (p.lo + 15) / 16 * 16;
   const int square = 4 * p.lop * ((p.lop + 63) / 64 * 64);
+  double least = 1e300;
   for (int cl = 1; cl <= 16; cl *= 2) {
     const int64_t hs = (((int64_t)p.hi + cl - 1) / cl + 63) / 64 * 64;
-    if (hs > 512 || (hs + 127) / 128 * p.lop > 512) continue;
-    const int sums = cl > 1 ? 4 * p.lop * p.lop : 0, stage = sums > 32768 ? sums : 32768;      // 4 KB a warp for the result
-    const int bytes = 4 * p.lop * (int)hs + 2 * square + stage + (128 - p.lop) * 128;       // tiles are read as 128 rows
+    if (hs > 512 || (hs + 127) / 128 * 2 * p.lop > 512) continue;                            // of TMEM
+    const int sums = cl > 1 ? 4 * p.lop * p.lop : 0;
+    const int bytes = 4 * p.lop * (int)hs + 2 * square + sums + (128 - p.lop) * 128;        // tiles are read as 128 rows
     if (bytes + 1024 > kSmallSmem) continue;
+    const double rounds = (double)(((int64_t)batch * cl + 147) / 148), wide = p.lop > 64 ? 2.0 : 1.0;
+    const double t = rounds * (wide * (4000.0 + 20.0 * (double)hs) + (cl > 1 ? 4500.0 : 0.0));
+    if (t >= least) continue;
+    least = t;
     p.hs = (int)hs; p.cl = cl;
     p.a_off = 4 * p.lop * p.hs; p.a2_off = p.a_off + square; p.p_off = p.a2_off + square;
     // more than half of an SM's shared memory, so that no two CTAs of a cluster meet on an SM: each takes all of its TMEM
     p.smem = bytes + 1024 < 120 * 1024 ? 120 * 1024 : bytes + 1024;
-    return true;
   }
-  return false;
+  return least < 1e300;
 }
 
 bool orth_args_ok(const OrthArgs& a) {
@@ -584,7 +700,7 @@ OrthPlan make_orth_plan(const OrthKey& a) {
   p.tall = a.rows > a.cols;
   p.lo = p.tall ? a.cols : a.rows;
   p.hi = p.tall ? a.rows : a.cols;
-  if ((int64_t)a.batch * 16 < (1 << 30) && small_plan(p)) { p.small = 1; return p; }
+  if ((int64_t)a.batch * 16 < (1 << 30) && small_plan(p, a.batch)) { p.small = 1; return p; }
   int64_t slots = 0;
   for (int k = 0; k < 2; ++k) {
     p.gram[k] = choose_tiling(a.batch, p.lo, p.lo, p.hi, k + 1, true, 32);
