@@ -57,6 +57,9 @@ struct Gemm16Args {
   int a_mn, b_mn;              // an operand is MN-major
   int sym;                     // square result that is symmetric: only tiles on and above the diagonal
   int bf16;                    // operands are bf16, else fp16
+  int a_bytes, b_bytes;        // of a stage and plane that copies bring (launch16 sets them and k_steps)
+  int k_steps;                 // steps of 16 elements in a block of K
+  int clear;                   // what copies leave out of the stages has to be zero
   uint32_t* status;
 };
 
@@ -321,6 +324,10 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
   }
+  if (g.clear) {
+    for (int i = threadIdx.x; i < C::kStages * C::kStageBytes / 16; i += kG16Threads) reinterpret_cast<uint4*>(stages)[i] = make_uint4(0, 0, 0, 0);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (C::kCtas == 2) cluster_sync_all();       // the peer's barriers are ready before anything is signalled there
@@ -342,7 +349,7 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
         const uint32_t bar = C::kCtas == 2 ? mapa_u32(smem_u32(&full[st]), 0) : smem_u32(&full[st]);
         const uint32_t sa = smem_u32(stages) + st * C::kStageBytes, sb = sa + C::kPlanes * C::kABytes;
         if (elect_one()) {
-          if (rank == 0) mbar_expect_tx(&full[st], C::kCtas * C::kStageBytes);
+          if (rank == 0) mbar_expect_tx(&full[st], (uint32_t)(C::kCtas * C::kPlanes * (g.a_bytes + g.b_bytes)));
 #pragma unroll
           for (int p = 0; p < C::kPlanes; ++p) {
             load_operand<C::kCtas, 128>(sa + p * C::kABytes, &g.a, bar, g.a_k0 + kb * kG16K, am, w.z * g.a_z + p, g.a_mn);
@@ -381,7 +388,8 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
             for (int q = 0; q < (C::kPlanes == 2 ? 3 : 1); ++q) {      // hi·lo, lo·hi, hi·hi
               const uint64_t da = sa + (q == 1 ? C::kABytes >> 4 : 0), db = sb + (C::kPlanes == 2 && q == 0 ? C::kBBytes >> 4 : 0);
 #pragma unroll
-              for (int k = 0; k < kG16K / 16; ++k) mma16<C::kCtas>(d, da + k * ka, db + k * kb_, idesc, q == 0 && k == 0 ? accumulate : 1u);
+              for (int k = 0; k < kG16K / 16; ++k)
+                if (k < g.k_steps) mma16<C::kCtas>(d, da + k * ka, db + k * kb_, idesc, q == 0 && k == 0 ? accumulate : 1u);
             }
             commit16<C::kCtas>(&empty[st]);
           }
@@ -550,9 +558,19 @@ int launch16(Chain& chain, psb::Gemm16Args& g, const Operand16& a, const Operand
   int dev = 0;
   const int sms = sm_count(&dev);
   if (sms <= 0) return (int)cudaErrorInvalidDevice;
-  int r = make_map16(&g.a, a.base, g.bf16, a.rows, a.cols, a.ld, a.stride, a.count, g.a_mn ? 64 : 128);
-  if (r == 0) r = make_map16(&g.b, b.base, g.bf16, b.rows, b.cols, b.ld, b.stride, b.count, g.b_mn ? 64 : C::kBRows);
+  // A copy that fills in rows from outside a matrix takes 2 to 3 cycles a row: one row of x in a box of 128 made scores of
+  // 400,000 classes take 190 us instead of 134.  Boxes are no higher than the matrix.  Rows of K-major operands that no copy
+  // brings may hold anything: their results are rows or columns that do not exist.  Lines of MN-major operands are
+  // elements of K and have to be zero; K is one block then, and the stages are cleared before the first.
+  auto up8 = [](int64_t v, int most) { return v >= most ? most : (int)((v + 7) / 8 * 8); };
+  const int lines = up8(g.K, psb::kG16K), ra = g.a_mn ? lines : up8(g.M, 128), rb = g.b_mn ? lines : up8(g.N, C::kBRows);
+  int r = make_map16(&g.a, a.base, g.bf16, a.rows, a.cols, a.ld, a.stride, a.count, ra);
+  if (r == 0) r = make_map16(&g.b, b.base, g.bf16, b.rows, b.cols, b.ld, b.stride, b.count, rb);
   if (r) return r;
+  g.a_bytes = ra * 128 * (g.a_mn ? 2 : 1);
+  g.b_bytes = rb * 128 * (g.b_mn ? C::kBRows / 64 : 1);
+  g.k_steps = g.K >= psb::kG16K ? psb::kG16K / 16 : (g.K + 15) / 16;
+  g.clear = (g.a_mn || g.b_mn) && lines < psb::kG16K;
   static bool attr[kMaxDevices] = {};
   if (!attr[dev]) {
     cudaError_t e = cudaFuncSetAttribute(psb::gemm16_kernel<C, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
@@ -572,7 +590,7 @@ inline int tiling_cols(int kind) { return kind == kPair256 ? 256 : kind == kOne1
 
 // The cheapest by this estimate, in cycles of an SM: rounds of tiles, each its blocks of K at the slower of the tensor
 // cores (128 x N x 64 in 2N cycles a product, as a rule) and the loads (48 bytes a cycle from L2, as measured with all SMs
-// busy), plus what does not overlap in the last round, plus storing and adding up the pieces of K (at 3000 bytes a cycle).
+// busy), plus what does not overlap in the last round, plus storing and adding up the pieces of K (a launch, 5000 bytes a cycle).
 inline Tiling choose_tiling(int64_t batch, int64_t M, int64_t N, int64_t K, int planes, bool sym, int max_splits, int only = -1) {
   const int64_t nkb = (K + psb::kG16K - 1) / psb::kG16K;
   Tiling best = {kOne64, 1, (int)nkb};
@@ -590,7 +608,7 @@ inline Tiling choose_tiling(int64_t batch, int64_t M, int64_t N, int64_t K, int 
       if (s > 1 && per < 4) break;
       const int64_t rounds = (tiles * s + slots - 1) / slots;
       double t = (double)rounds * (double)per * (mma > load ? mma : load) + 12.0 * (double)cols + 600.0 * (double)rounds;
-      if (s > 1) t += 4500.0 + (double)batch * M * N * (8.0 * s + 4.0) / 3000.0;
+      if (s > 1) t += 5000.0 + (double)batch * M * N * (8.0 * s + 4.0) / 5000.0;
       if (t < least) { least = t; best = {kind, (int)s, (int)per}; }
     }
   }

@@ -178,29 +178,57 @@ struct EpiNs {
 };
 
 // The splits of a product's K to planes: alpha · sum + beta · I, and the second matrix.  Of a symmetric product only the
-// tiles (tile x tile) on and above the diagonal exist.
+// tiles (tile x tile) on and above the diagonal exist.  A block takes 32 x 32, a thread four neighbours, and stores them
+// and, through shared memory, their transpose.
 __global__ void __launch_bounds__(256)
 k_orth_sum(const float* __restrict__ slots, int splits, int batch, int n, int tile, uint16_t* __restrict__ out, uint16_t* __restrict__ out2,
            int64_t ld, int64_t plane, float alpha, float beta, float alpha2, float beta2) {
+  __shared__ float sum[32][33];
+  const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32, z = blockIdx.z;
+  if (r0 / tile > c0 / tile) return;
+  const bool twice = r0 / tile < c0 / tile;
   pdl_wait();
-  const int64_t per = (int64_t)n * n, total = per * batch;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t z = i / per;
-    const int e = (int)(i - z * per), r = e / n, c = e - r * n;
-    if (r / tile > c / tile) continue;
-    float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += slots[s * total + i];
-    const int64_t at = z * 2 * plane + (int64_t)r * ld + c, mirror = z * 2 * plane + (int64_t)c * ld + r;
-    const bool twice = r / tile < c / tile;
-    __half h, l;
-    split16(alpha * v + (r == c ? beta : 0.f), h, l);
-    out[at] = __half_as_ushort(h); out[at + plane] = __half_as_ushort(l);
-    if (twice) { out[mirror] = __half_as_ushort(h); out[mirror + plane] = __half_as_ushort(l); }
-    if (out2 == nullptr) continue;
-    split16(alpha2 * v + (r == c ? beta2 : 0.f), h, l);
-    out2[at] = __half_as_ushort(h); out2[at + plane] = __half_as_ushort(l);
-    if (twice) { out2[mirror] = __half_as_ushort(h); out2[mirror + plane] = __half_as_ushort(l); }
+  const int ty = threadIdx.x >> 3, tx = (threadIdx.x & 7) * 4;
+  const int64_t per = (int64_t)n * n, total = per * batch, base = (int64_t)z * 2 * plane;
+  const float* src = slots + z * per + (int64_t)(r0 + ty) * n + c0 + tx;
+  float v[4] = {};
+  if (r0 + ty < n && c0 + tx < n) {
+    if ((n & 3) == 0) {
+#pragma unroll 8
+      for (int s = 0; s < splits; ++s) {
+        const float4 t = *reinterpret_cast<const float4*>(src + s * total);
+        v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
+      }
+    } else {
+#pragma unroll 4
+      for (int s = 0; s < splits; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += c0 + tx + j < n ? src[s * total + j] : 0.f;
+    }
   }
+  // four elements of row r from column c on; rows are padded to 8 elements and what lies behind their end is not read
+  auto put = [&](int r, int c, const float (&x)[4]) {
+    const int64_t at = base + (int64_t)r * ld + c;
+    uint2 h, l;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      if (m == 1 && out2 == nullptr) break;
+      float y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = (m ? alpha2 : alpha) * x[j] + (r == c + j ? (m ? beta2 : beta) : 0.f);
+      OutStage::pair<kFmtPlanes>(y[0], y[1], h.x, l.x);
+      OutStage::pair<kFmtPlanes>(y[2], y[3], h.y, l.y);
+      *reinterpret_cast<uint2*>((m ? out2 : out) + at) = h;
+      *reinterpret_cast<uint2*>((m ? out2 : out) + at + plane) = l;
+    }
+  };
+  if (r0 + ty < n && c0 + tx < n) put(r0 + ty, c0 + tx, v);
+  if (!twice) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum[ty][tx + j] = v[j];
+  __syncthreads();
+  const float t[4] = {sum[tx][ty], sum[tx + 1][ty], sum[tx + 2][ty], sum[tx + 3][ty]};       // column ty, a row of the mirror image
+  if (c0 + ty < n && r0 + tx < n) put(c0 + ty, r0 + tx, t);
 }
 
 // ------------------------------------------------------------------ matrices that fit into shared memory
@@ -780,7 +808,6 @@ int psb_orthogonal(const OrthArgs* ap, cudaStream_t s) {
   if (r) return r;
 
   const bool precise = a.m != nullptr || a.dtype != kOrthBF16;
-  const int64_t lo2 = (int64_t)a.batch * p.lo * p.lo;
   const Operand16 A{ab, p.lo, p.lo, p.ldl, p.lplane, 2 * a.batch}, A2{a2, p.lo, p.lo, p.ldl, p.lplane, 2 * a.batch},
       B{bb, p.lo, p.lo, p.ldl, p.lplane, 2 * a.batch};
   Gemm16Args g = {};
@@ -795,8 +822,8 @@ int psb_orthogonal(const OrthArgs* ap, cudaStream_t s) {
     if (t.splits > 1) e.slots = slots;
     int rc = product16<EpiNs>(chain, planes, t.kind, q, x, y, e);
     if (rc == 0 && t.splits > 1) {
-      const int64_t sb = (lo2 + 255) / 256;
-      rc = chain.launch(k_orth_sum, dim3((unsigned)(sb < 148 * 8 ? sb : 148 * 8)), 256, 0, 1, slots, t.splits, a.batch, p.lo, tiling_rows(t.kind), out, out2,
+      const unsigned nt = (unsigned)((p.lo + 31) / 32);
+      rc = chain.launch(k_orth_sum, dim3(nt, nt, (unsigned)a.batch), 256, 0, 1, slots, t.splits, a.batch, p.lo, tiling_rows(t.kind), out, out2,
                         p.ldl, p.lplane, e.alpha, e.beta, e.alpha2, e.beta2);
     }
     return rc;
