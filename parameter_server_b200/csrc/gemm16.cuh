@@ -17,7 +17,8 @@
 //                       double-buffered, so a tile's epilogue runs under the next tile's products
 // Sums of planes need 128 registers of an epilogue thread: its warps take over registers of the other four.
 // 16-bit results leave through shared memory as TMA stores of 32 x 32 boxes: a lane holds a row, and stores of rows by
-// lanes touch 32 lines an instruction (4096 x 4096 Newton-Schulz step: 2.6 times the time).
+// lanes touch 32 lines an instruction (4096 x 4096 Newton-Schulz step: 2.6 times the time; 16-byte stores of what the warp
+// turned round in shared memory: 1.05 times).
 // Launches of one call overlap: a kernel sets itself up while the one before it drains (programmatic dependent launch) and
 // waits for it before it touches memory.
 // No load is a multicast.
@@ -167,6 +168,14 @@ __device__ __forceinline__ uint32_t pack_half2(__half a, __half b) {
 }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
+// the columns from col to col + kHalf of a row of n floats, towards L2
+template <int kHalf>
+__device__ __forceinline__ void prefetch_l2(const float* row, int col, int n) {
+#pragma unroll
+  for (int c = 0; c < kHalf; c += 32)
+    if (col + c < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + col + c));
+}
+
 enum : int { kFmtF16 = 0, kFmtBF16 = 1, kFmtPlanes = 2 };      // fp16, bf16, hi and lo planes of fp16
 
 // An epilogue warp's way to global memory: its 4 KB of shared memory.  v: 32 columns from col on of this lane's row of the
@@ -175,80 +184,67 @@ struct OutStage {
   uint32_t addr;
   float* f;
   int lane;
+
   uint32_t turn = 0;
 
-  // The buffer that the next store uses, free again: one of two for one plane, the whole for two.
-  __device__ __forceinline__ uint32_t acquire(bool two) {
-    if (lane == 0) {
-      if (two) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-      else asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-    }
+  // The buffer that the next store uses, free again: the one before last has been read.
+  __device__ __forceinline__ uint32_t acquire() {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
     __syncwarp();
-    const uint32_t a = two ? addr : addr + (turn & 1u) * 2048u;
-    ++turn;
-    return a;
+    return addr + (turn++ & 1u) * 2048u;
   }
-  __device__ __forceinline__ void store_box(uint32_t src, const CUtensorMap* map, int x, int y, int z, bool two) {
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
-    if (lane == 0) {
-      asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
-                   ::"l"(map), "r"(x), "r"(y), "r"(z), "r"(src) : "memory");
-      if (two)
-        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
-                     ::"l"(map), "r"(x), "r"(y), "r"(z + 1), "r"(src + 2048u) : "memory");
-      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-    }
-  }
-  // 32 x 32 box, rows of 64 bytes, 64-byte swizzle (16-byte piece j of row r lies at j ^ ((r / 2) % 4)): free of bank conflicts.
-  // What lies outside the map is not written.
+  // 32 x 32 boxes in the format, a plane at a time, as they are and, for a mirror image, transposed.  Rows of 64 bytes, 64-byte
+  // swizzle (16-byte piece j of row r lies at j ^ ((r / 2) % 4)): free of bank conflicts.  What lies outside the map is not
+  // written.  A tile's epilogue runs once or a few times a launch, so its code is kept short.
   template <int fmt>
   __device__ __forceinline__ void store(const CUtensorMap* map, const float (&v)[32], int row, int col, int z, bool mirror) {
-    constexpr bool two = fmt == kFmtPlanes;
-    uint32_t a = acquire(two);
-    const uint32_t mine = a + (uint32_t)lane * 64u, sw = ((uint32_t)lane >> 1) & 3u;
+    const int planes = fmt == kFmtPlanes ? 2 : 1, passes = mirror ? 2 * planes : planes;
+#pragma unroll 1
+    for (int pass = 0; pass < passes; ++pass) {
+      const bool turned = pass >= planes, low = fmt == kFmtPlanes && (pass & 1);
+      uint32_t h[16];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t h[4], l[4];
+      for (int j = 0; j < 16; ++j) h[j] = pair<fmt>(v[2 * j], v[2 * j + 1], low);
+      const uint32_t a = acquire();
+      if (!turned) {
+        const uint32_t mine = a + (uint32_t)lane * 64u, sw = ((uint32_t)lane >> 1) & 3u;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pair<fmt>(v[8 * j + 2 * i], v[8 * j + 2 * i + 1], h[i], l[i]);
-      const uint32_t to = mine + (((uint32_t)j ^ sw) << 4);
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
-      if (two) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 2048u), "r"(l[0]), "r"(l[1]), "r"(l[2]), "r"(l[3]) : "memory");
-    }
-    store_box(a, map, col, row, z, two);
-    if (!mirror) return;
-    // the transposed box: row j holds column j, this lane's element
-    a = acquire(two);
+        for (int j = 0; j < 4; ++j)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + (((uint32_t)j ^ sw) << 4)), "r"(h[4 * j]), "r"(h[4 * j + 1]),
+                       "r"(h[4 * j + 2]), "r"(h[4 * j + 3]) : "memory");
+      } else {                                             // row j holds column j, this lane's element
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-      uint32_t h, l;
-      pair<fmt>(v[j], v[j + 1], h, l);
-      const uint32_t to = a + (uint32_t)j * 64u + ((((uint32_t)lane >> 3) ^ (((uint32_t)j >> 1) & 3u)) << 4) + ((uint32_t)lane & 7u) * 2u;
-      asm volatile("st.shared.b16 [%0], %1;" ::"r"(to), "h"((uint16_t)h) : "memory");
-      asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + 64u), "h"((uint16_t)(h >> 16)) : "memory");
-      if (two) {
-        asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + 2048u), "h"((uint16_t)l) : "memory");
-        asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + 2112u), "h"((uint16_t)(l >> 16)) : "memory");
+        for (int j = 0; j < 16; ++j) {
+          const uint32_t at = a + (uint32_t)j * 128u + ((((uint32_t)lane >> 3) ^ ((uint32_t)j & 3u)) << 4) + ((uint32_t)lane & 7u) * 2u;
+          asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"((uint16_t)h[j]) : "memory");
+          asm volatile("st.shared.b16 [%0], %1;" ::"r"(at + 64u), "h"((uint16_t)(h[j] >> 16)) : "memory");
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+                     ::"l"(map), "r"(turned ? row : col), "r"(turned ? col : row), "r"(z + low), "r"(a) : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
     }
-    store_box(a, map, row, col, z, two);
   }
-  // two neighbouring values in the format's halves, and their low planes
+  __device__ __forceinline__ void drain() {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  // two neighbouring values in the format's halves, or what the high plane leaves of them
   template <int fmt>
-  static __device__ __forceinline__ void pair(float x, float y, uint32_t& h, uint32_t& l) {
+  static __device__ __forceinline__ uint32_t pair(float x, float y, bool low) {
     if constexpr (fmt == kFmtBF16) {
       const __nv_bfloat162 t = __floats2bfloat162_rn(x, y);
-      h = *reinterpret_cast<const uint32_t*>(&t);
-      l = 0;
+      return *reinterpret_cast<const uint32_t*>(&t);
     } else {
-      const __half2 t = __floats2half2_rn(x, y);
-      h = *reinterpret_cast<const uint32_t*>(&t);
-      l = 0;
-      if constexpr (fmt != kFmtPlanes) return;
-      const float2 b = __half22float2(t);
-      const __half2 u = __floats2half2_rn(x - b.x, y - b.y);
-      l = *reinterpret_cast<const uint32_t*>(&u);
+      __half2 t = __floats2half2_rn(x, y);
+      if (fmt == kFmtPlanes && low) {
+        const float2 b = __half22float2(t);
+        t = __floats2half2_rn(x - b.x, y - b.y);
+      }
+      return *reinterpret_cast<const uint32_t*>(&t);
     }
   }
   // Results of any stride and alignment: f(r, v) for r = 0..31 with v = row r's value of column `lane`, so that a warp's
@@ -262,9 +258,6 @@ struct OutStage {
     f([&](int r) { return f32(r, lane); });
   }
   __device__ __forceinline__ float& f32(int r, int c) { return f[r * 32 + (c ^ r)]; }
-  __device__ __forceinline__ void drain() {
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-  }
 };
 
 // 32 sums of the half tile from column c on: from TMEM, or from the registers that they were added up in
@@ -282,11 +275,13 @@ struct SumsInTmem {
 template <int kHalf>
 struct SumsInRegisters {
   const float (&sum)[kHalf];
-  __device__ __forceinline__ void load(int c, float (&v)[32]) const {
+  __device__ __forceinline__ void load(int c, float (&v)[32]) const {       // by selection, so that loops over c need not be unrolled
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
-      v[j] = sum[c + j];
-      asm volatile("" : "+f"(v[j]));       // what is made of these 32 is not begun before the 32 before them are out: registers
+      float t = sum[j];
+#pragma unroll
+      for (int k = 32; k < kHalf; k += 32) t = c == k ? sum[k + j] : t;
+      v[j] = t;
     }
   }
 };
@@ -294,7 +289,8 @@ struct SumsInRegisters {
 // An epilogue is a struct with Params and
 //   run<kPlanes, kHalf>(params, args, tile, row, col, half, stage, sums, done)
 // row: the first of the warp's 32 rows, col: the first of its kHalf columns (either may lie outside the result); done() is
-// called after the last load of sums.
+// called after the last load of sums.  ahead<kHalf>(params, tile, row, col, lane) is called while the products of the tile are
+// made, for what the epilogue is going to read.
 template <class C, class Epi>
 __global__ void __launch_bounds__(kG16Threads, 1)
 gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ typename Epi::Params ep) {
@@ -309,6 +305,10 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
   const int rank = C::kCtas == 2 ? (int)cluster_rank() : 0;
   const int ntiles = tiles16<C>(g), first = blockIdx.x / C::kCtas, step = gridDim.x / C::kCtas;
 
+  if (threadIdx.x == kG16Threads - 1) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&g.a) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&g.b) : "memory");
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&tfull[i], 1); mbar_init(&tempty[i], 8 * C::kCtas); }
@@ -437,6 +437,7 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
     for (int t = first; t < ntiles && ok; t += step) {
       const Tile16 w = tile16<C>(g, t);
       const int row = w.m0 + rank * 128 + q * 32, col = w.n0 + half * kHalf;
+      Epi::template ahead<kHalf>(ep, w, row, col, lane);
       if constexpr (C::kPromote) {
         float sum[kHalf];
 #pragma unroll

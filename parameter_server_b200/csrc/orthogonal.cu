@@ -114,17 +114,21 @@ k_orth_pack(const void* __restrict__ x, const float* __restrict__ m, int rows, i
 // b A + c A² + a I = A (b I + c A) + a I and the new X = (a I + b A + c A²) X are plain products.
 struct EpiNs {
   struct Params {
-    CUtensorMap out, out2;
+    CUtensorMap out[2];
     float* slots;              // not null: raw sums, [split][batch][M][N]
     void* result;              // not null: the last product
     int M, N, batch, second, dtype, update;
     float alpha, beta, alpha2, beta2, lr;
   };
+  template <int kHalf>
+  static __device__ __forceinline__ void ahead(const Params& p, const Tile16& w, int row, int col, int lane) {
+    if (p.update && row + lane < p.M) prefetch_l2<kHalf>(reinterpret_cast<const float*>(p.result) + ((int64_t)w.z * p.M + row + lane) * p.N, col, p.N);
+  }
   template <int kPlanes, int kHalf, class Sums, class Done>
   static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int, OutStage& st,
                                              const Sums& sums, Done done) {
     constexpr int kFmt = kPlanes == 2 ? kFmtPlanes : kFmtF16;
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < kHalf; k += 32) {
       float v[32];
       sums.load(k, v);
@@ -133,15 +137,14 @@ struct EpiNs {
       if (row0 >= p.M || col >= p.N) continue;
       if (p.slots == nullptr && p.result == nullptr) {
         const bool diagonal = row0 == col;                 // both are multiples of 32
-        float u[32];
-        if (p.second) {
+#pragma unroll 1
+        for (int m = 0; m < (p.second ? 2 : 1); ++m) {
+          const float alpha = m ? p.alpha2 : p.alpha, beta = m ? p.beta2 : p.beta;
+          float u[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) u[j] = p.alpha2 * v[j] + (diagonal && j == st.lane ? p.beta2 : 0.f);
-          st.store<kFmt>(&p.out2, u, row0, col, w.z * 2, w.mirror);
+          for (int j = 0; j < 32; ++j) u[j] = alpha * v[j] + (diagonal && j == st.lane ? beta : 0.f);
+          st.store<kFmt>(&p.out[m], u, row0, col, w.z * 2, w.mirror);
         }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) u[j] = p.alpha * v[j] + (diagonal && j == st.lane ? p.beta : 0.f);
-        st.store<kFmt>(&p.out, u, row0, col, w.z * 2, w.mirror);
         continue;
       }
       const int rows = p.M - row0 < 32 ? p.M - row0 : 32, mine = col + st.lane;
@@ -155,14 +158,14 @@ struct EpiNs {
           return;
         }
         const int64_t at = ((int64_t)w.z * p.M + row0) * p.N + mine;
+#pragma unroll 1
+        for (int r0 = 0; r0 < 32; r0 += 16) {
+          float t[16];
 #pragma unroll
-        for (int r0 = 0; r0 < 32; r0 += 8) {
-          float t[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
+          for (int i = 0; i < 16; ++i)
             t[i] = p.update && in && r0 + i < rows ? reinterpret_cast<const float*>(p.result)[at + (int64_t)(r0 + i) * p.N] : 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 16; ++i) {
             const float x = p.alpha * kNsInv * value(r0 + i);
             const int64_t to = at + (int64_t)(r0 + i) * p.N;
             if (!in || r0 + i >= rows) continue;
@@ -216,8 +219,8 @@ k_orth_sum(const float* __restrict__ slots, int splits, int batch, int n, int ti
       float y[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) y[j] = (m ? alpha2 : alpha) * x[j] + (r == c + j ? (m ? beta2 : beta) : 0.f);
-      OutStage::pair<kFmtPlanes>(y[0], y[1], h.x, l.x);
-      OutStage::pair<kFmtPlanes>(y[2], y[3], h.y, l.y);
+      h = make_uint2(OutStage::pair<kFmtPlanes>(y[0], y[1], false), OutStage::pair<kFmtPlanes>(y[2], y[3], false));
+      l = make_uint2(OutStage::pair<kFmtPlanes>(y[0], y[1], true), OutStage::pair<kFmtPlanes>(y[2], y[3], true));
       *reinterpret_cast<uint2*>((m ? out2 : out) + at) = h;
       *reinterpret_cast<uint2*>((m ? out2 : out) + at + plane) = l;
     }
@@ -267,7 +270,10 @@ __device__ __forceinline__ float4 ld_own_v4(uint32_t addr) {
 __device__ __forceinline__ void planes8(const float* v, uint4& h, uint4& l) {
   uint32_t hs[4], ls[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) OutStage::pair<kFmtPlanes>(v[2 * i], v[2 * i + 1], hs[i], ls[i]);
+  for (int i = 0; i < 4; ++i) {
+    hs[i] = OutStage::pair<kFmtPlanes>(v[2 * i], v[2 * i + 1], false);
+    ls[i] = OutStage::pair<kFmtPlanes>(v[2 * i], v[2 * i + 1], true);
+  }
   h = make_uint4(hs[0], hs[1], hs[2], hs[3]);
   l = make_uint4(ls[0], ls[1], ls[2], ls[3]);
 }
@@ -812,6 +818,7 @@ int psb_orthogonal(const OrthArgs* ap, cudaStream_t s) {
       B{bb, p.lo, p.lo, p.ldl, p.lplane, 2 * a.batch};
   Gemm16Args g = {};
   g.batch = a.batch; g.a_z = 2; g.b_z = 2; g.splits = 1; g.status = a.status;
+
   CUtensorMap map_a, map_a2, map_b;
   if ((r = make_out_map(&map_a, A, 0)) != 0 || (r = make_out_map(&map_a2, A2, 0)) != 0 || (r = make_out_map(&map_b, B, 0)) != 0) return r;
 
@@ -830,19 +837,19 @@ int psb_orthogonal(const OrthArgs* ap, cudaStream_t s) {
   };
   for (int k = 0; k < a.steps; ++k) {
     const int planes = precise || k + 1 < a.steps ? 2 : 1;
-    const Operand16 X{xs[k & 1], a.rows, a.cols, p.ldx, p.xplane, 2 * a.batch}, Y{xs[(k + 1) & 1], a.rows, a.cols, p.ldx, p.xplane, 2 * a.batch};
+    const Operand16 X{xs[k & 1], a.rows, a.cols, p.ldx, p.xplane, 2 * a.batch};
     // A = X Xᵀ (or Xᵀ X), and b I + c A
     Gemm16Args gg = g;
     gg.K = p.hi; gg.a_mn = gg.b_mn = p.tall;
     EpiNs::Params ea = {};
-    ea.out = map_a; ea.out2 = map_a2; ea.second = 1;
+    ea.out[0] = map_a; ea.out[1] = map_a2; ea.second = 1;
     ea.alpha = kNsInv; ea.alpha2 = kNsC * kNsInv; ea.beta2 = kNsB * kNsScale;
     if ((r = square(p.gram[planes - 1], planes, gg, X, X, ea, ab, a2)) != 0) return r;
     // B = A (b I + c A) + a I
     Gemm16Args gs = g;
     gs.K = p.lo;
     EpiNs::Params eb = {};
-    eb.out = map_b; eb.alpha = kNsInv; eb.beta = kNsA * kNsScale;
+    eb.out[0] = map_b; eb.alpha = kNsInv; eb.beta = kNsA * kNsScale;
     if ((r = square(p.square[planes - 1], planes, gs, A, A2, eb, bb, nullptr)) != 0) return r;
     // B X (or X B)
     Gemm16Args gu = g;
@@ -850,7 +857,7 @@ int psb_orthogonal(const OrthArgs* ap, cudaStream_t s) {
     EpiNs::Params eu = {};
     eu.M = a.rows; eu.N = a.cols; eu.batch = a.batch; eu.alpha = kNsInv;
     if (k + 1 == a.steps) { eu.result = a.out; eu.update = a.m != nullptr; eu.dtype = a.dtype; eu.lr = a.lr; }
-    else if ((r = make_out_map(&eu.out, Y, 0)) != 0) return r;
+    else if ((r = make_out_map(&eu.out[0], Operand16{xs[(k + 1) & 1], a.rows, a.cols, p.ldx, p.xplane, 2 * a.batch}, 0)) != 0) return r;
     if ((r = product16<EpiNs>(chain, planes, p.step[planes - 1].kind, gu, p.tall ? X : B, p.tall ? B : X, eu)) != 0) return r;
   }
   return 0;

@@ -196,6 +196,8 @@ struct EpiScore {
     ScaleRef scale;
     int n, V, parts, keep;
   };
+  template <int kHalf>
+  static __device__ __forceinline__ void ahead(const Params&, const Tile16&, int, int, int) {}
   template <int kPlanes, int kHalf, class Sums, class Done>
   static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int half, OutStage& st,
                                              const Sums& sums, Done done) {
@@ -204,7 +206,7 @@ struct EpiScore {
     int64_t lab = -1;
     if (row < p.n) lab = p.y[row];
     float top = -INFINITY;
-#pragma unroll
+#pragma unroll 1
     for (int c = 0; c < kHalf; c += 32) {
       float v[32];
       sums.load(c, v);
@@ -220,7 +222,7 @@ struct EpiScore {
     // without a finite score the reference is 0: 2^(-inf) is 0 and nothing is subtracted from an infinity
     const float m = __fmul_rn(top, scale), ref = top == -INFINITY ? 0.f : m;
     float s = 0.f;
-#pragma unroll
+#pragma unroll 1
     for (int c = 0; c < kHalf; c += 32) {
       float v[32];
       sums.load(c, v);
@@ -259,6 +261,8 @@ struct EpiG {
     ScaleRef scale;
     int n, V, len, v0, dtype;
   };
+  template <int kHalf>
+  static __device__ __forceinline__ void ahead(const Params&, const Tile16&, int, int, int) {}
   template <int kPlanes, int kHalf, class Sums, class Done>
   static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16&, int row0, int col0, int, OutStage& st,
                                              const Sums& sums, Done done) {
@@ -272,7 +276,7 @@ struct EpiG {
       lse = p.lse[row];
     }
     const bool none = row >= p.n || !has_class(p.y[row], p.V);
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < kHalf; k += 32) {
       float v[32];
       sums.load(k, v);
@@ -306,11 +310,15 @@ struct EpiGrad {
     int M, N, dtype, with_w, by_map;
     int read, write;           // acc is added to the product; the sum goes to acc instead of the result
   };
+  template <int kHalf>
+  static __device__ __forceinline__ void ahead(const Params& p, const Tile16& w, int row, int col, int lane) {
+    if (p.read && row + lane < p.M) prefetch_l2<kHalf>(p.acc + w.split * p.slot + (int64_t)(row + lane) * p.N, col, p.N);
+  }
   template <int kPlanes, int kHalf, class Sums, class Done>
   static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int, OutStage& st,
                                              const Sums& sums, Done done) {
     const float scale = grad_scale(p.scale, p.with_w);
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < kHalf; k += 32) {
       float v[32];
       sums.load(k, v);
@@ -329,13 +337,22 @@ struct EpiGrad {
       const int64_t at = (int64_t)row0 * p.N + mine;
       float* acc = p.acc != nullptr ? p.acc + w.split * p.slot + at : nullptr;
       st.by_rows(v, [&](auto value) {
+        if (!p.read) {
 #pragma unroll
-        for (int r0 = 0; r0 < 32; r0 += 8) {
-          float t[8];
+          for (int r = 0; r < 32; ++r) {
+            if (!in || r >= rows) continue;
+            if (p.write) acc[(int64_t)r * p.N] = value(r);
+            else store_as(p.out, at + (int64_t)r * p.N, value(r) * scale, p.dtype);
+          }
+          return;
+        }
+#pragma unroll 1
+        for (int r0 = 0; r0 < 32; r0 += 16) {
+          float t[16];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) t[i] = p.read && in && r0 + i < rows ? acc[(int64_t)(r0 + i) * p.N] : 0.f;
+          for (int i = 0; i < 16; ++i) t[i] = in && r0 + i < rows ? acc[(int64_t)(r0 + i) * p.N] : 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 16; ++i) {
             t[i] += value(r0 + i);
             if (!in || r0 + i >= rows) continue;
             if (p.write) acc[(int64_t)(r0 + i) * p.N] = t[i];
