@@ -13,8 +13,8 @@
 // Shape.  Persistent CTAs, or CTA pairs (cta_group::2) where the problem has enough tiles:
 //   warp 0, one lane    TMA producer, a ring of stages of 64 elements of K (128-byte swizzle rows)
 //   warp 1, one lane    tcgen05.mma; in a pair the leader issues for both CTAs
-//   warps 4-11          epilogue: warp w reads TMEM lanes 32(w % 4)..+31, half of the tile's columns; the accumulator is
-//                       double-buffered, so a tile's epilogue runs under the next tile's products
+//   warps 4-11          epilogue: warp w reads TMEM lanes 32(w % 4)..+31, half of the tile's columns; TMEM holds two
+//                       or more accumulators, so a tile's epilogue runs under the next tile's products
 // Sums of planes need 128 registers of an epilogue thread: its warps take over registers of the other four.
 // 16-bit results leave through shared memory as TMA stores of 32 x 32 boxes: a lane holds a row, and stores of rows by
 // lanes touch 32 lines an instruction (4096 x 4096 Newton-Schulz step: 2.6 times the time; 16-byte stores of what the warp
@@ -32,8 +32,8 @@ namespace psb {
 
 constexpr int kG16Threads = 384, kG16K = 64;
 constexpr int kG16Epi = 4;                         // first warp of the epilogue, of eight
-constexpr int kStageOut = 4096;                   // bytes of shared memory of an epilogue warp
-constexpr int kG16Smem = 192 * 1024;              // of the stages
+constexpr int kG16Smem = 225 * 1024;              // of the stages and of what leaves
+constexpr int kBoxBytes = 2048;                   // 32 x 32 values of 16 bits
 
 template <int kCtas_, int kN_, int kPlanes_>
 struct Cfg16 {
@@ -41,12 +41,14 @@ struct Cfg16 {
   static constexpr int kM = 128 * kCtas, kBRows = kN / kCtas;
   static constexpr int kABytes = 128 * 128, kBBytes = kBRows * 128;
   static constexpr int kStageBytes = kPlanes * (kABytes + kBBytes);
-  static constexpr int kStages = kG16Smem / kStageBytes > 8 ? 8 : kG16Smem / kStageBytes;
-  static constexpr int kSmemBytes = kStages * kStageBytes + 8 * kStageOut + 1024 + 256;
+  // 4 KB of shared memory for an epilogue warp's stores; 8 KB with one plane, whose epilogues have less time
+  static constexpr int kBoxes = kPlanes == 1 ? 4 : 2;
+  static constexpr int kFit = (kG16Smem - 8 * kBoxes * kBoxBytes) / kStageBytes, kStages = kFit > 8 ? 8 : kFit;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 8 * kBoxes * kBoxBytes + 1024 + 512;
+  static constexpr int kBufs = 512 / kN;           // accumulators in TMEM: products run ahead of the epilogue by so many less one
   static constexpr bool kPromote = kPlanes == 2;   // sums of kChunk blocks of K are added up in registers
   static constexpr int kChunk = kPromote ? 2 : 1 << 30;
-  static constexpr uint32_t kTmem = 2 * kN < 32 ? 32 : 2 * kN;
-  static_assert(kStages >= 3 && kBRows % 64 == 0 && kTmem <= 512 && kSmemBytes <= 232448, "shape of a tile");
+  static_assert(kStages >= 3 && kBRows % 64 == 0 && kBufs >= 2 && kSmemBytes <= 232448, "shape of a tile");
 };
 
 struct Gemm16Args {
@@ -178,8 +180,24 @@ __device__ __forceinline__ void prefetch_l2(const float* row, int col, int n) {
 
 enum : int { kFmtF16 = 0, kFmtBF16 = 1, kFmtPlanes = 2 };      // fp16, bf16, hi and lo planes of fp16
 
-// An epilogue warp's way to global memory: its 4 KB of shared memory.  v: 32 columns from col on of this lane's row of the
+// two neighbouring values in the format's halves, or what the high plane leaves of them
+template <int fmt>
+__device__ __forceinline__ uint32_t pair16(float x, float y, bool low) {
+  if constexpr (fmt == kFmtBF16) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&t);
+  } else {
+    __half2 t = __floats2half2_rn(x, y);
+    if (fmt == kFmtPlanes && low) {
+      const float2 b = __half22float2(t);
+      t = __floats2half2_rn(x - b.x, y - b.y);
+    }
+    return *reinterpret_cast<const uint32_t*>(&t);
+  }
+}
+// An epilogue warp's way to global memory: its shared memory, kBoxes boxes.  v: 32 columns from col on of this lane's row of the
 // 32 rows from row on.
+template <int kBoxes>
 struct OutStage {
   uint32_t addr;
   float* f;
@@ -187,11 +205,11 @@ struct OutStage {
 
   uint32_t turn = 0;
 
-  // The buffer that the next store uses, free again: the one before last has been read.
+  // The buffer that the next store uses, free again: a store takes some 1000 cycles until its box has been read.
   __device__ __forceinline__ uint32_t acquire() {
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kBoxes - 1) : "memory");
     __syncwarp();
-    return addr + (turn++ & 1u) * 2048u;
+    return addr + (turn++ % kBoxes) * (uint32_t)kBoxBytes;
   }
   // 32 x 32 boxes in the format, a plane at a time, as they are and, for a mirror image, transposed.  Rows of 64 bytes, 64-byte
   // swizzle (16-byte piece j of row r lies at j ^ ((r / 2) % 4)): free of bank conflicts.  What lies outside the map is not
@@ -204,7 +222,7 @@ struct OutStage {
       const bool turned = pass >= planes, low = fmt == kFmtPlanes && (pass & 1);
       uint32_t h[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) h[j] = pair<fmt>(v[2 * j], v[2 * j + 1], low);
+      for (int j = 0; j < 16; ++j) h[j] = pair16<fmt>(v[2 * j], v[2 * j + 1], low);
       const uint32_t a = acquire();
       if (!turned) {
         const uint32_t mine = a + (uint32_t)lane * 64u, sw = ((uint32_t)lane >> 1) & 3u;
@@ -231,21 +249,6 @@ struct OutStage {
   }
   __device__ __forceinline__ void drain() {
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-  }
-  // two neighbouring values in the format's halves, or what the high plane leaves of them
-  template <int fmt>
-  static __device__ __forceinline__ uint32_t pair(float x, float y, bool low) {
-    if constexpr (fmt == kFmtBF16) {
-      const __nv_bfloat162 t = __floats2bfloat162_rn(x, y);
-      return *reinterpret_cast<const uint32_t*>(&t);
-    } else {
-      __half2 t = __floats2half2_rn(x, y);
-      if (fmt == kFmtPlanes && low) {
-        const float2 b = __half22float2(t);
-        t = __floats2half2_rn(x - b.x, y - b.y);
-      }
-      return *reinterpret_cast<const uint32_t*>(&t);
-    }
   }
   // Results of any stride and alignment: f(r, v) for r = 0..31 with v = row r's value of column `lane`, so that a warp's
   // accesses are pieces of one row.  The exclusive or keeps both directions free of bank conflicts.
@@ -297,9 +300,9 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* outs = stages + C::kStages * C::kStageBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(outs + 8 * kStageOut);
-  uint64_t *empty = full + C::kStages, *tfull = empty + C::kStages, *tempty = tfull + 2;
-  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint64_t* full = reinterpret_cast<uint64_t*>(outs + 8 * C::kBoxes * kBoxBytes);
+  uint64_t *empty = full + C::kStages, *tfull = empty + C::kStages, *tempty = tfull + C::kBufs;
+  uint32_t* tmem_base = reinterpret_cast<uint32_t*>(tempty + C::kBufs);
   volatile uint32_t* abort_flag = tmem_base + 1;
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = C::kCtas == 2 ? (int)cluster_rank() : 0;
@@ -311,16 +314,16 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&tfull[i], 1); mbar_init(&tempty[i], 8 * C::kCtas); }
+    for (int i = 0; i < C::kBufs; ++i) { mbar_init(&tfull[i], 1); mbar_init(&tempty[i], 8 * C::kCtas); }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) {
     if constexpr (C::kCtas == 2) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base)), "r"(C::kTmem) : "memory");
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base)), "r"(512u) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     } else {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base)), "r"(C::kTmem) : "memory");
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base)), "r"(512u) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
   }
@@ -372,8 +375,8 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
     for (int t = first; t < ntiles && ok; t += step) {
       const Tile16 w = tile16<C>(g, t);
       for (int kc = w.kb0; kc < w.kb1 && ok; kc += C::kChunk, ++n) {
-        const uint32_t acc = n & 1u;
-        if (n >= 2 && !(ok = mbar_wait_warp(&tempty[acc], ((n >> 1) - 1) & 1))) break;
+        const uint32_t acc = n % C::kBufs;
+        if (n >= C::kBufs && !(ok = mbar_wait_warp(&tempty[acc], (n / C::kBufs - 1) & 1))) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t d = tmem + acc * (uint32_t)C::kN;
         const int ke = w.kb1 - kc < C::kChunk ? w.kb1 : kc + C::kChunk;
@@ -407,8 +410,8 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
     if constexpr (C::kPromote) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     constexpr int kHalf = C::kN / 2;
     const int q = warp & 3, half = (warp - kG16Epi) >> 2;
-    uint8_t* mine = outs + (warp - kG16Epi) * kStageOut;
-    OutStage stage{smem_u32(mine), reinterpret_cast<float*>(mine), lane};
+    uint8_t* mine = outs + (warp - kG16Epi) * (C::kBoxes * kBoxBytes);
+    OutStage<C::kBoxes> stage{smem_u32(mine), reinterpret_cast<float*>(mine), lane};
     const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * kHalf);
     uint32_t n = 0;
     // warp-uniform, as the TMEM loads are warp-collective
@@ -443,8 +446,8 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
 #pragma unroll
         for (int j = 0; j < kHalf; ++j) sum[j] = 0.f;
         for (int kc = w.kb0; kc < w.kb1; kc += C::kChunk, ++n) {
-          const uint32_t acc = n & 1u;
-          if (!(ok = sums_ready(acc, (n >> 1) & 1))) break;
+          const uint32_t acc = n % C::kBufs;
+          if (!(ok = sums_ready(acc, (n / C::kBufs) & 1))) break;
 uint32_t r[2][32];
           tmem_load_32x32(lanes + acc * (uint32_t)C::kN, r[0]);
 #pragma unroll
@@ -459,8 +462,8 @@ uint32_t r[2][32];
         if (!ok) break;
         Epi::template run<C::kPlanes, kHalf>(ep, g, w, row, col, half, stage, SumsInRegisters<kHalf>{sum}, [] {});
       } else {
-        const uint32_t acc = n & 1u;
-        if (!(ok = sums_ready(acc, (n >> 1) & 1))) break;
+        const uint32_t acc = n % C::kBufs;
+        if (!(ok = sums_ready(acc, (n / C::kBufs) & 1))) break;
         ++n;
         Epi::template run<C::kPlanes, kHalf>(ep, g, w, row, col, half, stage, SumsInTmem<kHalf>{lanes + acc * (uint32_t)C::kN}, [&] { release(acc); });
       }
@@ -478,9 +481,9 @@ uint32_t r[2][32];
   if (C::kCtas == 2) cluster_sync_all();       // neither CTA frees its accumulators or leaves while the other still works
   if (warp == 0) {
     if constexpr (C::kCtas == 2)
-      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmem) : "memory");
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     else
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kTmem) : "memory");
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
 }
 
@@ -583,11 +586,11 @@ int launch16(Chain& chain, psb::Gemm16Args& g, const Operand16& a, const Operand
 }
 
 // ---- which tiles, and in how many pieces K is taken
-enum : int { kPair256 = 0, kOne128 = 1, kOne64 = 2 };      // 256x256 on a pair, 128x128, 128x64
+enum : int { kPair256 = 0, kPair128 = 1, kOne128 = 2, kOne64 = 3, kKinds = 4 };      // 256x256 and 256x128 on a pair, 128x128, 128x64
 struct Tiling { int kind, splits, kb_split; };
 
-inline int tiling_rows(int kind) { return kind == kPair256 ? 256 : 128; }
-inline int tiling_cols(int kind) { return kind == kPair256 ? 256 : kind == kOne128 ? 128 : 64; }
+inline int tiling_rows(int kind) { return kind <= kPair128 ? 256 : 128; }
+inline int tiling_cols(int kind) { return kind == kPair256 ? 256 : kind == kOne64 ? 64 : 128; }
 
 // The cheapest by this estimate, in cycles of an SM: rounds of tiles, each its blocks of K at the slower of the tensor
 // cores (128 x N x 64 in 2N cycles a product, as a rule) and the loads (48 bytes a cycle from L2, as measured with all SMs
@@ -596,13 +599,13 @@ inline Tiling choose_tiling(int64_t batch, int64_t M, int64_t N, int64_t K, int 
   const int64_t nkb = (K + psb::kG16K - 1) / psb::kG16K;
   Tiling best = {kOne64, 1, (int)nkb};
   double least = 1e300;
-  for (int kind = 0; kind < 3; ++kind) {
-    if ((only >= 0 && kind != only) || (sym && kind == kOne64)) continue;
+  for (int kind = 0; kind < kKinds; ++kind) {
     const int64_t rows = tiling_rows(kind), cols = tiling_cols(kind);
-    const int64_t tm = (M + rows - 1) / rows, tn = (N + cols - 1) / cols, slots = kind == kPair256 ? 74 : 148;
+    if ((only >= 0 && kind != only) || (sym && rows != cols)) continue;
+    const int64_t tm = (M + rows - 1) / rows, tn = (N + cols - 1) / cols, slots = rows == 256 ? 74 : 148;
     const int64_t tiles = batch * (sym ? tm * (tm + 1) / 2 : tm * tn);
     const double mma = 2.0 * cols * (planes == 2 ? 3 : 1);
-    const double load = planes * (kind == kPair256 ? 32768.0 : 16384.0 + 128.0 * cols) / 48.0;
+    const double load = planes * (16384.0 + 128.0 * cols * 128.0 / rows) / 48.0;
     for (int64_t s = 1; s <= max_splits && s <= nkb; ++s) {
       const int64_t per = (nkb + s - 1) / s, real = (nkb + per - 1) / per;
       if (real != s) continue;
@@ -619,6 +622,7 @@ inline Tiling choose_tiling(int64_t batch, int64_t M, int64_t N, int64_t K, int 
 template <int kPlanes, class Epi>
 int launch_tiled(Chain& chain, int kind, psb::Gemm16Args& g, const Operand16& a, const Operand16& b, const typename Epi::Params& ep) {
   if (kind == kPair256) return launch16<psb::Cfg16<2, 256, kPlanes>, Epi>(chain, g, a, b, ep);
+  if (kind == kPair128) return launch16<psb::Cfg16<2, 128, kPlanes>, Epi>(chain, g, a, b, ep);
   if (kind == kOne128) return launch16<psb::Cfg16<1, 128, kPlanes>, Epi>(chain, g, a, b, ep);
   return launch16<psb::Cfg16<1, 64, kPlanes>, Epi>(chain, g, a, b, ep);
 }

@@ -124,8 +124,8 @@ struct EpiNs {
   static __device__ __forceinline__ void ahead(const Params& p, const Tile16& w, int row, int col, int lane) {
     if (p.update && row + lane < p.M) prefetch_l2<kHalf>(reinterpret_cast<const float*>(p.result) + ((int64_t)w.z * p.M + row + lane) * p.N, col, p.N);
   }
-  template <int kPlanes, int kHalf, class Sums, class Done>
-  static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int, OutStage& st,
+  template <int kPlanes, int kHalf, class Stage, class Sums, class Done>
+  static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int, Stage& st,
                                              const Sums& sums, Done done) {
     constexpr int kFmt = kPlanes == 2 ? kFmtPlanes : kFmtF16;
 #pragma unroll 1
@@ -143,7 +143,7 @@ struct EpiNs {
           float u[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) u[j] = alpha * v[j] + (diagonal && j == st.lane ? beta : 0.f);
-          st.store<kFmt>(&p.out[m], u, row0, col, w.z * 2, w.mirror);
+          st.template store<kFmt>(&p.out[m], u, row0, col, w.z * 2, w.mirror);
         }
         continue;
       }
@@ -219,8 +219,8 @@ k_orth_sum(const float* __restrict__ slots, int splits, int batch, int n, int ti
       float y[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) y[j] = (m ? alpha2 : alpha) * x[j] + (r == c + j ? (m ? beta2 : beta) : 0.f);
-      h = make_uint2(OutStage::pair<kFmtPlanes>(y[0], y[1], false), OutStage::pair<kFmtPlanes>(y[2], y[3], false));
-      l = make_uint2(OutStage::pair<kFmtPlanes>(y[0], y[1], true), OutStage::pair<kFmtPlanes>(y[2], y[3], true));
+      h = make_uint2(pair16<kFmtPlanes>(y[0], y[1], false), pair16<kFmtPlanes>(y[2], y[3], false));
+      l = make_uint2(pair16<kFmtPlanes>(y[0], y[1], true), pair16<kFmtPlanes>(y[2], y[3], true));
       *reinterpret_cast<uint2*>((m ? out2 : out) + at) = h;
       *reinterpret_cast<uint2*>((m ? out2 : out) + at + plane) = l;
     }
@@ -271,8 +271,8 @@ __device__ __forceinline__ void planes8(const float* v, uint4& h, uint4& l) {
   uint32_t hs[4], ls[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    hs[i] = OutStage::pair<kFmtPlanes>(v[2 * i], v[2 * i + 1], false);
-    ls[i] = OutStage::pair<kFmtPlanes>(v[2 * i], v[2 * i + 1], true);
+    hs[i] = pair16<kFmtPlanes>(v[2 * i], v[2 * i + 1], false);
+    ls[i] = pair16<kFmtPlanes>(v[2 * i], v[2 * i + 1], true);
   }
   h = make_uint4(hs[0], hs[1], hs[2], hs[3]);
   l = make_uint4(ls[0], ls[1], ls[2], ls[3]);

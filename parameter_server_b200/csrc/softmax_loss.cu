@@ -198,8 +198,8 @@ struct EpiScore {
   };
   template <int kHalf>
   static __device__ __forceinline__ void ahead(const Params&, const Tile16&, int, int, int) {}
-  template <int kPlanes, int kHalf, class Sums, class Done>
-  static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int half, OutStage& st,
+  template <int kPlanes, int kHalf, class Stage, class Sums, class Done>
+  static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int half, Stage& st,
                                              const Sums& sums, Done done) {
     const float scale = score_scale(p.scale);
     const int row = row0 + st.lane;
@@ -245,7 +245,7 @@ struct EpiScore {
         s += v[j];
         v[j] *= (float)(1 << kExpScale);
       }
-      if (col < p.keep) st.store<kPlanes == 2 ? kFmtPlanes : kFmtF16>(&p.e, v, row0, col, 0, false);
+      if (col < p.keep) st.template store<kPlanes == 2 ? kFmtPlanes : kFmtF16>(&p.e, v, row0, col, 0, false);
     }
     if (row < p.n) p.part[(int64_t)row * p.parts + w.tn * 2 + half] = make_float2(top == -INFINITY ? top : m, s);
   }
@@ -263,8 +263,8 @@ struct EpiG {
   };
   template <int kHalf>
   static __device__ __forceinline__ void ahead(const Params&, const Tile16&, int, int, int) {}
-  template <int kPlanes, int kHalf, class Sums, class Done>
-  static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16&, int row0, int col0, int, OutStage& st,
+  template <int kPlanes, int kHalf, class Stage, class Sums, class Done>
+  static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16&, int row0, int col0, int, Stage& st,
                                              const Sums& sums, Done done) {
     const float scale = score_scale(p.scale);
     const int row = row0 + st.lane;
@@ -286,9 +286,9 @@ struct EpiG {
       const int at = lab >= col && lab < col + 32 ? (int)(lab - col) : -1;
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = none ? 0.f : c * (ex2(fmaf(v[j], scale, -lse)) - (at == j ? 1.f : 0.f));
-      if constexpr (kPlanes == 2) st.store<kFmtPlanes>(&p.g, v, row0, col, 0, false);
-      else if (p.dtype == kBF16) st.store<kFmtBF16>(&p.g, v, row0, col, 0, false);
-      else st.store<kFmtF16>(&p.g, v, row0, col, 0, false);
+      if constexpr (kPlanes == 2) st.template store<kFmtPlanes>(&p.g, v, row0, col, 0, false);
+      else if (p.dtype == kBF16) st.template store<kFmtBF16>(&p.g, v, row0, col, 0, false);
+      else st.template store<kFmtF16>(&p.g, v, row0, col, 0, false);
     }
   }
 };
@@ -314,8 +314,8 @@ struct EpiGrad {
   static __device__ __forceinline__ void ahead(const Params& p, const Tile16& w, int row, int col, int lane) {
     if (p.read && row + lane < p.M) prefetch_l2<kHalf>(p.acc + w.split * p.slot + (int64_t)(row + lane) * p.N, col, p.N);
   }
-  template <int kPlanes, int kHalf, class Sums, class Done>
-  static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int, OutStage& st,
+  template <int kPlanes, int kHalf, class Stage, class Sums, class Done>
+  static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int, Stage& st,
                                              const Sums& sums, Done done) {
     const float scale = grad_scale(p.scale, p.with_w);
 #pragma unroll 1
@@ -328,8 +328,8 @@ struct EpiGrad {
       if (kPlanes == 1 && p.by_map) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] *= scale;
-        if (p.dtype == kBF16) st.store<kFmtBF16>(&p.map, v, row0, col, 0, false);
-        else st.store<kFmtF16>(&p.map, v, row0, col, 0, false);
+        if (p.dtype == kBF16) st.template store<kFmtBF16>(&p.map, v, row0, col, 0, false);
+        else st.template store<kFmtF16>(&p.map, v, row0, col, 0, false);
         continue;
       }
       const int rows = p.M - row0 < 32 ? p.M - row0 : 32, mine = col + st.lane;
@@ -401,7 +401,7 @@ struct JoinArgs {
   uint16_t* x_out;
   int64_t ldx, ldxo;
   ScaleRef scale;
-  int n, V, d, parts, width, keep, dtype;    // width: classes of a part
+  int n, V, d, parts, shift, keep, dtype;    // 2^shift: classes of a part
   uint32_t* status;
 };
 // A row's log-sum-exp (log2) and loss and, in place, its kept exponentials to G.  kLanes threads a row; blockIdx.y shares
@@ -446,33 +446,45 @@ k_loss_rows(const __grid_constant__ JoinArgs p) {
   const float cg = c * pow2i(kg), at_label = cg * (ex2((target - a.x) - l2) - 1.f);
   const float shift = (float)kExpScale + l2;
   uint16_t* g = p.g + (int64_t)row * p.ldg;
-  for (int col = (blockIdx.y * kLanes + ln) * 8; col < p.keep; col += gridDim.y * kLanes * 8) {
-    uint4 h = *reinterpret_cast<const uint4*>(g + col), l = make_uint4(0, 0, 0, 0);
-    if (p.dtype == kF32) l = *reinterpret_cast<const uint4*>(g + p.plane + col);
-    const float f = cg * ex2((part[col / p.width].x - a.x) - shift);
-    uint32_t hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w};
+  // four eights a thread at a time: their loads do not wait for one another
+  const int step = gridDim.y * kLanes * 8;
+  for (int first = (blockIdx.y * kLanes + ln) * 8; first < p.keep; first += 4 * step) {
+    uint4 h[4], l[4];
+    float f[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hs[i]));
-      if (p.dtype == kF32) {
-        const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&ls[i]));
-        v.x += u.x; v.y += u.y;
-      }
-      v.x = ok ? (lab == col + 2 * i ? at_label : v.x * f) : 0.f;
-      v.y = ok ? (lab == col + 2 * i + 1 ? at_label : v.y * f) : 0.f;
-      if (p.dtype == kBF16) {
-        const __nv_bfloat162 t = __floats2bfloat162_rn(v.x, v.y);
-        hs[i] = *reinterpret_cast<const uint32_t*>(&t);
-      } else {
-        __half h0, l0, h1, l1;
-        split16(v.x, h0, l0);
-        split16(v.y, h1, l1);
-        hs[i] = pack_half2(h0, h1);
-        ls[i] = pack_half2(l0, l1);
-      }
+    for (int k = 0; k < 4; ++k) {
+      const int col = first + k * step;
+      if (col >= p.keep) break;
+      h[k] = *reinterpret_cast<const uint4*>(g + col);
+      if (p.dtype == kF32) l[k] = *reinterpret_cast<const uint4*>(g + p.plane + col);
+      f[k] = part[col >> p.shift].x;
     }
-    *reinterpret_cast<uint4*>(g + col) = make_uint4(hs[0], hs[1], hs[2], hs[3]);
-    if (p.dtype == kF32) *reinterpret_cast<uint4*>(g + p.plane + col) = make_uint4(ls[0], ls[1], ls[2], ls[3]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int col = first + k * step;
+      if (col >= p.keep) break;
+      const float scale = cg * ex2((f[k] - a.x) - shift);
+      const int at = lab >= col && lab < col + 8 ? (int)(lab - col) : -1;
+      uint32_t hs[4] = {h[k].x, h[k].y, h[k].z, h[k].w}, ls[4] = {l[k].x, l[k].y, l[k].z, l[k].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hs[i]));
+        if (p.dtype == kF32) {
+          const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&ls[i]));
+          v.x += u.x; v.y += u.y;
+        }
+        v.x = ok ? (at == 2 * i ? at_label : v.x * scale) : 0.f;
+        v.y = ok ? (at == 2 * i + 1 ? at_label : v.y * scale) : 0.f;
+        if (p.dtype == kBF16) {
+          hs[i] = pair16<kFmtBF16>(v.x, v.y, false);
+        } else {
+          hs[i] = pair16<kFmtPlanes>(v.x, v.y, false);
+          if (p.dtype == kF32) ls[i] = pair16<kFmtPlanes>(v.x, v.y, true);
+        }
+      }
+      *reinterpret_cast<uint4*>(g + col) = make_uint4(hs[0], hs[1], hs[2], hs[3]);
+      if (p.dtype == kF32) *reinterpret_cast<uint4*>(g + p.plane + col) = make_uint4(ls[0], ls[1], ls[2], ls[3]);
+    }
   }
 }
 
@@ -510,7 +522,7 @@ using namespace psb;
 
 namespace {
 
-constexpr int kMaxBlocks = 296;               // of the pass that finds the largest magnitudes, for either operand
+constexpr int kMaxBlocks = 148 * 8;           // of the pass that finds the largest magnitudes, for either operand
 
 // where things lie in the workspace; everything is 256-byte aligned
 struct LossPlan {
@@ -667,7 +679,7 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
   // losses, and G of the kept classes
   JoinArgs j = {};
   j.part = part; j.target = target; j.y = a.y; j.coef = a.coef; j.lse = lse; j.loss = a.loss; j.scale = scale;
-  j.n = a.n; j.V = a.V; j.d = a.d; j.parts = p.parts; j.width = tiling_cols(p.score.kind) / 2; j.keep = p.keep; j.dtype = a.dtype; j.status = a.status;
+  j.n = a.n; j.V = a.V; j.d = a.d; j.parts = p.parts; j.shift = tiling_cols(p.score.kind) == 256 ? 7 : tiling_cols(p.score.kind) == 128 ? 6 : 5; j.keep = p.keep; j.dtype = a.dtype; j.status = a.status;
   if (a.want_grad) {
     j.g = gb; j.ldg = p.ldg; j.plane = p.g_plane;
     if (!p.pack_x) { j.x = reinterpret_cast<const uint16_t*>(a.x); j.x_out = xb; j.ldx = a.ldx; j.ldxo = p.dp; }
@@ -675,7 +687,7 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
   if (p.parts <= 64 && a.V <= 2048) {           // a warp a row; with and without gradients alike, so that losses are the same
     r = chain.launch(k_loss_rows<32>, dim3((unsigned)(a.n + 7) / 8, 1), 256, 0, 1, j);
   } else {
-    int64_t share = a.want_grad ? (148 * 4 + a.n - 1) / a.n : 1, most = ((int64_t)p.keep + 2047) / 2048;
+    int64_t share = a.want_grad ? (148 * 6 + a.n - 1) / a.n : 1, most = ((int64_t)p.keep + 8191) / 8192;
     if (share > most) share = most < 1 ? 1 : most;
     r = chain.launch(k_loss_rows<256>, dim3((unsigned)a.n, (unsigned)share), 256, 0, 1, j);
   }
