@@ -13,8 +13,8 @@
 // Shape.  Persistent CTAs, or CTA pairs (cta_group::2) where the problem has enough tiles:
 //   warp 0, one lane    TMA producer, a ring of stages of 64 elements of K (128-byte swizzle rows)
 //   warp 1, one lane    tcgen05.mma; in a pair the leader issues for both CTAs
-//   warps 4-11          epilogue: warp w reads TMEM lanes 32(w % 4)..+31, half of the tile's columns; TMEM holds two
-//                       or more accumulators, so a tile's epilogue runs under the next tile's products
+//   warps 4-11 or -19   epilogue: warp w reads TMEM lanes 32(w % 4)..+31, half or a quarter of the tile's columns; TMEM holds
+//                       two or more accumulators, so a tile's epilogue runs under the next tile's products
 // Sums of planes need 128 registers of an epilogue thread: its warps take over registers of the other four.
 // 16-bit results leave through shared memory as TMA stores of 32 x 32 boxes: a lane holds a row, and stores of rows by
 // lanes touch 32 lines an instruction (4096 x 4096 Newton-Schulz step: 2.6 times the time; 16-byte stores of what the warp
@@ -30,21 +30,22 @@
 
 namespace psb {
 
-constexpr int kG16Threads = 384, kG16K = 64;
-constexpr int kG16Epi = 4;                         // first warp of the epilogue, of eight
+constexpr int kG16K = 64;
+constexpr int kG16Epi = 4;                         // first warp of the epilogue
 constexpr int kG16Smem = 225 * 1024;              // of the stages and of what leaves
 constexpr int kBoxBytes = 2048;                   // 32 x 32 values of 16 bits
 
-template <int kCtas_, int kN_, int kPlanes_>
+template <int kCtas_, int kN_, int kPlanes_, int kParts_ = 2>
 struct Cfg16 {
   static constexpr int kCtas = kCtas_, kN = kN_, kPlanes = kPlanes_;
   static constexpr int kM = 128 * kCtas, kBRows = kN / kCtas;
   static constexpr int kABytes = 128 * 128, kBBytes = kBRows * 128;
   static constexpr int kStageBytes = kPlanes * (kABytes + kBBytes);
-  // 4 KB of shared memory for an epilogue warp's stores; 8 KB with one plane, whose epilogues have less time
-  static constexpr int kBoxes = kPlanes == 1 ? 4 : 2;
-  static constexpr int kFit = (kG16Smem - 8 * kBoxes * kBoxBytes) / kStageBytes, kStages = kFit > 8 ? 8 : kFit;
-  static constexpr int kSmemBytes = kStages * kStageBytes + 8 * kBoxes * kBoxBytes + 1024 + 512;
+  // Epilogue warps for each 32 lanes of TMEM, and 4 KB of shared memory for the stores of each
+  static constexpr int kParts = kParts_, kPart = kN / kParts;
+  static constexpr int kThreads = 128 + 128 * kParts, kBoxes = 2;
+  static constexpr int kFit = (kG16Smem - 4 * kParts * kBoxes * kBoxBytes) / kStageBytes, kStages = kFit > 8 ? 8 : kFit;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 4 * kParts * kBoxes * kBoxBytes + 1024 + 512;
   static constexpr int kBufs = 512 / kN;           // accumulators in TMEM: products run ahead of the epilogue by so many less one
   static constexpr bool kPromote = kPlanes == 2;   // sums of kChunk blocks of K are added up in registers
   static constexpr int kChunk = kPromote ? 2 : 1 << 30;
@@ -77,33 +78,48 @@ __host__ __device__ __forceinline__ int tiles16(const Gemm16Args& g) {
   return g.batch * g.splits * (g.sym ? tm * (tm + 1) / 2 : tm * tn);
 }
 
-// The dimension with fewer tiles runs fastest: its operand stays in L2 while the other one is read once.
+// A CTA's (or pair's) tiles, every step-th from the first on.  The dimension with fewer tiles runs fastest: its operand stays in
+// L2 while the other one is read once.  Counted up digit by digit: the divisions that find a tile by its number are a fifth
+// of the time that the epilogue of a tile of short K has.
 template <class C>
-__device__ __forceinline__ Tile16 tile16(const Gemm16Args& g, int t) {
-  const int tm = (g.M + C::kM - 1) / C::kM, tn = (g.N + C::kN - 1) / C::kN;
-  const int per = g.sym ? tm * (tm + 1) / 2 : tm * tn;
-  Tile16 w;
-  const int zs = t / per;
-  int u = t - zs * per, i, j;
-  w.z = zs / g.splits;
-  w.split = zs - w.z * g.splits;
-  if (g.sym) {
-    j = (int)((sqrtf(8.f * (float)u + 1.f) - 1.f) * 0.5f);
-    while ((j + 1) * (j + 2) / 2 <= u) ++j;
-    while (j * (j + 1) / 2 > u) --j;
-    i = u - j * (j + 1) / 2;
-  } else if (tm <= tn) {
-    i = u % tm; j = u / tm;
-  } else {
-    j = u % tn; i = u / tn;
+struct Tiles16 {
+  const Gemm16Args& g;
+  int tm, tn, nf, ns, fast, slow, zs, by_fast, by_slow, by_zs;
+  __device__ __forceinline__ Tiles16(const Gemm16Args& g_, int first, int step) : g(g_) {
+    tm = (g.M + C::kM - 1) / C::kM;
+    tn = (g.N + C::kN - 1) / C::kN;
+    nf = g.sym ? tm * (tm + 1) / 2 : tm <= tn ? tm : tn;
+    ns = g.sym ? 1 : tm <= tn ? tn : tm;
+    fast = first % nf; by_fast = step % nf;
+    first /= nf; step /= nf;
+    slow = first % ns; by_slow = step % ns;
+    zs = first / ns; by_zs = step / ns;
   }
-  w.mirror = g.sym && i != j;
-  w.m0 = i * C::kM; w.n0 = j * C::kN; w.tn = j;
-  const int nkb = (g.K + kG16K - 1) / kG16K;
-  w.kb0 = w.split * g.kb_split;
-  w.kb1 = w.kb0 + g.kb_split < nkb ? w.kb0 + g.kb_split : nkb;
-  return w;
-}
+  __device__ __forceinline__ bool more() const { return zs < g.batch * g.splits; }
+  __device__ __forceinline__ void next() {
+    fast += by_fast; slow += by_slow; zs += by_zs;
+    if (fast >= nf) { fast -= nf; ++slow; }
+    if (slow >= ns) { slow -= ns; ++zs; }
+  }
+  __device__ __forceinline__ Tile16 get() const {
+    Tile16 w;
+    w.z = g.splits == 1 ? zs : zs / g.splits;
+    w.split = g.splits == 1 ? 0 : zs - w.z * g.splits;
+    int i = tm <= tn ? fast : slow, j = tm <= tn ? slow : fast;
+    if (g.sym) {                           // the fast-th tile on and above the diagonal, column by column
+      j = (int)((sqrtf(8.f * (float)fast + 1.f) - 1.f) * 0.5f);
+      while ((j + 1) * (j + 2) / 2 <= fast) ++j;
+      while (j * (j + 1) / 2 > fast) --j;
+      i = fast - j * (j + 1) / 2;
+    }
+    w.mirror = g.sym && i != j;
+    w.m0 = i * C::kM; w.n0 = j * C::kN; w.tn = j;
+    const int nkb = (g.K + kG16K - 1) / kG16K;
+    w.kb0 = w.split * g.kb_split;
+    w.kb1 = w.kb0 + g.kb_split < nkb ? w.kb0 + g.kb_split : nkb;
+    return w;
+  }
+};
 
 template <int kCtas>
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
@@ -170,11 +186,11 @@ __device__ __forceinline__ uint32_t pack_half2(__half a, __half b) {
 }
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
-// the columns from col to col + kHalf of a row of n floats, towards L2
-template <int kHalf>
+// the columns from col to col + kPart of a row of n floats, towards L2
+template <int kPart>
 __device__ __forceinline__ void prefetch_l2(const float* row, int col, int n) {
 #pragma unroll
-  for (int c = 0; c < kHalf; c += 32)
+  for (int c = 0; c < kPart; c += 32)
     if (col + c < n) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + col + c));
 }
 
@@ -263,8 +279,8 @@ struct OutStage {
   __device__ __forceinline__ float& f32(int r, int c) { return f[r * 32 + (c ^ r)]; }
 };
 
-// 32 sums of the half tile from column c on: from TMEM, or from the registers that they were added up in
-template <int kHalf>
+// 32 sums of the warp's part of a tile from column c on: from TMEM, or from the registers that they were added up in
+template <int kPart>
 struct SumsInTmem {
   uint32_t taddr;
   __device__ __forceinline__ void load(int c, float (&v)[32]) const {
@@ -275,46 +291,46 @@ struct SumsInTmem {
     for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
   }
 };
-template <int kHalf>
+template <int kPart>
 struct SumsInRegisters {
-  const float (&sum)[kHalf];
+  const float (&sum)[kPart];
   __device__ __forceinline__ void load(int c, float (&v)[32]) const {       // by selection, so that loops over c need not be unrolled
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
       float t = sum[j];
 #pragma unroll
-      for (int k = 32; k < kHalf; k += 32) t = c == k ? sum[k + j] : t;
+      for (int k = 32; k < kPart; k += 32) t = c == k ? sum[k + j] : t;
       v[j] = t;
     }
   }
 };
 
 // An epilogue is a struct with Params and
-//   run<kPlanes, kHalf>(params, args, tile, row, col, half, stage, sums, done)
-// row: the first of the warp's 32 rows, col: the first of its kHalf columns (either may lie outside the result); done() is
-// called after the last load of sums.  ahead<kHalf>(params, tile, row, col, lane) is called while the products of the tile are
+//   run<kPlanes, kPart>(params, args, tile, row, col, part, stage, sums, done)
+// row: the first of the warp's 32 rows, col: the first of its kPart columns, the tile's part-th (either may lie outside the result); done() is
+// called after the last load of sums.  ahead<kPart>(params, tile, row, col, lane) is called while the products of the tile are
 // made, for what the epilogue is going to read.
 template <class C, class Epi>
-__global__ void __launch_bounds__(kG16Threads, 1)
+__global__ void __launch_bounds__(C::kThreads, 1)
 gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ typename Epi::Params ep) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* outs = stages + C::kStages * C::kStageBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(outs + 8 * C::kBoxes * kBoxBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(outs + 4 * C::kParts * C::kBoxes * kBoxBytes);
   uint64_t *empty = full + C::kStages, *tfull = empty + C::kStages, *tempty = tfull + C::kBufs;
   uint32_t* tmem_base = reinterpret_cast<uint32_t*>(tempty + C::kBufs);
   volatile uint32_t* abort_flag = tmem_base + 1;
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = C::kCtas == 2 ? (int)cluster_rank() : 0;
-  const int ntiles = tiles16<C>(g), first = blockIdx.x / C::kCtas, step = gridDim.x / C::kCtas;
+  const int first = blockIdx.x / C::kCtas, step = gridDim.x / C::kCtas;
 
-  if (threadIdx.x == kG16Threads - 1) {
+  if (threadIdx.x == 32) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&g.a) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&g.b) : "memory");
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-    for (int i = 0; i < C::kBufs; ++i) { mbar_init(&tfull[i], 1); mbar_init(&tempty[i], 8 * C::kCtas); }
+    for (int i = 0; i < C::kBufs; ++i) { mbar_init(&tfull[i], 1); mbar_init(&tempty[i], 4 * C::kParts * C::kCtas); }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -328,7 +344,7 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
     }
   }
   if (g.clear) {
-    for (int i = threadIdx.x; i < C::kStages * C::kStageBytes / 16; i += kG16Threads) reinterpret_cast<uint4*>(stages)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < C::kStages * C::kStageBytes / 16; i += C::kThreads) reinterpret_cast<uint4*>(stages)[i] = make_uint4(0, 0, 0, 0);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -343,8 +359,8 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
   bool ok = true;                       // the same in all lanes of a warp
   if (warp == 0) {
     uint32_t it = 0;
-    for (int t = first; t < ntiles && ok; t += step) {
-      const Tile16 w = tile16<C>(g, t);
+    for (Tiles16<C> t(g, first, step); t.more() && ok; t.next()) {
+      const Tile16 w = t.get();
       const int am = g.a_m0 + w.m0 + rank * 128, bn = g.b_n0 + w.n0 + rank * C::kBRows;
       for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
         const int st = it % C::kStages;
@@ -372,8 +388,8 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
     const uint64_t ka = g.a_mn ? 2048 >> 4 : 32 >> 4, kb_ = g.b_mn ? 2048 >> 4 : 32 >> 4;
     const uint64_t base_a = operand_desc(smem_u32(stages), g.a_mn), base_b = operand_desc(smem_u32(stages) + C::kPlanes * C::kABytes, g.b_mn);
     uint32_t it = 0, n = 0;
-    for (int t = first; t < ntiles && ok; t += step) {
-      const Tile16 w = tile16<C>(g, t);
+    for (Tiles16<C> t(g, first, step); t.more() && ok; t.next()) {
+      const Tile16 w = t.get();
       for (int kc = w.kb0; kc < w.kb1 && ok; kc += C::kChunk, ++n) {
         const uint32_t acc = n % C::kBufs;
         if (n >= C::kBufs && !(ok = mbar_wait_warp(&tempty[acc], (n / C::kBufs - 1) & 1))) break;
@@ -408,11 +424,11 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
   }
   } else {
     if constexpr (C::kPromote) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    constexpr int kHalf = C::kN / 2;
-    const int q = warp & 3, half = (warp - kG16Epi) >> 2;
+    constexpr int kPart = C::kPart;
+    const int q = warp & 3, part = (warp - kG16Epi) >> 2;
     uint8_t* mine = outs + (warp - kG16Epi) * (C::kBoxes * kBoxBytes);
     OutStage<C::kBoxes> stage{smem_u32(mine), reinterpret_cast<float*>(mine), lane};
-    const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * kHalf);
+    const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(part * kPart);
     uint32_t n = 0;
     // warp-uniform, as the TMEM loads are warp-collective
     auto sums_ready = [&](uint32_t acc, uint32_t parity) {
@@ -431,41 +447,41 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
       __syncwarp();
       if (lane == 0) {
         if constexpr (C::kCtas == 2)
-          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapa_u32(smem_u32(&tempty[acc]), 0)) : "memory");
+          asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapa_u32(smem_u32(&tempty[acc]), 0)) : "memory");
         else
-          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&tempty[acc])) : "memory");
+          asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&tempty[acc])) : "memory");
       }
     };
     bool ok = true;
-    for (int t = first; t < ntiles && ok; t += step) {
-      const Tile16 w = tile16<C>(g, t);
-      const int row = w.m0 + rank * 128 + q * 32, col = w.n0 + half * kHalf;
-      Epi::template ahead<kHalf>(ep, w, row, col, lane);
+    for (Tiles16<C> t(g, first, step); t.more() && ok; t.next()) {
+      const Tile16 w = t.get();
+      const int row = w.m0 + rank * 128 + q * 32, col = w.n0 + part * kPart;
+      Epi::template ahead<kPart>(ep, w, row, col, lane);
       if constexpr (C::kPromote) {
-        float sum[kHalf];
+        float sum[kPart];
 #pragma unroll
-        for (int j = 0; j < kHalf; ++j) sum[j] = 0.f;
+        for (int j = 0; j < kPart; ++j) sum[j] = 0.f;
         for (int kc = w.kb0; kc < w.kb1; kc += C::kChunk, ++n) {
           const uint32_t acc = n % C::kBufs;
           if (!(ok = sums_ready(acc, (n / C::kBufs) & 1))) break;
 uint32_t r[2][32];
           tmem_load_32x32(lanes + acc * (uint32_t)C::kN, r[0]);
 #pragma unroll
-          for (int c = 0; c < kHalf; c += 32) {      // the next load is on its way while these are added
+          for (int c = 0; c < kPart; c += 32) {      // the next load is on its way while these are added
             tmem_load_wait();
-            if (c + 32 < kHalf) tmem_load_32x32(lanes + acc * (uint32_t)C::kN + (uint32_t)c + 32u, r[(c / 32 + 1) & 1]);
+            if (c + 32 < kPart) tmem_load_32x32(lanes + acc * (uint32_t)C::kN + (uint32_t)c + 32u, r[(c / 32 + 1) & 1]);
             else release(acc);
 #pragma unroll
             for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(r[(c / 32) & 1][j]);
           }
         }
         if (!ok) break;
-        Epi::template run<C::kPlanes, kHalf>(ep, g, w, row, col, half, stage, SumsInRegisters<kHalf>{sum}, [] {});
+        Epi::template run<C::kPlanes, kPart>(ep, g, w, row, col, part, stage, SumsInRegisters<kPart>{sum}, [] {});
       } else {
         const uint32_t acc = n % C::kBufs;
         if (!(ok = sums_ready(acc, (n / C::kBufs) & 1))) break;
         ++n;
-        Epi::template run<C::kPlanes, kHalf>(ep, g, w, row, col, half, stage, SumsInTmem<kHalf>{lanes + acc * (uint32_t)C::kN}, [&] { release(acc); });
+        Epi::template run<C::kPlanes, kPart>(ep, g, w, row, col, part, stage, SumsInTmem<kPart>{lanes + acc * (uint32_t)C::kN}, [&] { release(acc); });
       }
     }
     stage.drain();
@@ -582,15 +598,17 @@ int launch16(Chain& chain, psb::Gemm16Args& g, const Operand16& a, const Operand
     attr[dev] = true;
   }
   const int tiles = psb::tiles16<C>(g), most = sms / C::kCtas;
-  return chain.launch(psb::gemm16_kernel<C, Epi>, dim3((unsigned)((tiles < most ? tiles : most) * C::kCtas)), psb::kG16Threads, C::kSmemBytes, C::kCtas, g, ep);
+  return chain.launch(psb::gemm16_kernel<C, Epi>, dim3((unsigned)((tiles < most ? tiles : most) * C::kCtas)), C::kThreads, C::kSmemBytes, C::kCtas, g, ep);
 }
 
 // ---- which tiles, and in how many pieces K is taken
-enum : int { kPair256 = 0, kPair128 = 1, kOne128 = 2, kOne64 = 3, kKinds = 4 };      // 256x256 and 256x128 on a pair, 128x128, 128x64
+// 256x256 on a pair, with two or four epilogue warps for 32 rows, 256x128 on a pair, 128x128, 128x64
+enum : int { kPair256 = 0, kPair128 = 1, kOne128 = 2, kOne64 = 3, kKinds = 4, kPair256Wide = 4 };
 struct Tiling { int kind, splits, kb_split; };
 
-inline int tiling_rows(int kind) { return kind <= kPair128 ? 256 : 128; }
-inline int tiling_cols(int kind) { return kind == kPair256 ? 256 : kind == kOne64 ? 64 : 128; }
+inline int tiling_rows(int kind) { return kind <= kPair128 || kind == kPair256Wide ? 256 : 128; }
+inline int tiling_cols(int kind) { return kind == kPair256 || kind == kPair256Wide ? 256 : kind == kOne64 ? 64 : 128; }
+inline int tiling_parts(int kind) { return kind == kPair256Wide ? 4 : 2; }
 
 // The cheapest by this estimate, in cycles of an SM: rounds of tiles, each its blocks of K at the slower of the tensor
 // cores (128 x N x 64 in 2N cycles a product, as a rule) and the loads (48 bytes a cycle from L2, as measured with all SMs
@@ -616,12 +634,18 @@ inline Tiling choose_tiling(int64_t batch, int64_t M, int64_t N, int64_t K, int 
       if (t < least) { least = t; best = {kind, (int)s, (int)per}; }
     }
   }
+  // One plane: up to K = 768 a tile's products take less time than its epilogue, where two warps wait out each other's loads
+  // and exponentials (4096 x 65,536 scores, K = 512: 296 -> 208 us; K = 1024, 2 % slower: a stage less, more power).
+  if (best.kind == kPair256 && planes == 1 && best.kb_split <= 12) best.kind = kPair256Wide;
   return best;
 }
 
 template <int kPlanes, class Epi>
 int launch_tiled(Chain& chain, int kind, psb::Gemm16Args& g, const Operand16& a, const Operand16& b, const typename Epi::Params& ep) {
   if (kind == kPair256) return launch16<psb::Cfg16<2, 256, kPlanes>, Epi>(chain, g, a, b, ep);
+  if constexpr (kPlanes == 1) {
+    if (kind == kPair256Wide) return launch16<psb::Cfg16<2, 256, 1, 4>, Epi>(chain, g, a, b, ep);
+  }
   if (kind == kPair128) return launch16<psb::Cfg16<2, 128, kPlanes>, Epi>(chain, g, a, b, ep);
   if (kind == kOne128) return launch16<psb::Cfg16<1, 128, kPlanes>, Epi>(chain, g, a, b, ep);
   return launch16<psb::Cfg16<1, 64, kPlanes>, Epi>(chain, g, a, b, ep);

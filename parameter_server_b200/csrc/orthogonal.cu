@@ -120,19 +120,19 @@ struct EpiNs {
     int M, N, batch, second, dtype, update;
     float alpha, beta, alpha2, beta2, lr;
   };
-  template <int kHalf>
+  template <int kPart>
   static __device__ __forceinline__ void ahead(const Params& p, const Tile16& w, int row, int col, int lane) {
-    if (p.update && row + lane < p.M) prefetch_l2<kHalf>(reinterpret_cast<const float*>(p.result) + ((int64_t)w.z * p.M + row + lane) * p.N, col, p.N);
+    if (p.update && row + lane < p.M) prefetch_l2<kPart>(reinterpret_cast<const float*>(p.result) + ((int64_t)w.z * p.M + row + lane) * p.N, col, p.N);
   }
-  template <int kPlanes, int kHalf, class Stage, class Sums, class Done>
+  template <int kPlanes, int kPart, class Stage, class Sums, class Done>
   static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int, Stage& st,
                                              const Sums& sums, Done done) {
     constexpr int kFmt = kPlanes == 2 ? kFmtPlanes : kFmtF16;
 #pragma unroll 1
-    for (int k = 0; k < kHalf; k += 32) {
+    for (int k = 0; k < kPart; k += 32) {
       float v[32];
       sums.load(k, v);
-      if (k + 32 >= kHalf) done();
+      if (k + 32 >= kPart) done();
       const int col = col0 + k;
       if (row0 >= p.M || col >= p.N) continue;
       if (p.slots == nullptr && p.result == nullptr) {

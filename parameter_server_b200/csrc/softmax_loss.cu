@@ -4,12 +4,12 @@
 //   G_ij = c_i (e^{s_ij − lse_i} − [j = y_i])        gx = G w        gw = Gᵀ x
 //
 // The scores are tiles of a product on the tensor cores (gemm16.cuh) and never leave the SM: its epilogue keeps each row's
-// maximum m and sum Σ e^{s−m} over half a tile's classes, and the score of the row's label.  A second kernel joins the
-// halves of a row to its log-sum-exp.
+// maximum m and sum Σ e^{s−m} over a part of a tile's classes (32 to 128), and the score of the row's label.  A second
+// kernel joins the parts of a row to its log-sum-exp.
 //
-// For the gradients the epilogue also writes e^{s−m} · 2^15 in fp16 (relative to the half tile's own maximum, which is all
-// that is known then), for as many classes as the workspace holds; the second kernel turns it into G in place, with one
-// factor a half tile.  Making the scores once costs 6nVd operations instead of 8nVd, for a pass over 2 bytes an element
+// For the gradients the epilogue also writes e^{s−m} · 2^15 in fp16 (relative to the part's own maximum, which is all that
+// is known then), for as many classes as the workspace holds; the second kernel turns it into G in place, with one
+// factor a part.  Making the scores once costs 6nVd operations instead of 8nVd, for a pass over 2 bytes an element
 // (8192 rows, 131,072 classes, 2048 wide: 3.5 ms less for 0.7).  Classes beyond the workspace come in pieces, whose scores
 // are made again.  gw of a piece is complete, gx is summed over the pieces in fp32.  Sums have a fixed order: results do not
 // vary from run to run.
@@ -185,21 +185,21 @@ k_loss_pack(PackArgs px, PackArgs pw, int cols, const int64_t* __restrict__ y, i
 }
 
 // ------------------------------------------------------------------ epilogues
-// Each row's maximum and Σ 2^(s−m) over half a tile's classes, the score of its label, in units of log2 e, and the
+// Each row's maximum and Σ 2^(s−m) over a part of a tile's classes, the score of its label, in units of log2 e, and the
 // exponentials that are kept.
 struct EpiScore {
   struct Params {
     CUtensorMap e;             // exponentials [plane][n][keep]
-    float2* part;              // [n][2 · class tiles]
+    float2* part;              // [n][per_tile · class tiles]
     float* target;             // [n]
     const int64_t* y;
     ScaleRef scale;
-    int n, V, parts, keep;
+    int n, V, parts, per_tile, keep;
   };
-  template <int kHalf>
+  template <int kPart>
   static __device__ __forceinline__ void ahead(const Params&, const Tile16&, int, int, int) {}
-  template <int kPlanes, int kHalf, class Stage, class Sums, class Done>
-  static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int half, Stage& st,
+  template <int kPlanes, int kPart, class Stage, class Sums, class Done>
+  static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int part, Stage& st,
                                              const Sums& sums, Done done) {
     const float scale = score_scale(p.scale);
     const int row = row0 + st.lane;
@@ -207,7 +207,7 @@ struct EpiScore {
     if (row < p.n) lab = p.y[row];
     float top = -INFINITY;
 #pragma unroll 1
-    for (int c = 0; c < kHalf; c += 32) {
+    for (int c = 0; c < kPart; c += 32) {
       float v[32];
       sums.load(c, v);
       const int left = p.V - (col0 + c);
@@ -223,10 +223,10 @@ struct EpiScore {
     const float m = __fmul_rn(top, scale), ref = top == -INFINITY ? 0.f : m;
     float s = 0.f;
 #pragma unroll 1
-    for (int c = 0; c < kHalf; c += 32) {
+    for (int c = 0; c < kPart; c += 32) {
       float v[32];
       sums.load(c, v);
-      if (c + 32 >= kHalf) done();
+      if (c + 32 >= kPart) done();
       const int col = col0 + c, left = p.V - col;
       if (left <= 0) continue;
       if (lab >= col && lab < col + 32 && lab < p.V) {
@@ -247,7 +247,7 @@ struct EpiScore {
       }
       if (col < p.keep) st.template store<kPlanes == 2 ? kFmtPlanes : kFmtF16>(&p.e, v, row0, col, 0, false);
     }
-    if (row < p.n) p.part[(int64_t)row * p.parts + w.tn * 2 + half] = make_float2(top == -INFINITY ? top : m, s);
+    if (row < p.n) p.part[(int64_t)row * p.parts + w.tn * p.per_tile + part] = make_float2(top == -INFINITY ? top : m, s);
   }
 };
 
@@ -261,9 +261,9 @@ struct EpiG {
     ScaleRef scale;
     int n, V, len, v0, dtype;
   };
-  template <int kHalf>
+  template <int kPart>
   static __device__ __forceinline__ void ahead(const Params&, const Tile16&, int, int, int) {}
-  template <int kPlanes, int kHalf, class Stage, class Sums, class Done>
+  template <int kPlanes, int kPart, class Stage, class Sums, class Done>
   static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16&, int row0, int col0, int, Stage& st,
                                              const Sums& sums, Done done) {
     const float scale = score_scale(p.scale);
@@ -277,10 +277,10 @@ struct EpiG {
     }
     const bool none = row >= p.n || !has_class(p.y[row], p.V);
 #pragma unroll 1
-    for (int k = 0; k < kHalf; k += 32) {
+    for (int k = 0; k < kPart; k += 32) {
       float v[32];
       sums.load(k, v);
-      if (k + 32 >= kHalf) done();
+      if (k + 32 >= kPart) done();
       const int col = col0 + k;
       if (col >= p.len) continue;
       const int at = lab >= col && lab < col + 32 ? (int)(lab - col) : -1;
@@ -310,19 +310,19 @@ struct EpiGrad {
     int M, N, dtype, with_w, by_map;
     int read, write;           // acc is added to the product; the sum goes to acc instead of the result
   };
-  template <int kHalf>
+  template <int kPart>
   static __device__ __forceinline__ void ahead(const Params& p, const Tile16& w, int row, int col, int lane) {
-    if (p.read && row + lane < p.M) prefetch_l2<kHalf>(p.acc + w.split * p.slot + (int64_t)(row + lane) * p.N, col, p.N);
+    if (p.read && row + lane < p.M) prefetch_l2<kPart>(p.acc + w.split * p.slot + (int64_t)(row + lane) * p.N, col, p.N);
   }
-  template <int kPlanes, int kHalf, class Stage, class Sums, class Done>
+  template <int kPlanes, int kPart, class Stage, class Sums, class Done>
   static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int, Stage& st,
                                              const Sums& sums, Done done) {
     const float scale = grad_scale(p.scale, p.with_w);
 #pragma unroll 1
-    for (int k = 0; k < kHalf; k += 32) {
+    for (int k = 0; k < kPart; k += 32) {
       float v[32];
       sums.load(k, v);
-      if (k + 32 >= kHalf) done();
+      if (k + 32 >= kPart) done();
       const int col = col0 + k;
       if (row0 >= p.M || col >= p.N) continue;
       if (kPlanes == 1 && p.by_map) {
@@ -526,7 +526,7 @@ constexpr int kMaxBlocks = 148 * 8;           // of the pass that finds the larg
 
 // where things lie in the workspace; everything is 256-byte aligned
 struct LossPlan {
-  int planes, pack_x, pack_w, parts, keep, piece;
+  int planes, pack_x, pack_w, parts, per_tile, keep, piece;
   Tiling score, gx, gw;                       // gx, gw: of the kept classes, or of a piece
   int64_t dp, ldg, x_plane, w_plane, g_plane;
   int64_t scales, maxima, lse, target, x, w, part, g, gx_acc, gw_acc, total;
@@ -555,7 +555,8 @@ LossPlan make_loss_plan(const LossKey& a) {
   p.pack_w = a.pack_w;
   p.score = choose_tiling(1, a.n, a.V, a.d, p.planes, false, 1);
   const int cols = tiling_cols(p.score.kind);
-  p.parts = 2 * ((a.V + cols - 1) / cols);
+  p.per_tile = tiling_parts(p.score.kind);
+  p.parts = p.per_tile * ((a.V + cols - 1) / cols);
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
   p.scales = take(sizeof(Scales));
@@ -672,14 +673,14 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
   g.M = a.n; g.N = a.V; g.K = a.d;
   g.kb_split = (a.d + kG16K - 1) / kG16K;
   EpiScore::Params es = {};
-  es.part = part; es.target = target; es.y = a.y; es.scale = scale; es.n = a.n; es.V = a.V; es.parts = p.parts; es.keep = p.keep;
+  es.part = part; es.target = target; es.y = a.y; es.scale = scale; es.n = a.n; es.V = a.V; es.parts = p.parts; es.per_tile = p.per_tile; es.keep = p.keep;
   if (a.want_grad && (r = make_out_map(&es.e, Operand16{gb, a.n, p.keep, p.ldg, p.g_plane, p.planes}, 0)) != 0) return r;
   if ((r = product16<EpiScore>(chain, p.planes, p.score.kind, g, x, w, es)) != 0) return r;
 
   // losses, and G of the kept classes
   JoinArgs j = {};
   j.part = part; j.target = target; j.y = a.y; j.coef = a.coef; j.lse = lse; j.loss = a.loss; j.scale = scale;
-  j.n = a.n; j.V = a.V; j.d = a.d; j.parts = p.parts; j.shift = tiling_cols(p.score.kind) == 256 ? 7 : tiling_cols(p.score.kind) == 128 ? 6 : 5; j.keep = p.keep; j.dtype = a.dtype; j.status = a.status;
+  j.n = a.n; j.V = a.V; j.d = a.d; j.parts = p.parts; for (j.shift = 5; tiling_cols(p.score.kind) / p.per_tile > 1 << j.shift; ++j.shift) {} j.keep = p.keep; j.dtype = a.dtype; j.status = a.status;
   if (a.want_grad) {
     j.g = gb; j.ldg = p.ldg; j.plane = p.g_plane;
     if (!p.pack_x) { j.x = reinterpret_cast<const uint16_t*>(a.x); j.x_out = xb; j.ldx = a.ldx; j.ldxo = p.dp; }
