@@ -604,34 +604,40 @@ int launch16(Chain& chain, psb::Gemm16Args& g, const Operand16& a, const Operand
 // ---- which tiles, and in how many pieces K is taken
 // 256x256 on a pair, with two or four epilogue warps for 32 rows, 256x128 on a pair, 128x128, 128x64
 enum : int { kPair256 = 0, kPair128 = 1, kOne128 = 2, kOne64 = 3, kKinds = 4, kPair256Wide = 4 };
-struct Tiling { int kind, splits, kb_split; };
+struct Tiling { int kind, splits, kb_split, sym; };
 
 inline int tiling_rows(int kind) { return kind <= kPair128 || kind == kPair256Wide ? 256 : 128; }
 inline int tiling_cols(int kind) { return kind == kPair256 || kind == kPair256Wide ? 256 : kind == kOne64 ? 64 : 128; }
 inline int tiling_parts(int kind) { return kind == kPair256Wide ? 4 : 2; }
 
-// The cheapest by this estimate, in cycles of an SM: rounds of tiles, each its blocks of K at the slower of the tensor
-// cores (128 x N x 64 in 2N cycles a product, as a rule) and the loads (48 bytes a cycle from L2, as measured with all SMs
-// busy), plus what does not overlap in the last round, plus storing and adding up the pieces of K (a launch, 5000 bytes a cycle).
-inline Tiling choose_tiling(int64_t batch, int64_t M, int64_t N, int64_t K, int planes, bool sym, int max_splits, int only = -1) {
+// The cheapest by this estimate, in cycles of an SM.  A round of tiles costs its blocks of K, at the slower of the tensor
+// cores (128 x N x 64 in 2N cycles a product) and the loads (48 bytes a cycle), or the epilogue where that takes longer:
+// 700 cycles for 32 rows x 32 columns of a plane and a warp, by clock readings (`outputs` of them, twice for a mirror image).
+// The last round's epilogue comes on top; with two planes, whose sums are in its warps' registers, that of every round.  Pieces of
+// K cost a launch that adds them up and their bytes, 5000 a cycle.  A symmetric product may make all tiles: where one round
+// holds them, that saves the mirror images (512 x 512, two planes: 22 -> 14 k cycles).
+inline Tiling choose_tiling(int64_t batch, int64_t M, int64_t N, int64_t K, int planes, bool symmetric, int max_splits, int outputs = 1) {
   const int64_t nkb = (K + psb::kG16K - 1) / psb::kG16K;
-  Tiling best = {kOne64, 1, (int)nkb};
+  Tiling best = {kOne64, 1, (int)nkb, 0};
   double least = 1e300;
   for (int kind = 0; kind < kKinds; ++kind) {
     const int64_t rows = tiling_rows(kind), cols = tiling_cols(kind);
-    if ((only >= 0 && kind != only) || (sym && rows != cols)) continue;
     const int64_t tm = (M + rows - 1) / rows, tn = (N + cols - 1) / cols, slots = rows == 256 ? 74 : 148;
-    const int64_t tiles = batch * (sym ? tm * (tm + 1) / 2 : tm * tn);
-    const double mma = 2.0 * cols * (planes == 2 ? 3 : 1);
-    const double load = planes * (16384.0 + 128.0 * cols * 128.0 / rows) / 48.0;
-    for (int64_t s = 1; s <= max_splits && s <= nkb; ++s) {
-      const int64_t per = (nkb + s - 1) / s, real = (nkb + per - 1) / per;
-      if (real != s) continue;
-      if (s > 1 && per < 4) break;
-      const int64_t rounds = (tiles * s + slots - 1) / slots;
-      double t = (double)rounds * (double)per * (mma > load ? mma : load) + 12.0 * (double)cols + 600.0 * (double)rounds;
-      if (s > 1) t += 5000.0 + (double)batch * M * N * (8.0 * s + 4.0) / 5000.0;
-      if (t < least) { least = t; best = {kind, (int)s, (int)per}; }
+    for (int sym = 0; sym <= (symmetric && rows == cols ? 1 : 0); ++sym) {
+      const int64_t tiles = batch * (sym ? tm * (tm + 1) / 2 : tm * tn);
+      const double mma = 2.0 * cols * (planes == 2 ? 3 : 1);
+      const double load = planes * (16384.0 + 128.0 * cols * 128.0 / rows) / 48.0;
+      const double plain = 700.0 * cols / 64.0, epilogue = plain * planes * outputs * (sym && tm > 1 ? 1.8 : 1.0);
+      for (int64_t s = 1; s <= max_splits && s <= nkb; ++s) {
+        const int64_t per = (nkb + s - 1) / s, real = (nkb + per - 1) / per;
+        if (real != s) continue;
+        if (s > 1 && per < 4) break;
+        const double rounds = (double)((tiles * s + slots - 1) / slots), main = (double)per * (mma > load ? mma : load);
+        const double e = s > 1 ? 2.0 * plain : epilogue;          // fp32 sums of a piece
+        double t = planes == 2 ? rounds * (main + e + 600.0) : rounds * ((main > e ? main : e) + 600.0) + e;
+        if (s > 1) t += 5000.0 + (double)batch * M * N * (8.0 * s + 4.0) / 5000.0;
+        if (t < least) { least = t; best = {kind, (int)s, (int)per, sym}; }
+      }
     }
   }
   // One plane: up to K = 768 a tile's products take less time than its epilogue, where two warps wait out each other's loads

@@ -181,15 +181,15 @@ struct EpiNs {
 };
 
 // The splits of a product's K to planes: alpha · sum + beta · I, and the second matrix.  Of a symmetric product only the
-// tiles (tile x tile) on and above the diagonal exist.  A block takes 32 x 32, a thread four neighbours, and stores them
+// tiles (tile x tile) on and above the diagonal exist (tile 0: all do).  A block takes 32 x 32, a thread four neighbours, and stores them
 // and, through shared memory, their transpose.
 __global__ void __launch_bounds__(256)
 k_orth_sum(const float* __restrict__ slots, int splits, int batch, int n, int tile, uint16_t* __restrict__ out, uint16_t* __restrict__ out2,
            int64_t ld, int64_t plane, float alpha, float beta, float alpha2, float beta2) {
   __shared__ float sum[32][33];
   const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32, z = blockIdx.z;
-  if (r0 / tile > c0 / tile) return;
-  const bool twice = r0 / tile < c0 / tile;
+  if (tile > 0 && r0 / tile > c0 / tile) return;
+  const bool twice = tile > 0 && r0 / tile < c0 / tile;
   pdl_wait();
   const int ty = threadIdx.x >> 3, tx = (threadIdx.x & 7) * 4;
   const int64_t per = (int64_t)n * n, total = per * batch, base = (int64_t)z * 2 * plane;
@@ -737,7 +737,7 @@ OrthPlan make_orth_plan(const OrthKey& a) {
   if ((int64_t)a.batch * 16 < (1 << 30) && small_plan(p, a.batch)) { p.small = 1; return p; }
   int64_t slots = 0;
   for (int k = 0; k < 2; ++k) {
-    p.gram[k] = choose_tiling(a.batch, p.lo, p.lo, p.hi, k + 1, true, 32);
+    p.gram[k] = choose_tiling(a.batch, p.lo, p.lo, p.hi, k + 1, true, 32, 2);
     p.square[k] = choose_tiling(a.batch, p.lo, p.lo, p.lo, k + 1, true, 8);
     p.step[k] = choose_tiling(a.batch, a.rows, a.cols, p.lo, k + 1, false, 1);
     for (const Tiling& t : {p.gram[k], p.square[k]}) if (t.splits > 1 && t.splits > slots) slots = t.splits;
@@ -824,13 +824,13 @@ int psb_orthogonal(const OrthArgs* ap, cudaStream_t s) {
 
   // a symmetric product of side lo, whole or split
   auto square = [&](const Tiling& t, int planes, Gemm16Args q, const Operand16& x, const Operand16& y, EpiNs::Params e, uint16_t* out, uint16_t* out2) {
-    q.M = q.N = p.lo; q.sym = 1; q.splits = t.splits; q.kb_split = t.kb_split;
+    q.M = q.N = p.lo; q.sym = t.sym; q.splits = t.splits; q.kb_split = t.kb_split;
     e.M = e.N = p.lo; e.batch = a.batch;
     if (t.splits > 1) e.slots = slots;
     int rc = product16<EpiNs>(chain, planes, t.kind, q, x, y, e);
     if (rc == 0 && t.splits > 1) {
       const unsigned nt = (unsigned)((p.lo + 31) / 32);
-      rc = chain.launch(k_orth_sum, dim3(nt, nt, (unsigned)a.batch), 256, 0, 1, slots, t.splits, a.batch, p.lo, tiling_rows(t.kind), out, out2,
+      rc = chain.launch(k_orth_sum, dim3(nt, nt, (unsigned)a.batch), 256, 0, 1, slots, t.splits, a.batch, p.lo, t.sym ? tiling_rows(t.kind) : 0, out, out2,
                         p.ldl, p.lplane, e.alpha, e.beta, e.alpha2, e.beta2);
     }
     return rc;
