@@ -594,7 +594,11 @@ int launch16(Chain& chain, psb::Gemm16Args& g, const Operand16& a, const Operand
   static bool attr[kMaxDevices] = {};
   if (!attr[dev]) {
     cudaError_t e = cudaFuncSetAttribute(psb::gemm16_kernel<C, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+    cudaFuncAttributes fa;
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, psb::gemm16_kernel<C, Epi>);
     if (e != cudaSuccess) return (int)e;
+    // the epilogue's warps wait for registers that the launch has to have brought
+    if (C::kPromote && fa.numRegs * C::kThreads < 128 * 56 + 256 * 224) return (int)cudaErrorLaunchOutOfResources;
     attr[dev] = true;
   }
   const int tiles = psb::tiles16<C>(g), most = sms / C::kCtas;

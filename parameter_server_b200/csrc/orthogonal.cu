@@ -696,12 +696,12 @@ struct OrthPlan {
 constexpr int kSmallSmem = 226 * 1024;      // of 227 KB
 // How many CTAs hold a matrix with a short side of at most 128: the cheapest number by this estimate of a step's cycles,
 // which follows clock readings of 64x64 (5.4 k, one CTA), 128x128 (18 k, one) and 64x2048 (17.8 k on 4 CTAs).
-bool small_plan(OrthPlan& p, int batch) {
+bool small_plan(OrthPlan& p, int batch, int largest) {
   if (p.lo > 128) return false;
   p.lop = (p.lo + 15) / 16 * 16;
   const int square = 4 * p.lop * ((p.lop + 63) / 64 * 64);
   double least = 1e300;
-  for (int cl = 1; cl <= 16; cl *= 2) {
+  for (int cl = 1; cl <= largest; cl *= 2) {
     const int64_t hs = (((int64_t)p.hi + cl - 1) / cl + 63) / 64 * 64;
     if (hs > 512 || (hs + 127) / 128 * 2 * p.lop > 512) continue;                            // of TMEM
     const int sums = cl > 1 ? 4 * p.lop * p.lop : 0;
@@ -724,9 +724,38 @@ bool orth_args_ok(const OrthArgs& a) {
          a.dtype >= kOrthF32 && a.dtype <= kOrthF16;
 }
 
+// The largest cluster of k_orth_small that the current GPU takes: 16 CTAs, where its GPCs have as many SMs, 8 for certain;
+// 0 where it cannot run.
+int largest_cluster() {
+  static int known[kMaxDevices] = {};            // one more
+  int dev = 0;
+  if (sm_count(&dev) <= 0) return 0;
+  if (known[dev] == 0) {
+    cudaError_t e = cudaFuncSetAttribute(k_orth_small, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmallSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_orth_small, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    int largest = 0;
+    for (int cl = 16; cl >= 8 && e == cudaSuccess && largest == 0; cl /= 2) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)cl);
+      cfg.blockDim = dim3(kSmallThreads);
+      cfg.dynamicSmemBytes = kSmallSmem;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = (unsigned)cl; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      int clusters = 0;
+      if (cudaOccupancyMaxActiveClusters(&clusters, k_orth_small, &cfg) == cudaSuccess && clusters > 0) largest = cl;
+    }
+    cudaGetLastError();                          // what the question left behind
+    known[dev] = largest + 1;
+  }
+  return known[dev] - 1;
+}
+
 struct OrthKey {
-  int batch, rows, cols;
-  bool operator==(const OrthKey& o) const { return batch == o.batch && rows == o.rows && cols == o.cols; }
+  int batch, rows, cols, largest;
+  bool operator==(const OrthKey& o) const { return batch == o.batch && rows == o.rows && cols == o.cols && largest == o.largest; }
 };
 
 OrthPlan make_orth_plan(const OrthKey& a) {
@@ -734,7 +763,7 @@ OrthPlan make_orth_plan(const OrthKey& a) {
   p.tall = a.rows > a.cols;
   p.lo = p.tall ? a.cols : a.rows;
   p.hi = p.tall ? a.rows : a.cols;
-  if ((int64_t)a.batch * 16 < (1 << 30) && small_plan(p, a.batch)) { p.small = 1; return p; }
+  if ((int64_t)a.batch * 16 < (1 << 30) && small_plan(p, a.batch, a.largest)) { p.small = 1; return p; }
   int64_t slots = 0;
   for (int k = 0; k < 2; ++k) {
     p.gram[k] = choose_tiling(a.batch, p.lo, p.lo, p.hi, k + 1, true, 32, 2);
@@ -763,7 +792,7 @@ OrthPlan make_orth_plan(const OrthKey& a) {
 OrthPlan orth_plan(const OrthArgs& a) {
   struct Entry { OrthKey key; OrthPlan plan; bool used; };
   static thread_local Entry kept[16] = {};
-  const OrthKey k{a.batch, a.rows, a.cols};
+  const OrthKey k{a.batch, a.rows, a.cols, largest_cluster()};
   Entry& e = kept[((unsigned)k.batch * 31u + (unsigned)k.rows * 7u + (unsigned)k.cols * 13u) % 16u];
   if (!e.used || !(e.key == k)) e = Entry{k, make_orth_plan(k), true};
   return e.plan;
@@ -783,15 +812,6 @@ int psb_orthogonal(const OrthArgs* ap, cudaStream_t s) {
   const OrthPlan p = orth_plan(a);
   if (p.small) {
     Chain chain{s};
-    int dev = 0;
-    if (sm_count(&dev) <= 0) return (int)cudaErrorInvalidDevice;
-    static bool attr[kMaxDevices] = {};
-    if (!attr[dev]) {
-      cudaError_t e = cudaFuncSetAttribute(k_orth_small, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmallSmem);
-      if (e == cudaSuccess) e = cudaFuncSetAttribute(k_orth_small, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e != cudaSuccess) return (int)e;
-      attr[dev] = true;
-    }
     const SmallArgs q{a, p.lo, p.hi, p.tall, p.lop, p.hs, p.cl, p.a_off, p.a2_off, p.p_off};
     return chain.launch(k_orth_small, dim3((unsigned)(a.batch * p.cl)), kSmallThreads, p.smem, p.cl, q);
   }

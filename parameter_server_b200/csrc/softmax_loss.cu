@@ -67,8 +67,11 @@ __device__ __forceinline__ uint32_t block_max_u32(uint32_t v) {       // of 256 
 __device__ __forceinline__ uint32_t coef_max(const float* coef, const int64_t* y, int n, int V) {
   if (coef == nullptr) return __float_as_uint(1.f);
   uint32_t top = 0;
-  for (int i = threadIdx.x; i < n; i += 256)
-    if (has_class(y[i], V)) top = max(top, finite_bits(coef[i]));
+#pragma unroll 8
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const float c = coef[i];
+    if (has_class(y[i], V)) top = max(top, finite_bits(c));
+  }
   return block_max_u32(top);
 }
 // fp16 with coefficients: the scale of G alone (one block)

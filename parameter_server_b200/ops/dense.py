@@ -36,6 +36,8 @@ def check_status(dev) -> None:
     st = _status_for(dev).tolist()
     if st[0] != 0:
         _status_for(dev).zero_()
+        if st[0] != 1:
+            raise RuntimeError(f"{N.STATUS_NAMES.get(st[0], 'unknown status')} (code {st[0]}: {st[1]}, {st[2]})")
         raise RuntimeError(f"GEMM kernel gave up waiting (code {st[0]}, tile {st[1]},{st[2] - 100})")
 
 

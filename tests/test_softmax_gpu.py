@@ -227,6 +227,47 @@ def test_captured_replayed_and_on_another_stream():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_without_the_gradient_of_the_rows(dtype):
+    from parameter_server_b200.ops import softmax
+
+    x, w, y = _data(70, 400, 40, dtype, 10)
+    want = softmax.softmax_loss(x, w, y)
+    loss, gx, gw = softmax.softmax_loss(x, w, y, want_gx=False)
+    assert gx is None and torch.equal(loss, want[0]) and torch.equal(gw, want[2])
+
+
+def test_many_rows_of_few_classes():
+    """More rows than a pass of the grid, coefficients searched for their largest, one tile of classes."""
+    x, w, y = _data(70_001, 9, 12, torch.float16, 11)
+    _check(x, w, y, torch.rand(70_001, device="cuda") * 1e-3)
+
+
+def test_another_thread_and_other_operators_between():
+    """Two threads that call the operators on one stream: launches of one may come between those of the other."""
+    import threading
+
+    from parameter_server_b200.ops import orthogonal, softmax
+
+    x, w, y = _data(200, 3000, 96, torch.float32, 12)
+    m = torch.randn(300, 200, device="cuda")
+    want, want_o = softmax.softmax_loss(x, w, y), orthogonal.orthogonalize(m)
+    got = {}
+
+    def work(k):
+        got[k] = [softmax.softmax_loss(x, w, y) if (i + k) % 2 else orthogonal.orthogonalize(m) for i in range(20)]
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for results in got.values():
+        for r in results:
+            assert torch.equal(r, want_o) if isinstance(r, torch.Tensor) else all(torch.equal(a, b) for a, b in zip(r, want))
+
+
 def test_no_rows():
     from parameter_server_b200.ops import softmax
 
