@@ -679,6 +679,181 @@ k_orth_small(const __grid_constant__ SmallArgs p) {
   if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
+// ------------------------------------------------------------------ matrices with a short side of at most 16
+// Such a matrix stays in registers: a thread holds whole columns of X (C of the longer side's), A is summed over threads, warps
+// and CTAs of a cluster, and X = (a I + b A + c A²) X is C · lo² multiplications of a thread.  fp32 throughout, no tensor
+// cores: a product of 16 rows would leave seven eighths of theirs idle, and their cut sums are what the last bits of so
+// small a result would show.
+constexpr int kThinThreads = 256, kThinColumns = 1024;     // of a CTA
+
+struct ThinArgs {
+  OrthArgs o;
+  int lo, hi, tall, cl;
+};
+
+// Sums over the lanes of a warp: lane l ends up with v[0..PL) = the sums of values PL·l.. of the N (padded to 32 PL).  Halves
+// are exchanged, so that it takes N shuffles instead of 5 N.
+template <int PL, int kHalf = 16>
+__device__ __forceinline__ void warp_scatter_sum(float (&v)[32 * PL], int lane) {
+  const bool upper = lane & kHalf;
+#pragma unroll
+  for (int i = 0; i < kHalf * PL; ++i) {
+    const float keep = upper ? v[i + kHalf * PL] : v[i], give = upper ? v[i] : v[i + kHalf * PL];
+    v[i] = keep + __shfl_xor_sync(0xffffffffu, give, kHalf);
+  }
+  if constexpr (kHalf > 1) warp_scatter_sum<PL, kHalf / 2>(v, lane);
+}
+
+template <int LO, int C>
+__global__ void __launch_bounds__(kThinThreads, 1)
+k_orth_thin(const __grid_constant__ ThinArgs p) {
+  constexpr int kSums = LO * (LO + 1) / 2, PL = (kSums + 31) / 32, kWarps = kThinThreads / 32;
+  __shared__ float part[kWarps][32 * PL], all[2][16][32 * PL];
+  __shared__ __align__(16) float a[LO][LO], b[LO][LO < 4 ? 4 : LO];
+  __shared__ double norms[kWarps], slices[16];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = p.cl > 1 ? (int)cluster_rank() : 0, z = blockIdx.x / p.cl;
+  const int64_t at0 = (int64_t)z * p.o.rows * p.o.cols;
+  const int64_t by_row = p.tall ? 1 : p.hi, by_col = p.tall ? p.lo : 1;
+  pdl_wait();
+
+  float x[C][LO];
+  double acc = 0.0;
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    const int c = rank * (kThinThreads * C) + k * kThinThreads + tid;
+    const int64_t at = at0 + c * by_col;
+    float m[LO];
+#pragma unroll
+    for (int r = 0; r < LO; ++r) x[k][r] = r < p.lo && c < p.hi ? load_as(p.o.x, at + r * by_row, p.o.dtype) : 0.f;
+    if (p.o.m != nullptr) {
+#pragma unroll
+      for (int r = 0; r < LO; ++r) m[r] = r < p.lo && c < p.hi ? p.o.m[at + r * by_row] : 0.f;
+#pragma unroll
+      for (int r = 0; r < LO; ++r) {
+        m[r] = p.o.momentum * m[r] + x[k][r];
+        x[k][r] = update_direction(x[k][r], m[r], p.o.momentum, p.o.nesterov);
+        if (r < p.lo && c < p.hi) p.o.m[at + r * by_row] = m[r];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < LO; ++r) acc += (double)x[k][r] * x[k][r];
+  }
+  acc = warp_sum_d(acc);
+  if (lane == 0) norms[warp] = acc;
+  __syncthreads();
+  double total = 0.0;
+  for (int i = 0; i < kWarps; ++i) total += norms[i];
+  if (p.cl > 1) {
+    cluster_sync_all();                                   // every CTA runs
+    if (tid < p.cl)
+      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(mapa_u32(smem_u32(&slices[rank]), (uint32_t)tid)), "d"(total) : "memory");
+    cluster_sync_all();
+    total = 0.0;
+    for (int i = 0; i < p.cl; ++i) total += slices[i];
+  }
+  const double f = 1.0 / (sqrt(total) + (double)p.o.eps);
+#pragma unroll
+  for (int k = 0; k < C; ++k)
+#pragma unroll
+    for (int r = 0; r < LO; ++r) x[k][r] = (float)((double)x[k][r] * f);
+
+  for (int step = 0; step < p.o.steps; ++step) {
+    // A, the sums on and above the diagonal row by row
+    {
+      float v[32 * PL];
+#pragma unroll
+      for (int i = 0; i < LO; ++i)
+#pragma unroll
+        for (int j = i; j < LO; ++j) {
+          const int n = i * LO - i * (i - 1) / 2 + j - i;
+          v[n] = x[0][i] * x[0][j];
+#pragma unroll
+          for (int k = 1; k < C; ++k) v[n] += x[k][i] * x[k][j];
+        }
+#pragma unroll
+      for (int n = kSums; n < 32 * PL; ++n) v[n] = 0.f;
+      warp_scatter_sum<PL>(v, lane);
+#pragma unroll
+      for (int i = 0; i < PL; ++i) part[warp][lane * PL + i] = v[i];
+    }
+    __syncthreads();
+    float sum = 0.f;
+    if (tid < kSums)
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) sum += part[i][tid];
+    if (p.cl > 1) {                                       // to every CTA; the steps take turns, so one barrier is enough
+      if (tid < kSums)
+        for (int s = 0; s < p.cl; ++s)
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_u32(smem_u32(&all[step & 1][rank][tid]), (uint32_t)s)), "f"(sum) : "memory");
+      cluster_sync_all();
+      sum = 0.f;
+      if (tid < kSums)
+        for (int s = 0; s < p.cl; ++s) sum += all[step & 1][s][tid];
+    }
+    if (tid < kSums) {
+      int i = 0, j = tid;
+      while (j >= LO - i) { j -= LO - i; ++i; }
+      a[i][i + j] = sum;
+      a[i + j][i] = sum;
+    }
+    __syncthreads();
+    if (tid < LO * LO) {
+      const int i = tid / LO, j = tid % LO;
+      float sq = 0.f;
+#pragma unroll
+      for (int k = 0; k < LO; ++k) sq = fmaf(a[i][k], a[k][j], sq);
+      b[i][j] = fmaf(kNsC, sq, kNsB * a[i][j]) + (i == j ? kNsA : 0.f);
+    }
+    __syncthreads();
+    float y[C][LO];
+#pragma unroll
+    for (int i = 0; i < LO; ++i) {
+      float row[LO];
+#pragma unroll
+      for (int j = 0; j < LO; j += 4) {
+        const float4 t = *reinterpret_cast<const float4*>(&b[i][j]);
+        row[j] = t.x;
+        if (j + 1 < LO) row[j + 1] = t.y;
+        if (j + 2 < LO) row[j + 2] = t.z;
+        if (j + 3 < LO) row[j + 3] = t.w;
+      }
+#pragma unroll
+      for (int k = 0; k < C; ++k) {
+        float t = row[0] * x[k][0];
+#pragma unroll
+        for (int j = 1; j < LO; ++j) t = fmaf(row[j], x[k][j], t);
+        y[k][i] = t;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < C; ++k)
+#pragma unroll
+      for (int i = 0; i < LO; ++i) x[k][i] = y[k][i];
+  }
+
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    const int c = rank * (kThinThreads * C) + k * kThinThreads + tid;
+    if (c >= p.hi) continue;
+    const int64_t at = at0 + c * by_col;
+    float* out = reinterpret_cast<float*>(p.o.out);
+    float w[LO];
+#pragma unroll
+    for (int r = 0; r < LO; ++r) w[r] = p.o.m != nullptr && r < p.lo ? out[at + r * by_row] : 0.f;
+#pragma unroll
+    for (int r = 0; r < LO; ++r) {
+      if (r >= p.lo) continue;
+      const int64_t to = at + r * by_row;
+      if (p.o.m != nullptr) out[to] = w[r] - p.o.lr * x[k][r];
+      else if (p.o.dtype == kOrthF32) out[to] = x[k][r];
+      else if (p.o.dtype == kOrthBF16) reinterpret_cast<__nv_bfloat16*>(p.o.out)[to] = __float2bfloat16_rn(x[k][r]);
+      else reinterpret_cast<__half*>(p.o.out)[to] = __float2half_rn(x[k][r]);
+    }
+  }
+  if (p.cl > 1) cluster_sync_all();                       // no CTA leaves while another may still write to it
+}
+
 }  // namespace psb
 
 using namespace psb;
@@ -690,6 +865,7 @@ struct OrthPlan {
   Tiling gram[2], square[2], step[2];         // with one plane, with two
   int64_t ldx, xplane, ldl, lplane;
   int64_t part, x0, x1, a, a2, b, slots, total;
+  int thin;                                    // a cluster of cl CTAs of k_orth_thin, thin columns a thread
   int small, lop, hs, cl, a_off, a2_off, p_off, smem;      // small: a cluster of cl CTAs holds the matrix
 };
 
@@ -722,6 +898,20 @@ bool small_plan(OrthPlan& p, int batch, int largest) {
 bool orth_args_ok(const OrthArgs& a) {
   return a.batch > 0 && a.rows > 0 && a.cols > 0 && a.batch <= 65535 && a.rows <= (1 << 30) && a.cols <= (1 << 30) && a.steps > 0 &&
          a.dtype >= kOrthF32 && a.dtype <= kOrthF16;
+}
+
+// How many CTAs hold a matrix with a short side of at most 16, and how many columns a thread: as few columns as the SMs and the
+// clusters allow, as a step's work is the columns' and its barriers cost the same.
+bool thin_plan(OrthPlan& p, int batch, int largest) {
+  if (p.lo > 16) return false;
+  for (int c = 1; c <= kThinColumns / kThinThreads; c *= 2)
+    for (int cl = 1; cl <= largest; cl *= 2)
+      if ((int64_t)cl * kThinThreads * c >= p.hi && ((int64_t)batch * cl <= 148 || c == kThinColumns / kThinThreads)) {
+        p.thin = c;
+        p.cl = cl;
+        return true;
+      }
+  return false;
 }
 
 // The largest cluster of k_orth_small that the current GPU takes: 16 CTAs, where its GPCs have as many SMs, 8 for certain;
@@ -763,6 +953,8 @@ OrthPlan make_orth_plan(const OrthKey& a) {
   p.tall = a.rows > a.cols;
   p.lo = p.tall ? a.cols : a.rows;
   p.hi = p.tall ? a.rows : a.cols;
+  // registers, shared memory, or the general way
+  if ((int64_t)a.batch * 16 < (1 << 30) && thin_plan(p, a.batch, a.largest)) return p;
   if ((int64_t)a.batch * 16 < (1 << 30) && small_plan(p, a.batch, a.largest)) { p.small = 1; return p; }
   int64_t slots = 0;
   for (int k = 0; k < 2; ++k) {
@@ -788,6 +980,23 @@ OrthPlan make_orth_plan(const OrthKey& a) {
   return p;
 }
 
+template <int LO, int C>
+int thin_launch(Chain& chain, const ThinArgs& q) {
+  int dev = 0;
+  if (sm_count(&dev) <= 0) return (int)cudaErrorInvalidDevice;
+  static bool attr[kMaxDevices] = {};
+  if (!attr[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(k_orth_thin<LO, C>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return (int)e;
+    attr[dev] = true;
+  }
+  return chain.launch(k_orth_thin<LO, C>, dim3((unsigned)(q.o.batch * q.cl)), kThinThreads, 0, q.cl, q);
+}
+template <int LO>
+int thin_rows(Chain& chain, int columns, const ThinArgs& q) {
+  return columns == 1 ? thin_launch<LO, 1>(chain, q) : columns == 2 ? thin_launch<LO, 2>(chain, q) : thin_launch<LO, 4>(chain, q);
+}
+
 // a thread keeps the plans of the sizes that it met last: the search for tiles takes microseconds
 OrthPlan orth_plan(const OrthArgs& a) {
   struct Entry { OrthKey key; OrthPlan plan; bool used; };
@@ -810,6 +1019,14 @@ int psb_orthogonal(const OrthArgs* ap, cudaStream_t s) {
   const OrthArgs& a = *ap;
   if (!orth_args_ok(a)) return (int)cudaErrorInvalidValue;
   const OrthPlan p = orth_plan(a);
+  if (p.thin) {
+    Chain chain{s};
+    const ThinArgs q{a, p.lo, p.hi, p.tall, p.cl};
+    if (p.lo <= 1) return thin_rows<1>(chain, p.thin, q);
+    if (p.lo <= 2) return thin_rows<2>(chain, p.thin, q);
+    if (p.lo <= 4) return thin_rows<4>(chain, p.thin, q);
+    return p.lo <= 8 ? thin_rows<8>(chain, p.thin, q) : thin_rows<16>(chain, p.thin, q);
+  }
   if (p.small) {
     Chain chain{s};
     const SmallArgs q{a, p.lo, p.hi, p.tall, p.lop, p.hs, p.cl, p.a_off, p.a2_off, p.p_off};

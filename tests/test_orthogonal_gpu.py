@@ -76,7 +76,10 @@ def _check(x, steps=5):
                                    (1000, 520), (513, 2049), (1025, 1023), (2600, 2500), (3, 40, 72), (5, 72, 40), (2, 257, 1100), (300, 17, 5),
                                    # one CTA, clusters of 2 to 16, either way round, and what just does not fit
                                    (128, 128), (17, 512), (16, 513), (128, 200), (100, 400), (400, 100), (64, 1025), (128, 1024), (128, 1025),
-                                   (1024, 127), (112, 2048), (3, 48, 3000), (2, 8192, 64), (64, 8193), (129, 130)])
+                                   (1024, 127), (112, 2048), (3, 48, 3000), (2, 8192, 64), (64, 8193), (129, 130),
+                                   # in registers: every number of rows, columns a thread and CTAs, and what just does not fit
+                                   (2, 300), (3, 2), (4, 4097), (5, 70), (8, 512), (700, 9), (15, 1), (16, 16), (16, 257), (16, 16384), (16385, 16),
+                                   (17, 17), (200, 3, 5), (40, 16, 1100), (150, 700, 2), (1, 16500)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_orthogonalize(shape, dtype):
     _check(_data(shape).to(dtype))
