@@ -67,6 +67,14 @@ struct Gemm16Args {
   uint32_t* status;
 };
 
+// One product, or two whose tiles are dealt to the CTAs as one list: small ones that do not depend on one another.  (How many
+// is known to the compiler: arguments at an address that is not cost a large product 3 %.)
+template <class Epi, int kCount>
+struct Launch16 {
+  Gemm16Args g[kCount];
+  typename Epi::Params ep[kCount];
+};
+
 struct Tile16 {
   int z, split, m0, n0, kb0, kb1, tn;
   bool mirror;                 // the tile lies above the diagonal of a symmetric result
@@ -310,9 +318,9 @@ struct SumsInRegisters {
 // row: the first of the warp's 32 rows, col: the first of its kPart columns, the tile's part-th (either may lie outside the result); done() is
 // called after the last load of sums.  ahead<kPart>(params, tile, row, col, lane) is called while the products of the tile are
 // made, for what the epilogue is going to read.
-template <class C, class Epi>
+template <class C, class Epi, int kCount>
 __global__ void __launch_bounds__(C::kThreads, 1)
-gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ typename Epi::Params ep) {
+gemm16_kernel(const __grid_constant__ Launch16<Epi, kCount> launch) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* stages = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* outs = stages + C::kStages * C::kStageBytes;
@@ -323,10 +331,14 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = C::kCtas == 2 ? (int)cluster_rank() : 0;
   const int first = blockIdx.x / C::kCtas, step = gridDim.x / C::kCtas;
+  // the second product's tiles follow the first's
+  const int first1 = kCount > 1 ? (first + step - tiles16<C>(launch.g[0]) % step) % step : 0;
 
   if (threadIdx.x == 32) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&g.a) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&g.b) : "memory");
+    for (int pr = 0; pr < kCount; ++pr) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&launch.g[pr].a) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&launch.g[pr].b) : "memory");
+    }
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
@@ -343,7 +355,7 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
   }
-  if (g.clear) {
+  if (launch.g[0].clear || launch.g[kCount - 1].clear) {
     for (int i = threadIdx.x; i < C::kStages * C::kStageBytes / 16; i += C::kThreads) reinterpret_cast<uint4*>(stages)[i] = make_uint4(0, 0, 0, 0);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -355,73 +367,79 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
   pdl_wait();
 
   if (warp < kG16Epi) {
-  if constexpr (C::kPromote) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");    // 384 x 168 registers at launch = 128 x 56 + 256 x 224
-  bool ok = true;                       // the same in all lanes of a warp
-  if (warp == 0) {
-    uint32_t it = 0;
-    for (Tiles16<C> t(g, first, step); t.more() && ok; t.next()) {
-      const Tile16 w = t.get();
-      const int am = g.a_m0 + w.m0 + rank * 128, bn = g.b_n0 + w.n0 + rank * C::kBRows;
-      for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
-        const int st = it % C::kStages;
-        if (it >= (uint32_t)C::kStages && !(ok = mbar_wait_warp(&empty[st], ((it / C::kStages) - 1) & 1))) break;
-        const uint32_t bar = C::kCtas == 2 ? mapa_u32(smem_u32(&full[st]), 0) : smem_u32(&full[st]);
-        const uint32_t sa = smem_u32(stages) + st * C::kStageBytes, sb = sa + C::kPlanes * C::kABytes;
-        if (elect_one()) {
-          if (rank == 0) mbar_expect_tx(&full[st], (uint32_t)(C::kCtas * C::kPlanes * (g.a_bytes + g.b_bytes)));
+    if constexpr (C::kPromote) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");    // 384 x 168 registers at launch = 128 x 56 + 256 x 224
+    bool ok = true;                       // the same in all lanes of a warp
+    if (warp == 0) {
+      uint32_t it = 0;
+      for (int pr = 0; pr < kCount; ++pr) {
+        const Gemm16Args& g = launch.g[pr];
+        for (Tiles16<C> t(g, pr == 0 ? first : first1, step); t.more() && ok; t.next()) {
+          const Tile16 w = t.get();
+          const int am = g.a_m0 + w.m0 + rank * 128, bn = g.b_n0 + w.n0 + rank * C::kBRows;
+          for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
+            const int st = it % C::kStages;
+            if (it >= (uint32_t)C::kStages && !(ok = mbar_wait_warp(&empty[st], ((it / C::kStages) - 1) & 1))) break;
+            const uint32_t bar = C::kCtas == 2 ? mapa_u32(smem_u32(&full[st]), 0) : smem_u32(&full[st]);
+            const uint32_t sa = smem_u32(stages) + st * C::kStageBytes, sb = sa + C::kPlanes * C::kABytes;
+            if (elect_one()) {
+              if (rank == 0) mbar_expect_tx(&full[st], (uint32_t)(C::kCtas * C::kPlanes * (g.a_bytes + g.b_bytes)));
 #pragma unroll
-          for (int p = 0; p < C::kPlanes; ++p) {
-            load_operand<C::kCtas, 128>(sa + p * C::kABytes, &g.a, bar, g.a_k0 + kb * kG16K, am, w.z * g.a_z + p, g.a_mn);
-            load_operand<C::kCtas, C::kBRows>(sb + p * C::kBBytes, &g.b, bar, g.b_k0 + kb * kG16K, bn, w.z * g.b_z + p, g.b_mn);
-          }
-        }
-        __syncwarp();
-      }
-      ok = ok && __all_sync(0xffffffffu, *abort_flag == 0);
-    }
-    // the last releases must have landed here before this CTA's shared memory may go away
-    for (uint32_t u = it > (uint32_t)C::kStages ? it - C::kStages : 0; u < it && ok; ++u) ok = mbar_wait_warp(&empty[u % C::kStages], (u / C::kStages) & 1);
-    if (!ok) *abort_flag = 1;
-  } else if (warp == 1 && rank == 0) {
-    const uint32_t idesc = idesc16<C>(g);
-    // 16 elements of K: 32 bytes of a K-major row, 16 lines of 128 bytes MN-major
-    const uint64_t ka = g.a_mn ? 2048 >> 4 : 32 >> 4, kb_ = g.b_mn ? 2048 >> 4 : 32 >> 4;
-    const uint64_t base_a = operand_desc(smem_u32(stages), g.a_mn), base_b = operand_desc(smem_u32(stages) + C::kPlanes * C::kABytes, g.b_mn);
-    uint32_t it = 0, n = 0;
-    for (Tiles16<C> t(g, first, step); t.more() && ok; t.next()) {
-      const Tile16 w = t.get();
-      for (int kc = w.kb0; kc < w.kb1 && ok; kc += C::kChunk, ++n) {
-        const uint32_t acc = n % C::kBufs;
-        if (n >= C::kBufs && !(ok = mbar_wait_warp(&tempty[acc], (n / C::kBufs - 1) & 1))) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t d = tmem + acc * (uint32_t)C::kN;
-        const int ke = w.kb1 - kc < C::kChunk ? w.kb1 : kc + C::kChunk;
-        uint32_t accumulate = 0;
-        for (int kb = kc; kb < ke; ++kb, ++it) {
-          const int st = it % C::kStages;
-          if (!(ok = mbar_wait_warp(&full[st], (it / C::kStages) & 1))) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint64_t sa = base_a + (uint32_t)(st * (C::kStageBytes >> 4)), sb = base_b + (uint32_t)(st * (C::kStageBytes >> 4));
-          if (elect_one()) {
-#pragma unroll
-            for (int q = 0; q < (C::kPlanes == 2 ? 3 : 1); ++q) {      // hi·lo, lo·hi, hi·hi
-              const uint64_t da = sa + (q == 1 ? C::kABytes >> 4 : 0), db = sb + (C::kPlanes == 2 && q == 0 ? C::kBBytes >> 4 : 0);
-#pragma unroll
-              for (int k = 0; k < kG16K / 16; ++k)
-                if (k < g.k_steps) mma16<C::kCtas>(d, da + k * ka, db + k * kb_, idesc, q == 0 && k == 0 ? accumulate : 1u);
+              for (int p = 0; p < C::kPlanes; ++p) {
+                load_operand<C::kCtas, 128>(sa + p * C::kABytes, &g.a, bar, g.a_k0 + kb * kG16K, am, w.z * g.a_z + p, g.a_mn);
+                load_operand<C::kCtas, C::kBRows>(sb + p * C::kBBytes, &g.b, bar, g.b_k0 + kb * kG16K, bn, w.z * g.b_z + p, g.b_mn);
+              }
             }
-            commit16<C::kCtas>(&empty[st]);
+            __syncwarp();
           }
-          __syncwarp();
-          accumulate = 1;
+          ok = ok && __all_sync(0xffffffffu, *abort_flag == 0);
         }
-        if (ok && elect_one()) commit16<C::kCtas>(&tfull[acc]);
-        __syncwarp();
       }
-      ok = ok && __all_sync(0xffffffffu, *abort_flag == 0);
+      // the last releases must have landed here before this CTA's shared memory may go away
+      for (uint32_t u = it > (uint32_t)C::kStages ? it - C::kStages : 0; u < it && ok; ++u) ok = mbar_wait_warp(&empty[u % C::kStages], (u / C::kStages) & 1);
+      if (!ok) *abort_flag = 1;
+    } else if (warp == 1 && rank == 0) {
+      uint32_t it = 0, n = 0;
+      for (int pr = 0; pr < kCount; ++pr) {
+        const Gemm16Args& g = launch.g[pr];
+        const uint32_t idesc = idesc16<C>(g);
+        // 16 elements of K: 32 bytes of a K-major row, 16 lines of 128 bytes MN-major
+        const uint64_t ka = g.a_mn ? 2048 >> 4 : 32 >> 4, kb_ = g.b_mn ? 2048 >> 4 : 32 >> 4;
+        const uint64_t base_a = operand_desc(smem_u32(stages), g.a_mn), base_b = operand_desc(smem_u32(stages) + C::kPlanes * C::kABytes, g.b_mn);
+        for (Tiles16<C> t(g, pr == 0 ? first : first1, step); t.more() && ok; t.next()) {
+          const Tile16 w = t.get();
+          for (int kc = w.kb0; kc < w.kb1 && ok; kc += C::kChunk, ++n) {
+            const uint32_t acc = n % C::kBufs;
+            if (n >= C::kBufs && !(ok = mbar_wait_warp(&tempty[acc], (n / C::kBufs - 1) & 1))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t d = tmem + acc * (uint32_t)C::kN;
+            const int ke = w.kb1 - kc < C::kChunk ? w.kb1 : kc + C::kChunk;
+            uint32_t accumulate = 0;
+            for (int kb = kc; kb < ke; ++kb, ++it) {
+              const int st = it % C::kStages;
+              if (!(ok = mbar_wait_warp(&full[st], (it / C::kStages) & 1))) break;
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              const uint64_t sa = base_a + (uint32_t)(st * (C::kStageBytes >> 4)), sb = base_b + (uint32_t)(st * (C::kStageBytes >> 4));
+              if (elect_one()) {
+#pragma unroll
+                for (int q = 0; q < (C::kPlanes == 2 ? 3 : 1); ++q) {      // hi·lo, lo·hi, hi·hi
+                  const uint64_t da = sa + (q == 1 ? C::kABytes >> 4 : 0), db = sb + (C::kPlanes == 2 && q == 0 ? C::kBBytes >> 4 : 0);
+#pragma unroll
+                  for (int k = 0; k < kG16K / 16; ++k)
+                    if (k < g.k_steps) mma16<C::kCtas>(d, da + k * ka, db + k * kb_, idesc, q == 0 && k == 0 ? accumulate : 1u);
+                }
+                commit16<C::kCtas>(&empty[st]);
+              }
+              __syncwarp();
+              accumulate = 1;
+            }
+            if (ok && elect_one()) commit16<C::kCtas>(&tfull[acc]);
+            __syncwarp();
+          }
+          ok = ok && __all_sync(0xffffffffu, *abort_flag == 0);
+        }
+      }
+      if (!ok) *abort_flag = 1;
     }
-    if (!ok) *abort_flag = 1;
-  }
   } else {
     if constexpr (C::kPromote) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     constexpr int kPart = C::kPart;
@@ -453,35 +471,39 @@ gemm16_kernel(const __grid_constant__ Gemm16Args g, const __grid_constant__ type
       }
     };
     bool ok = true;
-    for (Tiles16<C> t(g, first, step); t.more() && ok; t.next()) {
-      const Tile16 w = t.get();
-      const int row = w.m0 + rank * 128 + q * 32, col = w.n0 + part * kPart;
-      Epi::template ahead<kPart>(ep, w, row, col, lane);
-      if constexpr (C::kPromote) {
-        float sum[kPart];
+    for (int pr = 0; pr < kCount; ++pr) {
+      const Gemm16Args& g = launch.g[pr];
+      const typename Epi::Params& ep = launch.ep[pr];
+      for (Tiles16<C> t(g, pr == 0 ? first : first1, step); t.more() && ok; t.next()) {
+        const Tile16 w = t.get();
+        const int row = w.m0 + rank * 128 + q * 32, col = w.n0 + part * kPart;
+        Epi::template ahead<kPart>(ep, w, row, col, lane);
+        if constexpr (C::kPromote) {
+          float sum[kPart];
 #pragma unroll
-        for (int j = 0; j < kPart; ++j) sum[j] = 0.f;
-        for (int kc = w.kb0; kc < w.kb1; kc += C::kChunk, ++n) {
+          for (int j = 0; j < kPart; ++j) sum[j] = 0.f;
+          for (int kc = w.kb0; kc < w.kb1; kc += C::kChunk, ++n) {
+            const uint32_t acc = n % C::kBufs;
+            if (!(ok = sums_ready(acc, (n / C::kBufs) & 1))) break;
+            uint32_t r[2][32];
+            tmem_load_32x32(lanes + acc * (uint32_t)C::kN, r[0]);
+#pragma unroll
+            for (int c = 0; c < kPart; c += 32) {      // the next load is on its way while these are added
+              tmem_load_wait();
+              if (c + 32 < kPart) tmem_load_32x32(lanes + acc * (uint32_t)C::kN + (uint32_t)c + 32u, r[(c / 32 + 1) & 1]);
+              else release(acc);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(r[(c / 32) & 1][j]);
+            }
+          }
+          if (!ok) break;
+          Epi::template run<C::kPlanes, kPart>(ep, g, w, row, col, part, stage, SumsInRegisters<kPart>{sum}, [] {});
+        } else {
           const uint32_t acc = n % C::kBufs;
           if (!(ok = sums_ready(acc, (n / C::kBufs) & 1))) break;
-uint32_t r[2][32];
-          tmem_load_32x32(lanes + acc * (uint32_t)C::kN, r[0]);
-#pragma unroll
-          for (int c = 0; c < kPart; c += 32) {      // the next load is on its way while these are added
-            tmem_load_wait();
-            if (c + 32 < kPart) tmem_load_32x32(lanes + acc * (uint32_t)C::kN + (uint32_t)c + 32u, r[(c / 32 + 1) & 1]);
-            else release(acc);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) sum[c + j] += __uint_as_float(r[(c / 32) & 1][j]);
-          }
+          ++n;
+          Epi::template run<C::kPlanes, kPart>(ep, g, w, row, col, part, stage, SumsInTmem<kPart>{lanes + acc * (uint32_t)C::kN}, [&] { release(acc); });
         }
-        if (!ok) break;
-        Epi::template run<C::kPlanes, kPart>(ep, g, w, row, col, part, stage, SumsInRegisters<kPart>{sum}, [] {});
-      } else {
-        const uint32_t acc = n % C::kBufs;
-        if (!(ok = sums_ready(acc, (n / C::kBufs) & 1))) break;
-        ++n;
-        Epi::template run<C::kPlanes, kPart>(ep, g, w, row, col, part, stage, SumsInTmem<kPart>{lanes + acc * (uint32_t)C::kN}, [&] { release(acc); });
       }
     }
     stage.drain();
@@ -490,7 +512,7 @@ uint32_t r[2][32];
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (*abort_flag) {
-    if (threadIdx.x == 0) set_status(g.status, kWaitTimeout, blockIdx.x, 400);
+    if (threadIdx.x == 0) set_status(launch.g[0].status, kWaitTimeout, blockIdx.x, 400);
     for (int i = 0; i < 200; ++i) __nanosleep(1000);
     __syncthreads();
   }
@@ -573,11 +595,9 @@ struct Chain {
   }
 };
 
-template <class C, class Epi>
-int launch16(Chain& chain, psb::Gemm16Args& g, const Operand16& a, const Operand16& b, const typename Epi::Params& ep) {
-  int dev = 0;
-  const int sms = sm_count(&dev);
-  if (sms <= 0) return (int)cudaErrorInvalidDevice;
+// what the device needs to know of a product's operands
+template <class C>
+int set_operands(psb::Gemm16Args& g, const Operand16& a, const Operand16& b) {
   // A copy that fills in rows from outside a matrix takes 2 to 3 cycles a row: one row of x in a box of 128 made scores of
   // 400,000 classes take 190 us instead of 134.  Boxes are no higher than the matrix.  Rows of K-major operands that no copy
   // brings may hold anything: their results are rows or columns that do not exist.  Lines of MN-major operands are
@@ -591,18 +611,32 @@ int launch16(Chain& chain, psb::Gemm16Args& g, const Operand16& a, const Operand
   g.b_bytes = rb * 128 * (g.b_mn ? C::kBRows / 64 : 1);
   g.k_steps = g.K >= psb::kG16K ? psb::kG16K / 16 : (g.K + 15) / 16;
   g.clear = (g.a_mn || g.b_mn) && lines < psb::kG16K;
+  return 0;
+}
+
+template <class C, class Epi, int kCount>
+int launch16(Chain& chain, psb::Launch16<Epi, kCount>& launch, const Operand16* a, const Operand16* b) {
+  int dev = 0;
+  const int sms = sm_count(&dev);
+  if (sms <= 0) return (int)cudaErrorInvalidDevice;
+  int tiles = 0;
+  for (int pr = 0; pr < kCount; ++pr) {
+    const int r = set_operands<C>(launch.g[pr], a[pr], b[pr]);
+    if (r) return r;
+    tiles += psb::tiles16<C>(launch.g[pr]);
+  }
   static bool attr[kMaxDevices] = {};
   if (!attr[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(psb::gemm16_kernel<C, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+    cudaError_t e = cudaFuncSetAttribute(psb::gemm16_kernel<C, Epi, kCount>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
     cudaFuncAttributes fa;
-    if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, psb::gemm16_kernel<C, Epi>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, psb::gemm16_kernel<C, Epi, kCount>);
     if (e != cudaSuccess) return (int)e;
     // the epilogue's warps wait for registers that the launch has to have brought
     if (C::kPromote && fa.numRegs * C::kThreads < 128 * 56 + 256 * 224) return (int)cudaErrorLaunchOutOfResources;
     attr[dev] = true;
   }
-  const int tiles = psb::tiles16<C>(g), most = sms / C::kCtas;
-  return chain.launch(psb::gemm16_kernel<C, Epi>, dim3((unsigned)((tiles < most ? tiles : most) * C::kCtas)), C::kThreads, C::kSmemBytes, C::kCtas, g, ep);
+  const int most = sms / C::kCtas;
+  return chain.launch(psb::gemm16_kernel<C, Epi, kCount>, dim3((unsigned)((tiles < most ? tiles : most) * C::kCtas)), C::kThreads, C::kSmemBytes, C::kCtas, launch);
 }
 
 // ---- which tiles, and in how many pieces K is taken
@@ -620,11 +654,13 @@ inline int tiling_parts(int kind) { return kind == kPair256Wide ? 4 : 2; }
 // The last round's epilogue comes on top; with two planes, whose sums are in its warps' registers, that of every round.  Pieces of
 // K cost a launch that adds them up and their bytes, 5000 a cycle.  A symmetric product may make all tiles: where one round
 // holds them, that saves the mirror images (512 x 512, two planes: 22 -> 14 k cycles).
-inline Tiling choose_tiling(int64_t batch, int64_t M, int64_t N, int64_t K, int planes, bool symmetric, int max_splits, int outputs = 1) {
+inline Tiling choose_tiling(int64_t batch, int64_t M, int64_t N, int64_t K, int planes, bool symmetric, int max_splits, int outputs = 1,
+                            int only = -1) {
   const int64_t nkb = (K + psb::kG16K - 1) / psb::kG16K;
   Tiling best = {kOne64, 1, (int)nkb, 0};
   double least = 1e300;
   for (int kind = 0; kind < kKinds; ++kind) {
+    if (only >= 0 && kind != only) continue;
     const int64_t rows = tiling_rows(kind), cols = tiling_cols(kind);
     const int64_t tm = (M + rows - 1) / rows, tn = (N + cols - 1) / cols, slots = rows == 256 ? 74 : 148;
     for (int sym = 0; sym <= (symmetric && rows == cols ? 1 : 0); ++sym) {
@@ -651,18 +687,26 @@ inline Tiling choose_tiling(int64_t batch, int64_t M, int64_t N, int64_t K, int 
 }
 
 template <int kPlanes, class Epi>
-int launch_tiled(Chain& chain, int kind, psb::Gemm16Args& g, const Operand16& a, const Operand16& b, const typename Epi::Params& ep) {
-  if (kind == kPair256) return launch16<psb::Cfg16<2, 256, kPlanes>, Epi>(chain, g, a, b, ep);
+int launch_tiled(Chain& chain, int kind, psb::Launch16<Epi, 1>& l, const Operand16& a, const Operand16& b) {
+  if (kind == kPair256) return launch16<psb::Cfg16<2, 256, kPlanes>, Epi, 1>(chain, l, &a, &b);
   if constexpr (kPlanes == 1) {
-    if (kind == kPair256Wide) return launch16<psb::Cfg16<2, 256, 1, 4>, Epi>(chain, g, a, b, ep);
+    if (kind == kPair256Wide) return launch16<psb::Cfg16<2, 256, 1, 4>, Epi, 1>(chain, l, &a, &b);
   }
-  if (kind == kPair128) return launch16<psb::Cfg16<2, 128, kPlanes>, Epi>(chain, g, a, b, ep);
-  if (kind == kOne128) return launch16<psb::Cfg16<1, 128, kPlanes>, Epi>(chain, g, a, b, ep);
-  return launch16<psb::Cfg16<1, 64, kPlanes>, Epi>(chain, g, a, b, ep);
+  if (kind == kPair128) return launch16<psb::Cfg16<2, 128, kPlanes>, Epi, 1>(chain, l, &a, &b);
+  if (kind == kOne128) return launch16<psb::Cfg16<1, 128, kPlanes>, Epi, 1>(chain, l, &a, &b);
+  return launch16<psb::Cfg16<1, 64, kPlanes>, Epi, 1>(chain, l, &a, &b);
 }
 template <class Epi>
-int product16(Chain& chain, int planes, int kind, psb::Gemm16Args& g, const Operand16& a, const Operand16& b, const typename Epi::Params& ep) {
-  return planes == 2 ? launch_tiled<2, Epi>(chain, kind, g, a, b, ep) : launch_tiled<1, Epi>(chain, kind, g, a, b, ep);
+int product16(Chain& chain, int planes, int kind, const psb::Gemm16Args& g, const Operand16& a, const Operand16& b, const typename Epi::Params& ep) {
+  psb::Launch16<Epi, 1> l = {{g}, {ep}};
+  return planes == 2 ? launch_tiled<2, Epi>(chain, kind, l, a, b) : launch_tiled<1, Epi>(chain, kind, l, a, b);
+}
+// two at once, in tiles of 128x128 or 128x64
+template <class Epi>
+int products16(Chain& chain, int planes, int kind, psb::Launch16<Epi, 2>& l, const Operand16* a, const Operand16* b) {
+  if (planes == 2)
+    return kind == kOne128 ? launch16<psb::Cfg16<1, 128, 2>, Epi, 2>(chain, l, a, b) : launch16<psb::Cfg16<1, 64, 2>, Epi, 2>(chain, l, a, b);
+  return kind == kOne128 ? launch16<psb::Cfg16<1, 128, 1>, Epi, 2>(chain, l, a, b) : launch16<psb::Cfg16<1, 64, 1>, Epi, 2>(chain, l, a, b);
 }
 
 }  // namespace

@@ -529,7 +529,7 @@ constexpr int kMaxBlocks = 148 * 8;           // of the pass that finds the larg
 
 // where things lie in the workspace; everything is 256-byte aligned
 struct LossPlan {
-  int planes, pack_x, pack_w, parts, per_tile, keep, piece;
+  int planes, pack_x, pack_w, parts, per_tile, keep, piece, together;
   Tiling score, gx, gw;                       // gx, gw: of the kept classes, or of a piece
   int64_t dp, ldg, x_plane, w_plane, g_plane;
   int64_t scales, maxima, lse, target, x, w, part, g, gx_acc, gw_acc, total;
@@ -581,6 +581,15 @@ LossPlan make_loss_plan(const LossKey& a) {
     const bool pieces = p.piece < a.V;
     p.gw = choose_tiling(1, p.piece, a.d, a.n, p.planes, false, pieces ? 1 : 16);
     p.gx = choose_tiling(1, a.n, a.d, p.piece, p.planes, false, pieces ? 1 : 64);
+    // both in one launch where their tiles, of one kind, are one round: a launch less, and a third of the SMs does not wait
+    if (a.want_gx && !pieces && (p.gw.kind == kOne128 || p.gw.kind == kOne64)) {
+      const Tiling t = choose_tiling(1, a.n, a.d, p.piece, p.planes, false, 64, 1, p.gw.kind);
+      auto tiles = [&](const Tiling& u, int64_t M) { return (M + 127) / 128 * ((a.d + tiling_cols(u.kind) - 1) / tiling_cols(u.kind)) * u.splits; };
+      if (tiles(p.gw, a.V) + tiles(t, a.n) <= 148) {
+        p.together = 1;
+        p.gx = t;
+      }
+    }
     if (a.want_gx && (p.gx.splits > 1 || pieces)) p.gx_acc = take((int64_t)p.gx.splits * a.n * a.d * 4);
     if (p.gw.splits > 1) p.gw_acc = take((int64_t)p.gw.splits * a.V * a.d * 4);
   }
@@ -608,21 +617,36 @@ bool loss_args_ok(const LossArgs& a) {
          a.keep_mb >= 0;
 }
 
-// out [M, N], contiguous, from a product, whole or split
-int gradient(Chain& chain, const LossPlan& p, const Tiling& t, Gemm16Args g, const Operand16& A, const Operand16& B, EpiGrad::Params e) {
-  g.splits = t.splits;
-  g.kb_split = t.splits > 1 ? t.kb_split : (g.K + kG16K - 1) / kG16K;
-  e.M = g.M; e.N = g.N;
-  if (t.splits > 1) { e.slot = (int64_t)g.M * g.N; e.write = 1; e.read = 0; }
-  e.by_map = !e.write && !e.read && e.dtype != kF32 && (g.N & 7) == 0 && (reinterpret_cast<uintptr_t>(e.out) & 15) == 0;
-  if (e.by_map) {
-    const int r = make_out_map(&e.map, Operand16{e.out, g.M, g.N, g.N, 0, 1}, e.dtype == kBF16);
-    if (r) return r;
-  }
-  int r = product16<EpiGrad>(chain, p.planes, t.kind, g, A, B, e);
-  if (r == 0 && t.splits > 1)
-    r = chain.launch(k_loss_sum, dim3(blocks_for(e.slot, 148 * 8)), 256, 0, 1, e.acc, t.splits, e.slot, e.slot, e.out, e.scale, e.dtype, e.with_w);
-  return r;
+// A gradient [M, N], contiguous, from a product, whole or split.
+struct Gradient {
+  Gemm16Args g;
+  Operand16 a, b;
+  EpiGrad::Params e;
+};
+int prepare(Gradient& q, const Tiling& t) {
+  q.g.splits = t.splits;
+  q.g.kb_split = t.splits > 1 ? t.kb_split : (q.g.K + kG16K - 1) / kG16K;
+  q.e.M = q.g.M; q.e.N = q.g.N;
+  if (t.splits > 1) { q.e.slot = (int64_t)q.g.M * q.g.N; q.e.write = 1; q.e.read = 0; }
+  q.e.by_map = !q.e.write && !q.e.read && q.e.dtype != kF32 && (q.g.N & 7) == 0 && (reinterpret_cast<uintptr_t>(q.e.out) & 15) == 0;
+  return q.e.by_map ? make_out_map(&q.e.map, Operand16{q.e.out, q.g.M, q.g.N, q.g.N, 0, 1}, q.e.dtype == kBF16) : 0;
+}
+int add_splits(Chain& chain, const Gradient& q) {
+  if (q.g.splits == 1) return 0;
+  const EpiGrad::Params& e = q.e;
+  return chain.launch(k_loss_sum, dim3(blocks_for(e.slot, 148 * 8)), 256, 0, 1, e.acc, q.g.splits, e.slot, e.slot, e.out, e.scale, e.dtype, e.with_w);
+}
+// One gradient, or two in one launch
+int gradient(Chain& chain, int planes, int kind, const Gradient& q) {
+  const int r = product16<EpiGrad>(chain, planes, kind, q.g, q.a, q.b, q.e);
+  return r ? r : add_splits(chain, q);
+}
+int gradients(Chain& chain, int planes, int kind, const Gradient (&q)[2]) {
+  Launch16<EpiGrad, 2> l = {{q[0].g, q[1].g}, {q[0].e, q[1].e}};
+  const Operand16 a[2] = {q[0].a, q[1].a}, b[2] = {q[0].b, q[1].b};
+  int r = products16<EpiGrad>(chain, planes, kind, l, a, b);
+  if (r == 0) r = add_splits(chain, q[0]);
+  return r ? r : add_splits(chain, q[1]);
 }
 
 }  // namespace
@@ -712,22 +736,24 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
     }
     EpiGrad::Params e = {};
     e.scale = scale; e.dtype = a.dtype;
+    Gradient q[2];
     // gw[v0.., :] = Gᵀ x
-    Gemm16Args gg = g;
-    gg.M = len; gg.N = a.d; gg.K = a.n; gg.a_mn = gg.b_mn = 1;
-    EpiGrad::Params ew = e;
-    ew.out = reinterpret_cast<uint8_t*>(a.gw) + (int64_t)v0 * a.d * es_out;
-    if (p.gw.splits > 1) ew.acc = reinterpret_cast<float*>(ws + p.gw_acc);
-    if ((r = gradient(chain, p, p.gw, gg, gop, xz, ew)) != 0) return r;
+    q[0] = Gradient{g, gop, xz, e};
+    q[0].g.M = len; q[0].g.N = a.d; q[0].g.K = a.n; q[0].g.a_mn = q[0].g.b_mn = 1;
+    q[0].e.out = reinterpret_cast<uint8_t*>(a.gw) + (int64_t)v0 * a.d * es_out;
+    if (p.gw.splits > 1) q[0].e.acc = reinterpret_cast<float*>(ws + p.gw_acc);
+    if ((r = prepare(q[0], p.gw)) != 0) return r;
+    if (!p.together && (r = gradient(chain, p.planes, p.gw.kind, q[0])) != 0) return r;
     if (a.gx == nullptr) continue;
     // gx += G w[v0.., :]
-    Gemm16Args gx = g;
-    gx.M = a.n; gx.N = a.d; gx.K = len; gx.b_k0 = v0; gx.b_mn = 1;
-    EpiGrad::Params ex = e;
-    ex.out = a.gx; ex.with_w = 1;
-    if (p.gx.splits > 1 || p.piece < a.V) ex.acc = reinterpret_cast<float*>(ws + p.gx_acc);
-    if (p.piece < a.V) { ex.read = v0 > 0; ex.write = v0 + len < a.V; }
-    if ((r = gradient(chain, p, p.gx, gx, gop, w, ex)) != 0) return r;
+    q[1] = Gradient{g, gop, w, e};
+    q[1].g.M = a.n; q[1].g.N = a.d; q[1].g.K = len; q[1].g.b_k0 = v0; q[1].g.b_mn = 1;
+    q[1].e.out = a.gx; q[1].e.with_w = 1;
+    if (p.gx.splits > 1 || p.piece < a.V) q[1].e.acc = reinterpret_cast<float*>(ws + p.gx_acc);
+    if (p.piece < a.V) { q[1].e.read = v0 > 0; q[1].e.write = v0 + len < a.V; }
+    if ((r = prepare(q[1], p.gx)) != 0) return r;
+    r = p.together ? gradients(chain, p.planes, p.gx.kind, q) : gradient(chain, p.planes, p.gx.kind, q[1]);
+    if (r) return r;
   }
   return 0;
 }
