@@ -150,30 +150,40 @@ struct EpiNs {
       const int rows = p.M - row0 < 32 ? p.M - row0 : 32, mine = col + st.lane;
       const bool in = mine < p.N;
       st.by_rows(v, [&](auto value) {
+        if (!in) return;
         if (p.slots != nullptr) {
           float* dst = p.slots + (((int64_t)w.split * p.batch + w.z) * p.M + row0) * p.N + mine;
-#pragma unroll
-          for (int r = 0; r < 32; ++r)
-            if (in && r < rows) dst[(int64_t)r * p.N] = value(r);
+#pragma unroll 8
+          for (int r = 0; r < rows; ++r, dst += p.N) *dst = value(r);
           return;
         }
         const int64_t at = ((int64_t)w.z * p.M + row0) * p.N + mine;
+        const float f = p.alpha * kNsInv;
+        if (!p.update) {
+          if (p.dtype == kOrthF32) {
+            float* dst = reinterpret_cast<float*>(p.result) + at;
+#pragma unroll 8
+            for (int r = 0; r < rows; ++r, dst += p.N) *dst = f * value(r);
+          } else if (p.dtype == kOrthBF16) {
+            __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.result) + at;
+#pragma unroll 8
+            for (int r = 0; r < rows; ++r, dst += p.N) *dst = __float2bfloat16_rn(f * value(r));
+          } else {
+            __half* dst = reinterpret_cast<__half*>(p.result) + at;
+#pragma unroll 8
+            for (int r = 0; r < rows; ++r, dst += p.N) *dst = __float2half_rn(f * value(r));
+          }
+          return;
+        }
+        float* wt = reinterpret_cast<float*>(p.result) + at;
 #pragma unroll 1
-        for (int r0 = 0; r0 < 32; r0 += 16) {
+        for (int r0 = 0; r0 < rows; r0 += 16) {
           float t[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            t[i] = p.update && in && r0 + i < rows ? reinterpret_cast<const float*>(p.result)[at + (int64_t)(r0 + i) * p.N] : 0.f;
+          for (int i = 0; i < 16; ++i) t[i] = r0 + i < rows ? wt[(int64_t)(r0 + i) * p.N] : 0.f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float x = p.alpha * kNsInv * value(r0 + i);
-            const int64_t to = at + (int64_t)(r0 + i) * p.N;
-            if (!in || r0 + i >= rows) continue;
-            if (p.update) reinterpret_cast<float*>(p.result)[to] = t[i] - p.lr * x;
-            else if (p.dtype == kOrthF32) reinterpret_cast<float*>(p.result)[to] = x;
-            else if (p.dtype == kOrthBF16) reinterpret_cast<__nv_bfloat16*>(p.result)[to] = __float2bfloat16_rn(x);
-            else reinterpret_cast<__half*>(p.result)[to] = __float2half_rn(x);
-          }
+          for (int i = 0; i < 16; ++i)
+            if (r0 + i < rows) wt[(int64_t)(r0 + i) * p.N] = t[i] - p.lr * (f * value(r0 + i));
         }
       });
     }

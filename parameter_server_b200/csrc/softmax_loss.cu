@@ -86,6 +86,16 @@ k_loss_coef(const float* __restrict__ coef, const int64_t* __restrict__ y, int n
 __device__ __forceinline__ uint32_t thread_absmax(const float* a, int64_t ld, int64_t rows, int cols, const int64_t* y, int V, int64_t first,
                                                   int64_t step) {
   uint32_t top = 0;
+  if (y == nullptr && ld == cols && (reinterpret_cast<uintptr_t>(a) & 15) == 0) {       // one long row, whatever its pieces' alignment
+    const int64_t n = rows * cols;
+#pragma unroll 4
+    for (int64_t i = first; i < n / 4; i += step) {
+      const float4 v = reinterpret_cast<const float4*>(a)[i];
+      top = max(max(top, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
+    }
+    for (int64_t i = n / 4 * 4 + first; i < n; i += step) top = max(top, finite_bits(a[i]));
+    return top;
+  }
   const bool vec = ((reinterpret_cast<uintptr_t>(a) & 15) | (ld & 3)) == 0;
   const int per = (cols + 3) / 4;
   const int64_t total = rows * per;
@@ -151,9 +161,28 @@ k_loss_pack(PackArgs px, PackArgs pw, int cols, const int64_t* __restrict__ y, i
     }
   }
   const T* a = reinterpret_cast<const T*>(p.a);
+  if (((reinterpret_cast<uintptr_t>(a) & 15) | ((p.ld * sizeof(T)) & 15)) != 0) {
+    // rows of any alignment: a warp a row, two columns a thread, so that loads and stores are pieces of one row
+    const int64_t warps = nb * 8;
+    for (int64_t r = b * 8 + (threadIdx.x >> 5); r < p.rows; r += warps) {
+      const T* src = a + r * p.ld;
+      uint16_t* dst = p.out + r * p.ldo;
+      const bool none = is_x && !has_class(y[r], V);
+#pragma unroll 4
+      for (int c = (threadIdx.x & 31) * 2; c < (int)p.ldo; c += 64) {
+        const T u = !none && c < cols ? src[c] : T(0), v = !none && c + 1 < cols ? src[c + 1] : T(0);
+        if constexpr (sizeof(T) == 4) {
+          *reinterpret_cast<uint32_t*>(dst + c) = pair16<kFmtPlanes>((float)u * s, (float)v * s, false);
+          *reinterpret_cast<uint32_t*>(dst + p.plane + c) = pair16<kFmtPlanes>((float)u * s, (float)v * s, true);
+        } else {
+          *reinterpret_cast<uint32_t*>(dst + c) = (uint32_t)*reinterpret_cast<const uint16_t*>(&u) | (uint32_t)*reinterpret_cast<const uint16_t*>(&v) << 16;
+        }
+      }
+    }
+    return;
+  }
   const int per = (int)(p.ldo / 8);
   const int64_t total = p.rows * per;
-  const bool vec = ((reinterpret_cast<uintptr_t>(a) & 15) | ((p.ld * sizeof(T)) & 15)) == 0;
   for (int64_t i = b * 256 + threadIdx.x; i < total; i += nb * 256) {
     const int64_t r = i / per;
     const int c = (int)(i - r * per) * 8;
@@ -162,7 +191,7 @@ k_loss_pack(PackArgs px, PackArgs pw, int cols, const int64_t* __restrict__ y, i
     if (is_x && !has_class(y[r], V)) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = T(0);
-    } else if (vec && c + 8 <= cols) {
+    } else if (c + 8 <= cols) {
 #pragma unroll
       for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(v)[j] = reinterpret_cast<const uint4*>(src)[j];
     } else {
@@ -174,10 +203,8 @@ k_loss_pack(PackArgs px, PackArgs pw, int cols, const int64_t* __restrict__ y, i
       uint32_t h[4], l[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        __half h0, l0, h1, l1;
-        split16((float)v[2 * j] * s, h0, l0);
-        split16((float)v[2 * j + 1] * s, h1, l1);
-        h[j] = pack_half2(h0, h1); l[j] = pack_half2(l0, l1);
+        h[j] = pair16<kFmtPlanes>((float)v[2 * j] * s, (float)v[2 * j + 1] * s, false);
+        l[j] = pair16<kFmtPlanes>((float)v[2 * j] * s, (float)v[2 * j + 1] * s, true);
       }
       *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
       *reinterpret_cast<uint4*>(dst + p.plane) = make_uint4(l[0], l[1], l[2], l[3]);
@@ -340,12 +367,21 @@ struct EpiGrad {
       const int64_t at = (int64_t)row0 * p.N + mine;
       float* acc = p.acc != nullptr ? p.acc + w.split * p.slot + at : nullptr;
       st.by_rows(v, [&](auto value) {
-        if (!p.read) {
-#pragma unroll
-          for (int r = 0; r < 32; ++r) {
-            if (!in || r >= rows) continue;
-            if (p.write) acc[(int64_t)r * p.N] = value(r);
-            else store_as(p.out, at + (int64_t)r * p.N, value(r) * scale, p.dtype);
+        if (!in) return;
+        if (!p.read) {                                       // by type and by pointer: an index for each row was half of this loop
+          if (p.write || p.dtype == kF32) {
+            float* dst = p.write ? acc : reinterpret_cast<float*>(p.out) + at;
+            const float f = p.write ? 1.f : scale;
+#pragma unroll 8
+            for (int r = 0; r < rows; ++r, dst += p.N) *dst = value(r) * f;
+          } else if (p.dtype == kBF16) {
+            __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + at;
+#pragma unroll 8
+            for (int r = 0; r < rows; ++r, dst += p.N) *dst = __float2bfloat16_rn(value(r) * scale);
+          } else {
+            __half* dst = reinterpret_cast<__half*>(p.out) + at;
+#pragma unroll 8
+            for (int r = 0; r < rows; ++r, dst += p.N) *dst = __float2half_rn(value(r) * scale);
           }
           return;
         }
