@@ -63,7 +63,6 @@ struct Gemm16Args {
   int bf16;                    // operands are bf16, else fp16
   int a_bytes, b_bytes;        // of a stage and plane that copies bring (launch16 sets them and k_steps)
   int k_steps;                 // steps of 16 elements in a block of K
-  int clear;                   // what copies leave out of the stages has to be zero
   uint32_t* status;
 };
 
@@ -178,7 +177,9 @@ __device__ __forceinline__ void commit16(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// Wait until the launches before this one are complete and their writes visible, then let the next one start its set-up.
+// Wait until the launches before this one are complete and their writes visible, then let the next one start its set-up.  What a
+// launch before wrote is read through pointers without __restrict__: the kernel may be running while it is written, so that it
+// is no read-only data, whose loads may be moved before the wait.
 __device__ __forceinline__ void pdl_wait() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -354,10 +355,6 @@ gemm16_kernel(const __grid_constant__ Launch16<Epi, kCount> launch) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base)), "r"(512u) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-  }
-  if (launch.g[0].clear || launch.g[kCount - 1].clear) {
-    for (int i = threadIdx.x; i < C::kStages * C::kStageBytes / 16; i += C::kThreads) reinterpret_cast<uint4*>(stages)[i] = make_uint4(0, 0, 0, 0);
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -601,16 +598,15 @@ int set_operands(psb::Gemm16Args& g, const Operand16& a, const Operand16& b) {
   // A copy that fills in rows from outside a matrix takes 2 to 3 cycles a row: one row of x in a box of 128 made scores of
   // 400,000 classes take 190 us instead of 134.  Boxes are no higher than the matrix.  Rows of K-major operands that no copy
   // brings may hold anything: their results are rows or columns that do not exist.  Lines of MN-major operands are
-  // elements of K and have to be zero; K is one block then, and the stages are cleared before the first.
-  auto up8 = [](int64_t v, int most) { return v >= most ? most : (int)((v + 7) / 8 * 8); };
-  const int lines = up8(g.K, psb::kG16K), ra = g.a_mn ? lines : up8(g.M, 128), rb = g.b_mn ? lines : up8(g.N, C::kBRows);
+  // elements of K: all of those that a step of 16 multiplies are brought, zeros behind the last.
+  auto up = [](int64_t v, int by, int most) { return v >= most ? most : (int)((v + by - 1) / by * by); };
+  const int lines = up(g.K, 16, psb::kG16K), ra = g.a_mn ? lines : up(g.M, 8, 128), rb = g.b_mn ? lines : up(g.N, 8, C::kBRows);
   int r = make_map16(&g.a, a.base, g.bf16, a.rows, a.cols, a.ld, a.stride, a.count, ra);
   if (r == 0) r = make_map16(&g.b, b.base, g.bf16, b.rows, b.cols, b.ld, b.stride, b.count, rb);
   if (r) return r;
   g.a_bytes = ra * 128 * (g.a_mn ? 2 : 1);
   g.b_bytes = rb * 128 * (g.b_mn ? C::kBRows / 64 : 1);
-  g.k_steps = g.K >= psb::kG16K ? psb::kG16K / 16 : (g.K + 15) / 16;
-  g.clear = (g.a_mn || g.b_mn) && lines < psb::kG16K;
+  g.k_steps = lines / 16;
   return 0;
 }
 

@@ -197,6 +197,25 @@ def test_nan_and_infinity_in_rows_with_a_class():
         assert bool(torch.isnan(gx[bad]).any(1).all()) and bool(torch.isfinite(gx[~bad]).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V,d", [(100, 3, 40), (200, 40, 24), (130, 50, 200), (300, 1000, 64)])
+def test_infinity_in_a_row_stays_in_its_row(n, V, d, dtype):
+    """Also where both gradients are one launch, whose products read the same shared memory in turn, and few classes
+    leave most of a block of it unused."""
+    from parameter_server_b200.ops import softmax
+
+    x, w, y = _data(n, V, d, dtype, seed=n)
+    x[0, 0] = 8.0                                  # the largest, so that fp32 operands have the same scale in both calls
+    bad = [9, 14, 40, n - 1]
+    x[bad] = 0.0
+    loss, gx, gw = softmax.softmax_loss(x, w, y)
+    x[bad] = float("inf")
+    loss2, gx2, _ = softmax.softmax_loss(x, w, y)
+    keep = torch.ones(n, dtype=torch.bool, device=x.device)
+    keep[bad] = False
+    assert torch.equal(loss2[keep], loss[keep]) and torch.equal(gx2[keep], gx[keep]) and not bool(gx2[bad].isfinite().any())
+
+
 def test_captured_replayed_and_on_another_stream():
     from parameter_server_b200.ops import softmax
 
