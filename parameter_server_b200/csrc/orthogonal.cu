@@ -73,8 +73,8 @@ k_orth_norm(const void* __restrict__ x, float* __restrict__ m, int64_t numel, in
 
 // U / (|U| + eps) into the planes
 __global__ void __launch_bounds__(256)
-k_orth_pack(const void* __restrict__ x, const float* __restrict__ m, int rows, int cols, int dtype, float mu, int nesterov,
-            const double* __restrict__ part, int nparts, float eps, uint16_t* __restrict__ out, int64_t ld, int64_t plane) {
+k_orth_pack(const void* __restrict__ x, const float* m, int rows, int cols, int dtype, float mu, int nesterov, const double* part,
+            int nparts, float eps, uint16_t* __restrict__ out, int64_t ld, int64_t plane) {
   __shared__ double sh[8];
   pdl_wait();
   const int64_t base = (int64_t)blockIdx.y * rows * cols;
@@ -194,7 +194,7 @@ struct EpiNs {
 // tiles (tile x tile) on and above the diagonal exist (tile 0: all do).  A block takes 32 x 32, a thread four neighbours, and stores them
 // and, through shared memory, their transpose.
 __global__ void __launch_bounds__(256)
-k_orth_sum(const float* __restrict__ slots, int splits, int batch, int n, int tile, uint16_t* __restrict__ out, uint16_t* __restrict__ out2,
+k_orth_sum(const float* slots, int splits, int batch, int n, int tile, uint16_t* __restrict__ out, uint16_t* __restrict__ out2,
            int64_t ld, int64_t plane, float alpha, float beta, float alpha2, float beta2) {
   __shared__ float sum[32][33];
   const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32, z = blockIdx.z;

@@ -137,7 +137,7 @@ struct PackArgs {
 template <typename T>
 __global__ void __launch_bounds__(256)
 k_loss_pack(PackArgs px, PackArgs pw, int cols, const int64_t* __restrict__ y, int n, int V, const float* __restrict__ coef, int bx,
-            const uint32_t* __restrict__ maxima, int mx, int mw, Scales* found) {
+            const uint32_t* maxima, int mx, int mw, Scales* found) {
   pdl_wait();
   const bool is_x = (int)blockIdx.x < bx;
   const PackArgs& p = is_x ? px : pw;
@@ -529,7 +529,7 @@ k_loss_rows(const __grid_constant__ JoinArgs p) {
 
 // the splits of K to the result
 __global__ void __launch_bounds__(256)
-k_loss_sum(const float* __restrict__ acc, int splits, int64_t slot, int64_t numel, void* out, ScaleRef scale_ref, int dtype, int with_w) {
+k_loss_sum(const float* acc, int splits, int64_t slot, int64_t numel, void* out, ScaleRef scale_ref, int dtype, int with_w) {
   pdl_wait();
   const float scale = grad_scale(scale_ref, with_w);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < numel; i += (int64_t)gridDim.x * 256) {
@@ -711,7 +711,7 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
   if (a.dtype == kF32 || (a.dtype == kF16 && a.coef != nullptr && a.want_grad)) scale.found = found;
   if (scale.found != nullptr && a.dtype == kF16) r = chain.launch(k_loss_coef, dim3(1), 256, 0, 1, a.coef, a.y, a.n, a.V, found);
   unsigned mx = 0, mw = 0;
-  const bool small = (int64_t)(a.n + a.V) * a.d <= 32768;      // 128 KB: 32 values a thread, less than a launch
+  const bool small = ((int64_t)a.n + a.V) * a.d <= 32768;      // 128 KB: 32 values a thread, less than a launch
   if (a.dtype == kF32 && !small) {
     mx = blocks_for((int64_t)a.n * ((a.d + 3) / 4), kMaxBlocks);
     mw = blocks_for((int64_t)a.V * ((a.d + 3) / 4), kMaxBlocks);

@@ -256,6 +256,8 @@ class SoftmaxLossLayer(Layer):
         self.classes = int(self.conf.size)
         if self.classes <= 0:
             raise ValueError("a softmax loss needs the number of classes (size)")
+        if self.classes > 1 << 24:
+            raise ValueError("a data layer keeps labels as float32: at most 2^24 classes")
 
     def forward(self) -> float:
         x, y = self.inputs[0].value, self.inputs[1].value

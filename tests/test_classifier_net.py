@@ -134,6 +134,8 @@ def test_rows_that_are_data_get_no_gradient(cpu_ops):
 def test_number_of_classes_is_asked_for():
     with pytest.raises(ValueError, match="classes"):
         nn.SGDSolver(_conf(classes=0), PeerGroup.single(torch.device("cpu")))
+    with pytest.raises(ValueError, match="classes"):                # labels are float32
+        nn.SGDSolver(_conf(classes=(1 << 24) + 1), PeerGroup.single(torch.device("cpu")))
 
 
 def _write_libsvm(path, X, y):
