@@ -17,6 +17,9 @@
 // directions over weak noise (ratio 10^2 and more) comes out 4 % off, which 16-bit results show.  bf16 results take one plane
 // in the last step only, which leaves 0.05 to 0.12 % (they are rounded to 0.17 % on average); fp32 and fp16 results take
 // two throughout (8e-6 for the same matrix, 3e-7 for a random one).
+//
+// 4096 x 4096, bf16: 3.2 ms for 1.37 TFLOP (symmetric products in halves), 3.57 with the products of planes, which take 2.1 ms
+// at the rate of a plain cuBLAS product.  Tiles come in whole rounds of 74 pairs, and a round ends with an epilogue of two planes.
 #include "gemm16.cuh"
 
 namespace psb {

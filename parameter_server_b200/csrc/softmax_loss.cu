@@ -10,9 +10,12 @@
 // For the gradients the epilogue also writes e^{s−m} · 2^15 in fp16 (relative to the part's own maximum, which is all that
 // is known then), for as many classes as the workspace holds; the second kernel turns it into G in place, with one
 // factor a part.  Making the scores once costs 6nVd operations instead of 8nVd, for a pass over 2 bytes an element
-// (8192 rows, 131,072 classes, 2048 wide: 3.5 ms less for 0.7).  Classes beyond the workspace come in pieces, whose scores
+// (8192 rows, 131,072 classes, 2048 wide: 3.2 ms less for 0.85).  Classes beyond the workspace come in pieces, whose scores
 // are made again.  gw of a piece is complete, gx is summed over the pieces in fp32.  Sums have a fixed order: results do not
 // vary from run to run.
+//
+// Bound by the tensor cores: bf16 scores of 4096 rows against 131,072 classes, 1024 wide, take 785 us, 0.83 of the rate of a plain
+// cuBLAS product; 8192 x 131,072 x 2048 with gradients takes 10.4 ms where the products alone, at its sustained rate, take 9.5.
 //
 // Scores, maxima, sums and losses are fp32 (in units of log2 e: 2^x is the hardware's exponential).  The exponentials keep 11
 // bits (two planes for fp32: 22); the label's entry of G, where they would cancel, is made from the label's score in fp32.
