@@ -558,6 +558,190 @@ struct LossArgs {
   uint32_t* status;
 };
 
+// ------------------------------------------------------------------ small calls
+// Rows and classes that fit into shared memory take one launch without a workspace, in fp32 on the CUDA cores: each of the four
+// launches of the general way costs 3 us of host time and 4 on the GPU, whatever its size.  One CTA, or a cluster of 8 in which each
+// holds all of x, w and the scores and makes a share of the scores, which it sends to the others, and of the gradients.
+//   calls behind one another with gradients, general way -> this one (on the GPU alone), us:
+//     16 x 100 x 64 fp32 25 -> 15 (15 -> 9.5), bf16 23 -> 15 (10 -> 9.5); 64 x 64 x 64 (2^18) 25 -> 18 (16 -> 14);
+//     1 x 500 x 64 25 -> 16.5 (19 -> 14.6); 128 x 128 x 64 (2^20) 25 -> 28 (19 -> 27), which is beyond the limit.
+//   One CTA instead of 8: 16 x 100 x 64 12.9 us on the GPU, 3 x 7 x 8 the same 5.2.
+// Bound by latency: loads from L2, two cluster barriers, chains of shared-memory reads.
+//
+// A thread makes four results next to one another, from four rows of one factor (read by all lanes alike) and a column of the
+// other; where there are fewer of those than threads, neighbouring lanes share a sum.  Rows of x and w are an odd number of
+// 16 bytes apart, free of bank conflicts.
+struct TinyArgs {
+  LossArgs a;
+  int ld, ldg, cl;             // floats from a row of x and w to the next, and of the scores; CTAs of the cluster
+};
+constexpr int kTinyThreads = 512, kTinySmem = 200 * 1024, kTinyCtas = 8;
+constexpr int kTinyRows = 512;                             // and classes
+constexpr int64_t kTinyWork = 1 << 18, kTinyAlone = 1 << 12;        // rows x classes x columns: of a call, of a single CTA
+
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
+
+// A CTA's share of `units` results of four: sum(unit, part, parts, v) adds a part of the terms, store(unit, v) takes the sums
+template <class Sum, class Store>
+__device__ __forceinline__ void four_at_once(int units, int terms, int rank, int cl, Sum sum, Store store) {
+  const int per = (units + cl - 1) / cl, first = rank * per, left = units - first, count = left < per ? left : per;
+  int shift = 0;
+  while (shift < 5 && per << (shift + 1) <= kTinyThreads && terms >> (shift + 1) >= 4) ++shift;
+  const int lane = threadIdx.x & 31;
+  for (int b = threadIdx.x; b - lane < count << shift; b += kTinyThreads) {
+    const int u = b >> shift, part = b & ((1 << shift) - 1);
+    float v[4] = {};
+    if (u < count) sum(first + u, part, 1 << shift, v);
+    for (int o = 1; o < 1 << shift; o <<= 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    if (u < count && part == 0) store(first + u, v);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kTinyThreads, 1)
+k_loss_tiny(const __grid_constant__ TinyArgs q) {
+  extern __shared__ __align__(16) float tiny_smem[];
+  const LossArgs& a = q.a;
+  const int n = a.n, V = a.V, d = a.d, ld = q.ld, ldg = q.ldg, n4 = (n + 3) / 4 * 4, v4 = (V + 3) / 4 * 4;
+  float *xs = tiny_smem, *wsm = xs + n4 * ld, *S = wsm + v4 * ld;
+  const int tid = threadIdx.x, lane = tid & 31, rank = q.cl > 1 ? (int)cluster_rank() : 0;
+
+  // fours of columns; zeros beside the matrices and in rows without a class
+  const int per_row = ld / 4, fours = (n4 + v4) * per_row;
+#pragma unroll 4
+  for (int i = tid; i < fours; i += kTinyThreads) {
+    const int r = i / per_row, c = (i - r * per_row) * 4, j = r - n4;
+    const bool in = r < n4 ? r < n && has_class(a.y[r < n ? r : 0], V) : j < V;
+    const T* src = r < n4 ? reinterpret_cast<const T*>(a.x) + (int64_t)r * a.ldx : reinterpret_cast<const T*>(a.w) + (int64_t)j * a.ldw;
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = in && c + k < d ? as_float(src[c + k]) : 0.f;
+    *reinterpret_cast<float4*>(xs + r * ld + c) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+  if (q.cl > 1) cluster_sync_all();                       // every CTA runs
+  else __syncthreads();
+
+  // scores in units of log2 e: four rows against a class
+  four_at_once(n4 / 4 * V, ld / 4, rank, q.cl,
+    [&](int u, int part, int parts, float (&v)[4]) {
+      const int i = u / V, j = u - i * V;
+      const float4 *wr = reinterpret_cast<const float4*>(wsm + j * ld), *xr = reinterpret_cast<const float4*>(xs + i * 4 * ld);
+      for (int k0 = part; k0 < per_row; k0 += 16 * parts) {
+        float t[4] = {};
+#pragma unroll 4
+        for (int k = k0; k < per_row && k < k0 + 16 * parts; k += parts) {
+          const float4 w = wr[k];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float4 x = xr[r * per_row + k];
+            t[r] = fmaf(x.x, w.x, fmaf(x.y, w.y, fmaf(x.z, w.z, fmaf(x.w, w.w, t[r]))));
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] += t[r];
+      }
+    },
+    [&](int u, const float (&v)[4]) {
+      const int i = u / V, j = u - i * V;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float* at = S + (i * 4 + r) * ldg + j;
+        const float s = __fmul_rn(v[r], kLog2e);
+        if (q.cl == 1) *at = s;
+        else
+          for (int c = 0; c < q.cl; ++c)
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_u32(smem_u32(at), (uint32_t)c)), "f"(s) : "memory");
+      }
+    });
+  if (q.cl > 1) cluster_sync_all();
+  else __syncthreads();
+
+  // losses, and the gradient of the scores in place: a few lanes a row
+  int shift = 0;
+  while (shift < 5 && 4 << shift < V) ++shift;
+  for (int b = tid; b - lane < n << shift; b += kTinyThreads) {
+    const int row = b >> shift, part = b & ((1 << shift) - 1), parts = 1 << shift;
+    const bool in = row < n;
+    float* s = S + (in ? row : 0) * ldg;
+    float top = -INFINITY, sum = 0.f;
+    if (in) for (int j = part; j < V; j += parts) top = fmaxf(top, s[j]);
+    for (int o = 1; o < parts; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float ref = top == -INFINITY ? 0.f : top;
+    if (in) for (int j = part; j < V; j += parts) sum += ex2(s[j] - ref);
+    for (int o = 1; o < parts; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (!in) continue;
+    const float l2 = log2f(sum);
+    const int64_t lab = a.y[row];
+    const bool ok = has_class(lab, V);
+    const float c = ok ? (a.coef != nullptr ? a.coef[row] : 1.f) : 0.f;
+    if (part == 0 && rank == 0) {
+      if (lab != -1 && !ok) set_status(a.status, kBadIndex, (uint32_t)row, (uint32_t)lab);
+      if (!ok) a.loss[row] = 0.f;
+    }
+    if (ok && (int)lab % parts == part && rank == 0) a.loss[row] = c * (kLn2 * ((top - s[lab]) + l2));
+    if (!a.want_grad) continue;
+    for (int j = part; j < ldg; j += parts) {
+      const float p = ok && j < V ? ex2((s[j] - top) - l2) : 0.f;
+      s[j] = ok && j < V ? c * (j == lab ? p - 1.f : p) : 0.f;
+    }
+  }
+  if (!a.want_grad) return;
+  __syncthreads();
+
+  if (a.gx != nullptr)
+    four_at_once(n4 / 4 * d, ldg / 4, rank, q.cl,           // four rows, a column
+      [&](int u, int part, int parts, float (&v)[4]) {
+        const int i = u / d, c = u - i * d, terms = ldg / 4;
+        const float4* g = reinterpret_cast<const float4*>(S + i * 4 * ldg);
+        for (int k0 = part; k0 < terms; k0 += 16 * parts) {
+          float t[4] = {};
+#pragma unroll 4
+          for (int k = k0; k < terms && k < k0 + 16 * parts; k += parts) {
+            const float* w = wsm + k * 4 * ld + c;
+            const float w0 = w[0], w1 = w[ld], w2 = w[2 * ld], w3 = w[3 * ld];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float4 x = g[r * terms + k];
+              t[r] = fmaf(x.x, w0, fmaf(x.y, w1, fmaf(x.z, w2, fmaf(x.w, w3, t[r]))));
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] += t[r];
+        }
+      },
+      [&](int u, const float (&v)[4]) {
+        const int i = u / d, c = u - i * d;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (i * 4 + r < n) store_as(a.gx, (int64_t)(i * 4 + r) * d + c, v[r], a.dtype);
+      });
+  four_at_once(v4 / 4 * d, n, rank, q.cl,                   // four classes, a column
+    [&](int u, int part, int parts, float (&v)[4]) {
+      const int j = u / d, c = u - j * d;
+      for (int k0 = part; k0 < n; k0 += 64 * parts) {
+        float t[4] = {};
+#pragma unroll 4
+        for (int k = k0; k < n && k < k0 + 64 * parts; k += parts) {
+          const float4 g = *reinterpret_cast<const float4*>(S + k * ldg + j * 4);
+          const float x = xs[k * ld + c];
+          t[0] = fmaf(g.x, x, t[0]); t[1] = fmaf(g.y, x, t[1]); t[2] = fmaf(g.z, x, t[2]); t[3] = fmaf(g.w, x, t[3]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] += t[r];
+      }
+    },
+    [&](int u, const float (&v)[4]) {
+      const int j = u / d, c = u - j * d;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (j * 4 + r < V) store_as(a.gw, (int64_t)(j * 4 + r) * d + c, v[r], a.dtype);
+    });
+}
+
 }  // namespace psb
 
 using namespace psb;
@@ -569,6 +753,7 @@ constexpr int kMaxBlocks = 148 * 8;           // of the pass that finds the larg
 // where things lie in the workspace; everything is 256-byte aligned
 struct LossPlan {
   int planes, pack_x, pack_w, parts, per_tile, keep, piece, together;
+  int tiny, tiny_ld, tiny_ldg, tiny_smem;     // CTAs of k_loss_tiny, 0: the general way
   Tiling score, gx, gw;                       // gx, gw: of the kept classes, or of a piece
   int64_t dp, ldg, x_plane, w_plane, g_plane;
   int64_t scales, maxima, lse, target, x, w, part, g, gx_acc, gw_acc, total;
@@ -589,8 +774,22 @@ LossKey loss_key(const LossArgs& a) {
   return LossKey{a.n, a.V, a.d, a.dtype, a.want_grad, a.gx != nullptr, a.keep_mb, !direct(a.x, a.ldx), !direct(a.w, a.ldw)};
 }
 
+// One launch where rows, classes and scores fit into shared memory and the multiplications do not take the CUDA cores longer than
+// the general way takes for its launches.
+bool tiny_plan(LossPlan& p, const LossKey& a) {
+  const int64_t work = (int64_t)a.n * a.V * (a.d < kTinyWork ? a.d : kTinyWork);
+  if (a.n > kTinyRows || a.V > kTinyRows || work > kTinyWork) return false;
+  const int64_t ld = ((int64_t)a.d + 3) / 4 | 1, n4 = ((int64_t)a.n + 3) / 4, v4 = ((int64_t)a.V + 3) / 4;       // in fours
+  const int64_t bytes = ((n4 + v4) * 4 * ld + n4 * 4 * v4) * 16;
+  if (bytes > kTinySmem) return false;
+  p.tiny = work <= kTinyAlone ? 1 : kTinyCtas;
+  p.tiny_ld = (int)ld * 4; p.tiny_ldg = (int)v4 * 4; p.tiny_smem = (int)bytes;
+  return true;
+}
+
 LossPlan make_loss_plan(const LossKey& a) {
   LossPlan p = {};
+  if (tiny_plan(p, a)) return p;
   p.planes = a.dtype == kF32 ? 2 : 1;
   p.dp = ((int64_t)a.d + 7) / 8 * 8;
   p.pack_x = a.pack_x;
@@ -656,6 +855,20 @@ bool loss_args_ok(const LossArgs& a) {
          a.keep_mb >= 0;
 }
 
+template <typename T>
+int tiny_launch(cudaStream_t stream, const LossPlan& p, const TinyArgs& q) {
+  int dev = 0;
+  if (sm_count(&dev) <= 0) return (int)cudaErrorInvalidDevice;
+  static bool attr[kMaxDevices] = {};
+  if (!attr[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(k_loss_tiny<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTinySmem);
+    if (e != cudaSuccess) return (int)e;
+    attr[dev] = true;
+  }
+  Chain chain{stream};
+  return chain.launch(k_loss_tiny<T>, dim3((unsigned)p.tiny), kTinyThreads, (size_t)p.tiny_smem, p.tiny, q);
+}
+
 // A gradient [M, N], contiguous, from a product, whole or split.
 struct Gradient {
   Gemm16Args g;
@@ -700,6 +913,10 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
   const LossArgs& a = *ap;
   if (!loss_args_ok(a)) return (int)cudaErrorInvalidValue;
   const LossPlan p = loss_plan(a);
+  if (p.tiny) {
+    const TinyArgs q{a, p.tiny_ld, p.tiny_ldg, p.tiny};
+    return a.dtype == kF32 ? tiny_launch<float>(s, p, q) : a.dtype == kBF16 ? tiny_launch<__nv_bfloat16>(s, p, q) : tiny_launch<__half>(s, p, q);
+  }
   if (p.total > a.ws_bytes || (reinterpret_cast<uintptr_t>(a.ws) & 255)) return (int)cudaErrorInvalidValue;
   uint8_t* ws = reinterpret_cast<uint8_t*>(a.ws);
   Scales* found = reinterpret_cast<Scales*>(ws + p.scales);

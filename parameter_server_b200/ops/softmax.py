@@ -32,7 +32,7 @@ def softmax_loss(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, coef: Option
     no part in the gradients.  Another label counts as -1 and is reported by :func:`dense.check_status`.  ``coef``: fp32 [n]
     (None: ones).  Rows of x and w are contiguous, their strides are free.  fp32 operands are multiplied with 22 bits
     (three fp16 products) relative to the largest of x, of w and of coef: what is below 2^-17 of it keeps fewer.  16-bit
-    operands are multiplied as they are; sums are fp32.  The gradients need a workspace of 2 bytes (fp32: 4) for each row and
+    operands are multiplied as they are; sums are fp32.  A small call is one launch, in fp32 throughout.  The gradients need a workspace of 2 bytes (fp32: 4) for each row and
     class, at most 2 GB (or 256 classes): beyond it the classes come in pieces, whose scores are made twice, and n·d floats."""
     gpu = x.get_device()
     for name, t in (("x", x), ("w", w), ("y", y), ("coef", coef)):
@@ -76,8 +76,8 @@ def softmax_loss(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, coef: Option
         if len(_sizes) >= 1024:
             _sizes.clear()
         _sizes[key] = size
-    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None      # small calls need none
     args = _ARGS.pack(px, pw, y.data_ptr(), 0 if coef is None else coef.data_ptr(), loss.data_ptr(), pgx, pgw, ldx, ldw, n, classes, d,
-                      dtype, want, KEEP_MB, ws.data_ptr(), size, dense.status_ptr(dev))
+                      dtype, want, KEEP_MB, 0 if ws is None else ws.data_ptr(), size, dense.status_ptr(dev))
     N.check(lib.psb_softmax_loss(args, N.raw_stream(gpu)), "softmax_loss")
     return loss, gx, gw

@@ -200,8 +200,7 @@ def test_nan_and_infinity_in_rows_with_a_class():
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,V,d", [(100, 3, 40), (200, 40, 24), (130, 50, 200), (300, 1000, 64)])
 def test_infinity_in_a_row_stays_in_its_row(n, V, d, dtype):
-    """Also where both gradients are one launch, whose products read the same shared memory in turn, and few classes
-    leave most of a block of it unused."""
+    """Also where few classes leave most of a block of terms unused."""
     from parameter_server_b200.ops import softmax
 
     x, w, y = _data(n, V, d, dtype, seed=n)
@@ -293,6 +292,36 @@ def test_no_rows():
     w = torch.randn(5, 8, device="cuda")
     loss, gx, gw = softmax.softmax_loss(torch.empty(0, 8, device="cuda"), w, torch.empty(0, dtype=torch.int64, device="cuda"))
     assert loss.shape == (0,) and gx.shape == (0, 8) and not gw.any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V,d", [(512, 8, 64), (513, 8, 60), (8, 512, 64), (9, 513, 50), (64, 64, 64), (64, 64, 65), (1, 1, 5000), (4, 4, 2048),
+                                   (2, 2, 13_000), (100, 100, 26), (200, 210, 6), (16, 16, 16), (17, 16, 16), (1, 512, 512), (5, 3, 1)])
+def test_small_calls_and_the_first_that_are_not(n, V, d, dtype):
+    """Sizes on both sides of the limits of the single launch, of its single CTA and of shared memory; rows without a class that
+    hold anything, coefficients, strides and odd addresses.  Its sums take a rounding for each of 64 terms and then one for each
+    64: for terms of either sign they are independent and relative to sums that are a root of the terms, about 2^-24 of the
+    terms' magnitudes, below a cut of the tensor cores."""
+    from parameter_server_b200.ops import dense, softmax
+
+    x, w, y = _data(n, V, d, dtype, seed=1)
+    c = torch.rand(n, device="cuda") * 3 - 1
+    first = _check(x, w, y, c)
+    xs, ws = torch.zeros(n, d + 5, dtype=dtype, device="cuda"), torch.zeros(V, d + 2, dtype=dtype, device="cuda")
+    xs[:, 3:3 + d], ws[:, 1:1 + d] = x, w
+    second = softmax.softmax_loss(xs[:, 3:3 + d], ws[:, 1:1 + d], y, c)
+    for a, b in zip(first, second):
+        assert torch.equal(a, b)
+    y2, x2, c2 = y.clone(), x.clone(), c.clone()
+    y2[::2] = -1
+    x2[::2], c2[::2] = float("nan"), float("inf")
+    loss, gx, _ = _check(x2, w, y2, c2) if n > 1 else softmax.softmax_loss(x2, w, y2, c2)
+    assert not bool(loss[::2].any()) and not bool(gx[::2].any())
+    y2[0] = V
+    loss, gx, _ = softmax.softmax_loss(x2, w, y2, c2)
+    with pytest.raises(RuntimeError):
+        dense.check_status(x.device)
+    assert loss[0].item() == 0 and not bool(gx[0].any())
 
 
 def test_classes_in_several_pieces(monkeypatch):
