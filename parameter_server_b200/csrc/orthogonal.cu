@@ -119,6 +119,17 @@ k_orth_norm(const void* __restrict__ x, float* __restrict__ m, int64_t numel, in
   }
 }
 
+__device__ __forceinline__ void planes8(const float* v, uint4& h, uint4& l) {
+  uint32_t hs[4], ls[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    hs[i] = pair16<kFmtPlanes>(v[2 * i], v[2 * i + 1], false);
+    ls[i] = pair16<kFmtPlanes>(v[2 * i], v[2 * i + 1], true);
+  }
+  h = make_uint4(hs[0], hs[1], hs[2], hs[3]);
+  l = make_uint4(ls[0], ls[1], ls[2], ls[3]);
+}
+
 // U / (|U| + eps) into the planes
 __global__ void __launch_bounds__(256)
 k_orth_pack(const void* __restrict__ x, const float* m, int rows, int cols, int dtype, float mu, int nesterov, const double* part,
@@ -135,6 +146,36 @@ k_orth_pack(const void* __restrict__ x, const float* m, int rows, int cols, int 
   for (int i = 0; i < 8; ++i) t += sh[i];
   const double f = (double)kNsScale / (sqrt(t) + (double)eps);
   uint16_t* dst = out + (int64_t)blockIdx.y * 2 * plane;
+  // rows without padding are one long row: eights of it, two at a time
+  if (ld == cols && ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(x)) & 15) == 0) {
+    const int64_t eights = (int64_t)rows * cols / 8, step = (int64_t)gridDim.x * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < eights; i += 2 * step) {
+      float4 u[2][2], v[2][2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (i + k * step >= eights) break;
+        const int64_t at = base + (i + k * step) * 8;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          u[k][h] = load4_as(x, at + 4 * h, dtype);
+          if (m != nullptr) v[k][h] = *reinterpret_cast<const float4*>(m + at + 4 * h);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (i + k * step >= eights) break;
+        float e[8] = {u[k][0].x, u[k][0].y, u[k][0].z, u[k][0].w, u[k][1].x, u[k][1].y, u[k][1].z, u[k][1].w};
+        const float t[8] = {v[k][0].x, v[k][0].y, v[k][0].z, v[k][0].w, v[k][1].x, v[k][1].y, v[k][1].z, v[k][1].w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = (float)((double)(m != nullptr ? update_direction(e[j], t[j], mu, nesterov) : e[j]) * f);
+        uint4 h, l;
+        planes8(e, h, l);
+        *reinterpret_cast<uint4*>(dst + (i + k * step) * 8) = h;
+        *reinterpret_cast<uint4*>(dst + plane + (i + k * step) * 8) = l;
+      }
+    }
+    return;
+  }
   const int per = (int)(ld / 2);
   const int64_t total = (int64_t)rows * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
@@ -324,16 +365,6 @@ __device__ __forceinline__ float4 ld_own_v4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cta.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
-}
-__device__ __forceinline__ void planes8(const float* v, uint4& h, uint4& l) {
-  uint32_t hs[4], ls[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    hs[i] = pair16<kFmtPlanes>(v[2 * i], v[2 * i + 1], false);
-    ls[i] = pair16<kFmtPlanes>(v[2 * i], v[2 * i + 1], true);
-  }
-  h = make_uint4(hs[0], hs[1], hs[2], hs[3]);
-  l = make_uint4(ls[0], ls[1], ls[2], ls[3]);
 }
 // Byte offset of eight columns (the c8-th eight) of a row in an operand of `rows` rows: blocks of 64 columns, the hi and then
 // the lo plane of each.
