@@ -183,6 +183,30 @@ def test_update(shape, gtype, nesterov):
         assert (w1.double() - want).norm().item() <= tol.item()
 
 
+@pytest.mark.parametrize("shape", [(2, 264, 520), (130, 136), (203, 301), (300, 8000), (64, 64), (96, 700), (5, 72)])
+@pytest.mark.parametrize("gtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("offsets", [(0, 0, 0), (1, 2, 3), (0, 4, 0), (4, 0, 1), (2, 8, 4)])
+def test_update_and_matrix_at_any_address(shape, gtype, offsets):
+    """Tensors that start inside others, so that wide loads apply to all, some or none: the same result but for the order of the
+    norm's fp64 sum, a last bit of its quotient in fp32 (2^-24), which five steps multiply by at most 4.3 each."""
+    from parameter_server_b200.ops import orthogonal
+
+    numel = torch.Size(shape).numel()
+    data = [torch.randn(*shape, device="cuda"), (_data(shape, 8) * 1e-2).to(gtype), _data(shape, 9) * 1e-2]
+    bound = 4.3 ** 5 * 2.0 ** -23 + (2 * HALF_STEP[gtype] * numel ** 0.5 if gtype != torch.float32 else 0)
+    results = []
+    for at in ((0, 0, 0), offsets):
+        w, g, m = (torch.zeros(numel + 16, dtype=t.dtype, device="cuda")[o: o + numel].view(shape).copy_(t) for t, o in zip(data, at))
+        orthogonal.orthogonal_update(w, g, m, 0.5, momentum=0.9)
+        results.append((w, m, orthogonal.orthogonalize(g)))
+    (w0, m0, x0), (w1, m1, x1) = results
+    assert torch.equal(m0, m1)
+    step = 0.5 * max(1.0, shape[-2] / shape[-1]) ** 0.5
+    batch = shape[0] if len(shape) == 3 else 1
+    assert (w1.double() - w0.double()).norm().item() <= step * 4.3 ** 5 * 2.0 ** -23 * batch + 2.0 ** -23 * w0.double().norm().item()
+    assert (x1.double() - x0.double()).norm().item() <= bound * batch
+
+
 def test_update_captured_and_on_another_stream():
     from parameter_server_b200.ops import orthogonal
 

@@ -324,6 +324,45 @@ def test_small_calls_and_the_first_that_are_not(n, V, d, dtype):
     assert loss[0].item() == 0 and not bool(gx[0].any())
 
 
+@pytest.mark.parametrize("n,V,d", [(3, 7, 8), (60, 50, 64)])
+def test_small_calls_captured_and_in_two_threads(n, V, d):
+    """One CTA and a cluster: replayed from two graphs, and called from two threads on streams of their own."""
+    import threading
+
+    from parameter_server_b200.ops import softmax
+
+    x, w, y = _data(n, V, d, torch.bfloat16, 3)
+    want = softmax.softmax_loss(x, w, y)
+    only, _, only_w = softmax.softmax_loss(x, w, y, want_gx=False)
+    assert torch.equal(only, want[0]) and torch.equal(only_w, want[2])
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = [softmax.softmax_loss(x, w, y) for _ in range(3)]
+        graphs.append((graph, out))
+    for graph, _ in graphs * 2:
+        graph.replay()
+    torch.cuda.synchronize()
+    got = [r for _, out in graphs for r in out]
+
+    def work():
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            mine = [softmax.softmax_loss(x, w, y) for _ in range(50)]
+        stream.synchronize()
+        got.extend(mine)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 106
+    for r in got:
+        assert all(torch.equal(a, b) for a, b in zip(r, want))
+
+
 def test_classes_in_several_pieces(monkeypatch):
     """More rows × classes than are kept for the gradients: 256 MB of fp16 planes are 22,000 classes of 3,050 rows."""
     from parameter_server_b200.ops import dense, softmax
