@@ -563,7 +563,7 @@ struct LossArgs {
 // launches of the general way costs 3 us of host time and 4 on the GPU, whatever its size.  One CTA, or a cluster of 8 in which each
 // holds all of x, w and the scores and makes a share of the scores, which it sends to the others, and of the gradients.
 //   calls behind one another with gradients, general way -> this one (on the GPU alone), us:
-//     16 x 100 x 64 fp32 25 -> 15 (15 -> 9.5), bf16 23 -> 15 (10 -> 9.5); 64 x 64 x 64 (2^18) 25 -> 18 (16 -> 14);
+//     16 x 100 x 64 fp32 25 -> 16 (15 -> 9.5), bf16 23 -> 16 (10 -> 9.5); 64 x 64 x 64 (2^18) 25 -> 18 (16 -> 14);
 //     1 x 500 x 64 25 -> 16.5 (19 -> 14.6); 128 x 128 x 64 (2^20) 25 -> 28 (19 -> 27), which is beyond the limit.
 //   One CTA instead of 8: 16 x 100 x 64 12.9 us on the GPU, 3 x 7 x 8 the same 5.2.
 // Bound by latency: loads from L2, two cluster barriers, chains of shared-memory reads.
