@@ -276,9 +276,11 @@ struct OutStage {
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   // Results of any stride and alignment: f(r, v) for r = 0..31 with v = row r's value of column `lane`, so that a warp's
-  // accesses are pieces of one row.  The exclusive or keeps both directions free of bank conflicts.
+  // accesses are pieces of one row.  The exclusive or keeps both directions free of bank conflicts.  Boxes of the tile before, which
+  // may be another product's of the launch and go by store(), have been read before they are overwritten.
   template <class F>
   __device__ __forceinline__ void by_rows(const float (&v)[32], F f) {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 32; ++j) f32(lane, j) = v[j];
