@@ -296,6 +296,7 @@ struct SumsInTmem {
   uint32_t taddr;
   __device__ __forceinline__ void load(int c, float (&v)[32]) const {
     uint32_t r[32];
+    __syncwarp();                        // lanes may have gone apart over the columns before; the load is the whole warp's
     tmem_load_32x32(taddr + (uint32_t)c, r);
     tmem_load_wait();
 #pragma unroll
@@ -485,6 +486,7 @@ gemm16_kernel(const __grid_constant__ Launch16<Epi, kCount> launch) {
             const uint32_t acc = n % C::kBufs;
             if (!(ok = sums_ready(acc, (n / C::kBufs) & 1))) break;
             uint32_t r[2][32];
+            __syncwarp();
             tmem_load_32x32(lanes + acc * (uint32_t)C::kN, r[0]);
 #pragma unroll
             for (int c = 0; c < kPart; c += 32) {      // the next load is on its way while these are added

@@ -497,6 +497,7 @@ k_orth_small(const __grid_constant__ SmallArgs p) {
   const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
   auto add16 = [&](float (&v)[16], uint32_t column) {
     uint32_t r[16];
+    __syncwarp();                                          // half of the lanes may have left the turn before
     tmem_load_32x16(lanes + column, r);
     tmem_load_wait();
 #pragma unroll

@@ -233,3 +233,9 @@ def test_update_captured_and_on_another_stream():
     torch.cuda.synchronize()
     for a, b, c in ((w, w2, w3), (m, m2, m3)):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("shape", [(48, 48), (80, 80), (112, 100), (40, 1000), (700, 75), (110, 1500), (4, 80, 300)])
+def test_short_sides_that_end_inside_a_warp(shape):
+    """Rounded up to 16 they are 48, 80 or 112: of the warp that holds the last 16 rows, half has none."""
+    _check(_data(shape, 10))
