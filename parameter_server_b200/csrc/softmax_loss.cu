@@ -50,7 +50,13 @@ __device__ __forceinline__ float pow2i(int e) {       // 2^e, kept finite; 0 bel
   return e < -126 ? 0.f : __int_as_float((e + 127) << 23);
 }
 __device__ __forceinline__ float score_scale(const ScaleRef& r) { const Scales k = r.get(); return kLog2e * pow2i(-(k.x + k.w)); }
-__device__ __forceinline__ float grad_scale(const ScaleRef& r, int with_w) { const Scales k = r.get(); return pow2i(-(k.g + (with_w ? k.w : k.x))); }
+// 2^e in two factors of the same direction: the power may lie outside fp32 where what it scales does not leave it
+struct Pow2 {
+  float a, b;
+  __device__ __forceinline__ explicit Pow2(int e) : a(pow2i(e / 2)), b(pow2i(e - e / 2)) {}
+  __device__ __forceinline__ float operator*(float v) const { return v * a * b; }
+};
+__device__ __forceinline__ Pow2 grad_scale(const ScaleRef& r, int with_w) { const Scales k = r.get(); return Pow2(-(k.g + (with_w ? k.w : k.x))); }
 __device__ __forceinline__ bool has_class(int64_t y, int V) { return y >= 0 && y < V; }
 
 // ------------------------------------------------------------------ preparation
@@ -332,7 +338,7 @@ __device__ __forceinline__ void store_as(void* out, int64_t at, float v, int dty
   else reinterpret_cast<__half*>(out)[at] = __float2half_rn(v);
 }
 
-// A gradient: to the result, or raw fp32 sums to `acc` (piece by piece, or one slot per split of K)
+// A gradient: to the result, or as fp32 sums to `acc` (piece by piece, or one slot per split of K)
 struct EpiGrad {
   struct Params {
     CUtensorMap map;           // of the result, where it is 16-bit and aligned
@@ -350,7 +356,7 @@ struct EpiGrad {
   template <int kPlanes, int kPart, class Stage, class Sums, class Done>
   static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int, Stage& st,
                                              const Sums& sums, Done done) {
-    const float scale = grad_scale(p.scale, p.with_w);
+    const Pow2 scale = grad_scale(p.scale, p.with_w);
 #pragma unroll 1
     for (int k = 0; k < kPart; k += 32) {
       float v[32];
@@ -358,9 +364,9 @@ struct EpiGrad {
       if (k + 32 >= kPart) done();
       const int col = col0 + k;
       if (row0 >= p.M || col >= p.N) continue;
-      if (kPlanes == 1 && p.by_map) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] *= scale;
+      for (int j = 0; j < 32; ++j) v[j] = scale * v[j];
+      if (kPlanes == 1 && p.by_map) {
         if (p.dtype == kBF16) st.template store<kFmtBF16>(&p.map, v, row0, col, 0, false);
         else st.template store<kFmtF16>(&p.map, v, row0, col, 0, false);
         continue;
@@ -374,17 +380,16 @@ struct EpiGrad {
         if (!p.read) {                                       // by type and by pointer: an index for each row was half of this loop
           if (p.write || p.dtype == kF32) {
             float* dst = p.write ? acc : reinterpret_cast<float*>(p.out) + at;
-            const float f = p.write ? 1.f : scale;
 #pragma unroll 8
-            for (int r = 0; r < rows; ++r, dst += p.N) *dst = value(r) * f;
+            for (int r = 0; r < rows; ++r, dst += p.N) *dst = value(r);
           } else if (p.dtype == kBF16) {
             __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out) + at;
 #pragma unroll 8
-            for (int r = 0; r < rows; ++r, dst += p.N) *dst = __float2bfloat16_rn(value(r) * scale);
+            for (int r = 0; r < rows; ++r, dst += p.N) *dst = __float2bfloat16_rn(value(r));
           } else {
             __half* dst = reinterpret_cast<__half*>(p.out) + at;
 #pragma unroll 8
-            for (int r = 0; r < rows; ++r, dst += p.N) *dst = __float2half_rn(value(r) * scale);
+            for (int r = 0; r < rows; ++r, dst += p.N) *dst = __float2half_rn(value(r));
           }
           return;
         }
@@ -398,7 +403,7 @@ struct EpiGrad {
             t[i] += value(r0 + i);
             if (!in || r0 + i >= rows) continue;
             if (p.write) acc[(int64_t)(r0 + i) * p.N] = t[i];
-            else store_as(p.out, at + (int64_t)(r0 + i) * p.N, t[i] * scale, p.dtype);
+            else store_as(p.out, at + (int64_t)(r0 + i) * p.N, t[i], p.dtype);
           }
         }
       });
@@ -532,13 +537,12 @@ k_loss_rows(const __grid_constant__ JoinArgs p) {
 
 // the splits of K to the result
 __global__ void __launch_bounds__(256)
-k_loss_sum(const float* acc, int splits, int64_t slot, int64_t numel, void* out, ScaleRef scale_ref, int dtype, int with_w) {
+k_loss_sum(const float* acc, int splits, int64_t slot, int64_t numel, void* out, int dtype) {
   pdl_wait();
-  const float scale = grad_scale(scale_ref, with_w);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < numel; i += (int64_t)gridDim.x * 256) {
     float v = 0.f;
     for (int q = 0; q < splits; ++q) v += acc[q * slot + i];
-    store_as(out, i, v * scale, dtype);
+    store_as(out, i, v, dtype);
   }
 }
 
@@ -886,7 +890,7 @@ int prepare(Gradient& q, const Tiling& t) {
 int add_splits(Chain& chain, const Gradient& q) {
   if (q.g.splits == 1) return 0;
   const EpiGrad::Params& e = q.e;
-  return chain.launch(k_loss_sum, dim3(blocks_for(e.slot, 148 * 8)), 256, 0, 1, e.acc, q.g.splits, e.slot, e.slot, e.out, e.scale, e.dtype, e.with_w);
+  return chain.launch(k_loss_sum, dim3(blocks_for(e.slot, 148 * 8)), 256, 0, 1, e.acc, q.g.splits, e.slot, e.slot, e.out, e.dtype);
 }
 // One gradient, or two in one launch
 int gradient(Chain& chain, int planes, int kind, const Gradient& q) {

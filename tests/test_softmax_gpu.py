@@ -398,3 +398,11 @@ def test_small_pieces(dtype, monkeypatch):
     monkeypatch.setattr(softmax, "KEEP_MB", 0)
     got = _check(x, w, y, coef)
     assert torch.equal(got[0], whole[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("coef,x_size,w_size", [(1e-32, 1.0, 1.0), (1e-20, 1e12, 1e-12), (1e-20, 1e-12, 1e12), (1e-18, 1e-14, 1e-6), (1e25, 1e10, 1e-10)])
+def test_gradients_far_from_one(dtype, coef, x_size, w_size):
+    """Coefficients, rows and classes whose product is a normal fp32 number, whatever their powers of two add up to."""
+    x, w, y = _data(150, 333, 56, dtype, 13)
+    _check(x * x_size, w * w_size, y, (torch.rand(150, device="cuda") + 0.5) * coef)
