@@ -21,6 +21,15 @@
 // bits (two planes for fp32: 22); the label's entry of G, where they would cancel, is made from the label's score in fp32.
 // G is rounded to the operands' type: bf16 for bf16; fp16 for fp16, scaled by a power of two so that the largest
 // coefficient is near 2^13; two planes of fp16 for fp32, where x and w are such planes too.
+//
+// Scales of fp32 operands.  Every row of x and every class of w has a power of two of its own, 2^kx_i and 2^kw_j, that brings its
+// largest element to [2^14, 2^15); the epilogues of the scores undo both.  (One power for all of x lets one large row take the bits
+// of all the others: 64 rows, one times 10^10, and the others' losses are 0.1 off.)  The two gradient products sum over different
+// indices and take G scaled differently:
+//   gx_i = 2^{a_i} Σ_j (G_ij 2^{-kw_j} 2^{-a_i}) (2^{kw_j} w_j)      a_i of a row, from the row's largest G_ij 2^{-kw_j}
+//   gw_j = 2^{b_t} Σ_i (G_ij 2^{-kx_i} 2^{-b_t}) (2^{kx_i} x_i)      b_t of a part of a tile's classes, from the largest G_ij 2^{-kx_i} there
+// so that either sum keeps 22 bits of terms down to 2^-17 of its largest, and a unit of 2^-38 of that below.  The maxima follow
+// from the parts' maxima once a row's log-sum-exp is known.
 #include "gemm16.cuh"
 
 namespace psb {
@@ -30,13 +39,12 @@ constexpr int kExpScale = 15;                 // exponentials relative to their 
 
 enum : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
 
-// Exponents of the operands' scales: x and w are multiplied by 2^x and 2^w, G by 2^g.
-struct Scales { int x, w, g; };
-// They are 0 for 16-bit operands and g is known where there are no coefficients; else the device finds them.
+// Exponent of the scale of G with 16-bit operands: 0 for bf16; for fp16 it is known where there are no coefficients, else the
+// device finds it.
 struct ScaleRef {
-  Scales fixed;
-  const Scales* found;         // null: as fixed
-  __device__ __forceinline__ Scales get() const { return found != nullptr ? *found : fixed; }
+  int fixed;
+  const int* found;            // null: as fixed
+  __device__ __forceinline__ int get() const { return found != nullptr ? *found : fixed; }
 };
 // exponent that brings the magnitude with these bits into [2^top, 2^(top+1)); subnormals count as 2^-127, as the scale only
 // has to be representable
@@ -49,14 +57,16 @@ __device__ __forceinline__ float pow2i(int e) {       // 2^e, kept finite; 0 bel
   e = e > 127 ? 127 : e;
   return e < -126 ? 0.f : __int_as_float((e + 127) << 23);
 }
-__device__ __forceinline__ float score_scale(const ScaleRef& r) { const Scales k = r.get(); return kLog2e * pow2i(-(k.x + k.w)); }
 // 2^e in two factors of the same direction: the power may lie outside fp32 where what it scales does not leave it
 struct Pow2 {
   float a, b;
   __device__ __forceinline__ explicit Pow2(int e) : a(pow2i(e / 2)), b(pow2i(e - e / 2)) {}
   __device__ __forceinline__ float operator*(float v) const { return v * a * b; }
 };
-__device__ __forceinline__ Pow2 grad_scale(const ScaleRef& r, int with_w) { const Scales k = r.get(); return Pow2(-(k.g + (with_w ? k.w : k.x))); }
+__device__ __forceinline__ int exponent(float v) { return (int)(__float_as_uint(v) >> 23 & 255u) - 127; }       // of a normal number
+// The exponent of a part's scale from that of its largest G_ij 2^{-kx_i}; no row has any: 0
+constexpr int kScaleTop = 14, kNoRow = -(1 << 30);
+__device__ __forceinline__ int part_scale(int largest) { return largest == kNoRow ? 0 : largest - kScaleTop; }
 __device__ __forceinline__ bool has_class(int64_t y, int V) { return y >= 0 && y < V; }
 
 // ------------------------------------------------------------------ preparation
@@ -85,54 +95,10 @@ __device__ __forceinline__ uint32_t coef_max(const float* coef, const int64_t* y
 }
 // fp16 with coefficients: the scale of G alone (one block)
 __global__ void __launch_bounds__(256)
-k_loss_coef(const float* __restrict__ coef, const int64_t* __restrict__ y, int n, int V, Scales* out) {
+k_loss_coef(const float* __restrict__ coef, const int64_t* __restrict__ y, int n, int V, int* out) {
   pdl_wait();
   const uint32_t top = coef_max(coef, y, n, V);
-  if (threadIdx.x == 0) *out = Scales{0, 0, scale_exp(top, 13)};
-}
-
-// the largest finite magnitude that a thread finds, taking each step-th four columns from the first on (y null: all rows count)
-__device__ __forceinline__ uint32_t thread_absmax(const float* a, int64_t ld, int64_t rows, int cols, const int64_t* y, int V, int64_t first,
-                                                  int64_t step) {
-  uint32_t top = 0;
-  if (y == nullptr && ld == cols && (reinterpret_cast<uintptr_t>(a) & 15) == 0) {       // one long row, whatever its pieces' alignment
-    const int64_t n = rows * cols;
-#pragma unroll 4
-    for (int64_t i = first; i < n / 4; i += step) {
-      const float4 v = reinterpret_cast<const float4*>(a)[i];
-      top = max(max(top, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
-    }
-    for (int64_t i = n / 4 * 4 + first; i < n; i += step) top = max(top, finite_bits(a[i]));
-    return top;
-  }
-  const bool vec = ((reinterpret_cast<uintptr_t>(a) & 15) | (ld & 3)) == 0;
-  const int per = (cols + 3) / 4;
-  const int64_t total = rows * per;
-  for (int64_t i = first; i < total; i += step) {
-    const int64_t r = i / per;
-    const int c = (int)(i - r * per) * 4;
-    if (y != nullptr && !has_class(y[r], V)) continue;
-    const float* p = a + r * ld + c;
-    if (vec && c + 4 <= cols) {
-      const float4 v = *reinterpret_cast<const float4*>(p);
-      top = max(max(top, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
-    } else {
-      for (int j = 0; j < 4 && c + j < cols; ++j) top = max(top, finite_bits(p[j]));
-    }
-  }
-  return top;
-}
-// Largest finite magnitudes of fp32 operands, a block's each: blocks 0..bx-1 take x (rows without a class do not count),
-// the others w.
-__global__ void __launch_bounds__(256)
-k_loss_absmax(const float* __restrict__ x, int64_t ldx, const float* __restrict__ w, int64_t ldw, int n, int V, int d,
-              const int64_t* __restrict__ y, int bx, uint32_t* __restrict__ out) {
-  pdl_wait();
-  const int b = (int)blockIdx.x;
-  const uint32_t top = block_max_u32(b < bx ? thread_absmax(x, ldx, n, d, y, V, (int64_t)b * 256 + threadIdx.x, (int64_t)bx * 256)
-                                            : thread_absmax(w, ldw, V, d, nullptr, V, (int64_t)(b - bx) * 256 + threadIdx.x,
-                                                            (int64_t)(gridDim.x - bx) * 256));
-  if (threadIdx.x == 0) out[b] = top;
+  if (threadIdx.x == 0) *out = scale_exp(top, 13);
 }
 
 struct PackArgs {
@@ -141,36 +107,17 @@ struct PackArgs {
   uint16_t* out;               // operand planes [plane][row][ldo]
   int64_t ldo, plane;
 };
-// Operands into planes of their own: blocks 0..bx-1 pack x, the others w (either may have no blocks).  Rows of x without a
-// class become zeros, whatever they held.  fp32: the scales come from the blocks' maxima and are written for those who follow.
+// 16-bit operands into rows of their own: blocks 0..bx-1 copy x, the others w (either may have no blocks).  Rows of x without a
+// class become zeros, whatever they held.
 template <typename T>
 __global__ void __launch_bounds__(256)
-k_loss_pack(PackArgs px, PackArgs pw, int cols, const int64_t* __restrict__ y, int n, int V, const float* __restrict__ coef, int bx,
-            const uint32_t* maxima, int mx, int mw, Scales* found) {
+k_loss_pack(PackArgs px, PackArgs pw, int cols, const int64_t* __restrict__ y, int V, int bx) {
   pdl_wait();
   const bool is_x = (int)blockIdx.x < bx;
   const PackArgs& p = is_x ? px : pw;
   const int64_t nb = is_x ? bx : gridDim.x - bx, b = is_x ? blockIdx.x : blockIdx.x - bx;
-  float s = 1.f;
-  if (sizeof(T) == 4) {
-    uint32_t tx = 0, tw = 0;
-    const bool last = blockIdx.x == gridDim.x - 1;
-    if (maxima == nullptr) {                 // small operands: every block looks through them itself
-      if (is_x || last) tx = thread_absmax(reinterpret_cast<const float*>(px.a), px.ld, px.rows, cols, y, V, threadIdx.x, 256);
-      if (!is_x) tw = thread_absmax(reinterpret_cast<const float*>(pw.a), pw.ld, pw.rows, cols, nullptr, V, threadIdx.x, 256);
-    } else {
-      if (is_x || last) for (int i = threadIdx.x; i < mx; i += 256) tx = max(tx, maxima[i]);
-      if (!is_x) for (int i = threadIdx.x; i < mw; i += 256) tw = max(tw, maxima[mx + i]);
-    }
-    const int kx = scale_exp(block_max_u32(tx), 14), kw = scale_exp(block_max_u32(tw), 14);
-    s = pow2i(is_x ? kx : kw);
-    if (last) {
-      const uint32_t tc = coef_max(coef, y, n, V);
-      if (threadIdx.x == 0) *found = Scales{kx, kw, scale_exp(tc, 13)};
-    }
-  }
   const T* a = reinterpret_cast<const T*>(p.a);
-  if (((reinterpret_cast<uintptr_t>(a) & 15) | ((p.ld * sizeof(T)) & 15)) != 0) {
+  if (((reinterpret_cast<uintptr_t>(a) & 15) | (p.ld & 7)) != 0) {
     // rows of any alignment: a warp a row, two columns a thread, so that loads and stores are pieces of one row
     const int64_t warps = nb * 8;
     for (int64_t r = b * 8 + (threadIdx.x >> 5); r < p.rows; r += warps) {
@@ -180,12 +127,7 @@ k_loss_pack(PackArgs px, PackArgs pw, int cols, const int64_t* __restrict__ y, i
 #pragma unroll 4
       for (int c = (threadIdx.x & 31) * 2; c < (int)p.ldo; c += 64) {
         const T u = !none && c < cols ? src[c] : T(0), v = !none && c + 1 < cols ? src[c + 1] : T(0);
-        if constexpr (sizeof(T) == 4) {
-          *reinterpret_cast<uint32_t*>(dst + c) = pair16<kFmtPlanes>((float)u * s, (float)v * s, false);
-          *reinterpret_cast<uint32_t*>(dst + p.plane + c) = pair16<kFmtPlanes>((float)u * s, (float)v * s, true);
-        } else {
-          *reinterpret_cast<uint32_t*>(dst + c) = (uint32_t)*reinterpret_cast<const uint16_t*>(&u) | (uint32_t)*reinterpret_cast<const uint16_t*>(&v) << 16;
-        }
+        *reinterpret_cast<uint32_t*>(dst + c) = (uint32_t)*reinterpret_cast<const uint16_t*>(&u) | (uint32_t)*reinterpret_cast<const uint16_t*>(&v) << 16;
       }
     }
     return;
@@ -201,55 +143,129 @@ k_loss_pack(PackArgs px, PackArgs pw, int cols, const int64_t* __restrict__ y, i
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = T(0);
     } else if (c + 8 <= cols) {
-#pragma unroll
-      for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(v)[j] = reinterpret_cast<const uint4*>(src)[j];
+      *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(src);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? src[j] : T(0);
     }
-    uint16_t* dst = p.out + r * p.ldo + c;
-    if constexpr (sizeof(T) == 4) {
-      uint32_t h[4], l[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        h[j] = pair16<kFmtPlanes>((float)v[2 * j] * s, (float)v[2 * j + 1] * s, false);
-        l[j] = pair16<kFmtPlanes>((float)v[2 * j] * s, (float)v[2 * j + 1] * s, true);
+    *reinterpret_cast<uint4*>(p.out + r * p.ldo + c) = *reinterpret_cast<uint4*>(v);
+  }
+}
+
+// fp32 operands into planes, the rows of x and then those of w: kLanes threads (a warp, or the block of 256) find a row's largest
+// finite magnitude, write the power of two that undoes its scale, and split the row.  Rows of x without a class become
+// zeros.  A row of zeros has the largest scale, so that it has no part in maxima over rows.
+template <int kLanes>
+__global__ void __launch_bounds__(256)
+k_loss_planes(PackArgs px, PackArgs pw, int cols, const int64_t* __restrict__ y, int n, int V, float* __restrict__ fx, float* __restrict__ fw,
+              int* __restrict__ largest, int parts) {
+  pdl_wait();
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < parts; i += gridDim.x * 256) largest[i] = kNoRow;
+  const int ln = threadIdx.x % kLanes;
+  const int64_t rows = (int64_t)n + V;
+  for (int64_t r = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes; r < rows; r += (int64_t)gridDim.x * (256 / kLanes)) {
+    const bool is_x = r < n;
+    const PackArgs& p = is_x ? px : pw;
+    const int64_t row = is_x ? r : r - n;
+    const float* src = reinterpret_cast<const float*>(p.a) + row * p.ld;
+    uint16_t* dst = p.out + row * p.ldo;
+    const int d = is_x && !has_class(y[row], V) ? 0 : cols;
+    const bool vec = ((reinterpret_cast<uintptr_t>(p.a) & 15) | (p.ld & 3)) == 0;
+    uint32_t top = 0;
+    if (vec) {
+#pragma unroll 4
+      for (int c = ln * 4; c < d; c += kLanes * 4) {
+        if (c + 4 <= d) {
+          const float4 v = *reinterpret_cast<const float4*>(src + c);
+          top = max(max(top, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
+        } else {
+          for (int j = c; j < d; ++j) top = max(top, finite_bits(src[j]));
+        }
       }
-      *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[2], h[3]);
-      *reinterpret_cast<uint4*>(dst + p.plane) = make_uint4(l[0], l[1], l[2], l[3]);
     } else {
-      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(v);
+#pragma unroll 4
+      for (int c = ln; c < d; c += kLanes) top = max(top, finite_bits(src[c]));
+    }
+    top = kLanes == 32 ? __reduce_max_sync(0xffffffffu, top) : block_max_u32(top);
+    const int k = top == 0 ? 126 : scale_exp(top, kScaleTop);
+    const float s = pow2i(k);
+    if (ln == 0) (is_x ? fx : fw)[row] = pow2i(-k);
+    if (vec) {
+#pragma unroll 4
+      for (int c = ln * 4; c < (int)p.ldo; c += kLanes * 4) {
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c + 4 <= d) v = *reinterpret_cast<const float4*>(src + c);
+        else {
+          if (c < d) v.x = src[c];
+          if (c + 1 < d) v.y = src[c + 1];
+          if (c + 2 < d) v.z = src[c + 2];
+        }
+        *reinterpret_cast<uint2*>(dst + c) = make_uint2(pair16<kFmtPlanes>(v.x * s, v.y * s, false), pair16<kFmtPlanes>(v.z * s, v.w * s, false));
+        *reinterpret_cast<uint2*>(dst + p.plane + c) = make_uint2(pair16<kFmtPlanes>(v.x * s, v.y * s, true), pair16<kFmtPlanes>(v.z * s, v.w * s, true));
+      }
+    } else {                                  // two columns a thread, so that loads and stores are pieces of one row
+#pragma unroll 4
+      for (int c = ln * 2; c < (int)p.ldo; c += kLanes * 2) {
+        const float u = c < d ? src[c] * s : 0.f, v = c + 1 < d ? src[c + 1] * s : 0.f;
+        *reinterpret_cast<uint32_t*>(dst + c) = pair16<kFmtPlanes>(u, v, false);
+        *reinterpret_cast<uint32_t*>(dst + p.plane + c) = pair16<kFmtPlanes>(u, v, true);
+      }
     }
   }
 }
 
 // ------------------------------------------------------------------ epilogues
 // Each row's maximum and Σ 2^(s−m) over a part of a tile's classes, the score of its label, in units of log2 e, and the
-// exponentials that are kept.
+// exponentials that are kept.  With planes, the largest 2^(s−m) 2^{-kw} and the largest 2^(s−m) of the part as well, both without
+// the label's class: where its softmax is near 1, its G is near 0.
 struct EpiScore {
   struct Params {
     CUtensorMap e;             // exponentials [plane][n][keep]
-    float2* part;              // [n][per_tile · class tiles]
+    float2* part;              // [n][per_tile · class tiles]; null: the exponentials alone, of classes from v0 on
+    float2* widest;            // [n][the same]
     float* target;             // [n]
     const int64_t* y;
-    ScaleRef scale;
-    int n, V, parts, per_tile, keep;
+    const float *fx, *fw;      // powers of two that undo the scales of rows and classes
+    int n, V, parts, per_tile, keep, v0;
   };
   template <int kPart>
   static __device__ __forceinline__ void ahead(const Params&, const Tile16&, int, int, int) {}
   template <int kPlanes, int kPart, class Stage, class Sums, class Done>
   static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int part, Stage& st,
                                              const Sums& sums, Done done) {
-    const float scale = score_scale(p.scale);
+    constexpr bool kScaled = kPlanes == 2;
     const int row = row0 + st.lane;
     int64_t lab = -1;
-    if (row < p.n) lab = p.y[row];
+    if (row < p.n) lab = p.y[row] < p.V ? p.y[row] - p.v0 : -1;
+    // A row's factor comes before the class's where it is below 1 and after it elsewhere: no product leaves fp32 on the way to a score
+    // that does not.
+    float before = kLog2e, after = 1.f;
+    if (kScaled && row < p.n) {
+      const float f = p.fx[row];
+      before = kLog2e * fminf(f, 1.f);
+      after = fmaxf(f, 1.f);
+    }
+    // 32 scores; without planes they are not in units of log2 e yet
+    auto scores = [&](int c, float (&v)[32], float (&f)[32]) {
+      sums.load(c, v);
+      if constexpr (kScaled) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 t = *reinterpret_cast<const float4*>(p.fw + p.v0 + col0 + c + j);       // behind the last class lies padding
+          f[j] = t.x; f[j + 1] = t.y; f[j + 2] = t.z; f[j + 3] = t.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __fmul_rn(v[j], before) * f[j] * after;
+      }
+    };
+    auto scaled = [](float v) { return kScaled ? v : __fmul_rn(v, kLog2e); };
+    const int classes = p.V - p.v0;
     float top = -INFINITY;
 #pragma unroll 1
     for (int c = 0; c < kPart; c += 32) {
-      float v[32];
-      sums.load(c, v);
-      const int left = p.V - (col0 + c);
+      float v[32], f[32];
+      scores(c, v, f);
+      const int left = classes - (col0 + c);
       if (left >= 32) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) top = fmaxf(top, v[j]);
@@ -259,41 +275,62 @@ struct EpiScore {
       }
     }
     // without a finite score the reference is 0: 2^(-inf) is 0 and nothing is subtracted from an infinity
-    const float m = __fmul_rn(top, scale), ref = top == -INFINITY ? 0.f : m;
+    const float m = scaled(top), ref = top == -INFINITY ? 0.f : m;
     float s = 0.f;
+    float2 widest = make_float2(0.f, 0.f);
 #pragma unroll 1
     for (int c = 0; c < kPart; c += 32) {
-      float v[32];
-      sums.load(c, v);
+      float v[32], f[32];
+      scores(c, v, f);
       if (c + 32 >= kPart) done();
-      const int col = col0 + c, left = p.V - col;
+      const int col = col0 + c, left = classes - col;
       if (left <= 0) continue;
-      if (lab >= col && lab < col + 32 && lab < p.V) {
-        const int at = (int)(lab - col);
+      const int at = lab >= col && lab < col + 32 ? (int)(lab - col) : -1;
+      if (p.part != nullptr && at >= 0) {
         float t = 0.f;
 #pragma unroll
         for (int j = 0; j < 32; ++j) t = j == at ? v[j] : t;
-        p.target[row] = __fmul_rn(t, scale);
+        p.target[row] = scaled(t);
       }
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
         // product and difference rounded apart, as those of the maximum and of the label are: a row whose class is certain has
         // a loss of 0, not of a rounding
-        v[j] = ex2(__fsub_rn(__fmul_rn(v[j], scale), ref));
+        v[j] = ex2(__fsub_rn(scaled(v[j]), ref));
         if (left < 32) v[j] = j < left ? v[j] : 0.f;
         s += v[j];
-        v[j] *= (float)(1 << kExpScale);
       }
+      if constexpr (kScaled) {
+        if (p.widest != nullptr) {
+          if (__any_sync(0xffffffffu, at >= 0)) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = j == at ? 0.f : f[j];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) widest.y = j == at ? widest.y : fmaxf(widest.y, v[j]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) widest.y = fmaxf(widest.y, v[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) widest.x = fmaxf(widest.x, v[j] * f[j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] *= (float)(1 << kExpScale);
       if (col < p.keep) st.template store<kPlanes == 2 ? kFmtPlanes : kFmtF16>(&p.e, v, row0, col, 0, false);
     }
-    if (row < p.n) p.part[(int64_t)row * p.parts + w.tn * p.per_tile + part] = make_float2(top == -INFINITY ? top : m, s);
+    if (row < p.n && p.part != nullptr) {
+      const int64_t at = (int64_t)row * p.parts + w.tn * p.per_tile + part;
+      p.part[at] = make_float2(top == -INFINITY ? top : m, s);
+      if (kScaled && p.widest != nullptr) p.widest[at] = widest;
+    }
   }
 };
 
-// G of a piece of the classes, in the operands' type, from scores made again
+// G of a piece of the classes, in the operands' 16-bit type, from scores made again
 struct EpiG {
   struct Params {
-    CUtensorMap g;             // [plane][n][len]
+    CUtensorMap g;             // [n][len]
     const float* lse;          // [n], log2
     const float* coef;
     const int64_t* y;
@@ -305,13 +342,12 @@ struct EpiG {
   template <int kPlanes, int kPart, class Stage, class Sums, class Done>
   static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16&, int row0, int col0, int, Stage& st,
                                              const Sums& sums, Done done) {
-    const float scale = score_scale(p.scale);
     const int row = row0 + st.lane;
     float c = 0.f, lse = 0.f;
     int64_t lab = -1;
     if (row < p.n && has_class(p.y[row], p.V)) {
       lab = p.y[row] - p.v0;
-      c = (p.coef != nullptr ? p.coef[row] : 1.f) * pow2i(p.scale.get().g);
+      c = (p.coef != nullptr ? p.coef[row] : 1.f) * pow2i(p.scale.get());
       lse = p.lse[row];
     }
     const bool none = row >= p.n || !has_class(p.y[row], p.V);
@@ -324,9 +360,8 @@ struct EpiG {
       if (col >= p.len) continue;
       const int at = lab >= col && lab < col + 32 ? (int)(lab - col) : -1;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = none ? 0.f : c * (ex2(fmaf(v[j], scale, -lse)) - (at == j ? 1.f : 0.f));
-      if constexpr (kPlanes == 2) st.template store<kFmtPlanes>(&p.g, v, row0, col, 0, false);
-      else if (p.dtype == kBF16) st.template store<kFmtBF16>(&p.g, v, row0, col, 0, false);
+      for (int j = 0; j < 32; ++j) v[j] = none ? 0.f : c * (ex2(fmaf(v[j], kLog2e, -lse)) - (at == j ? 1.f : 0.f));
+      if (p.dtype == kBF16) st.template store<kFmtBF16>(&p.g, v, row0, col, 0, false);
       else st.template store<kFmtF16>(&p.g, v, row0, col, 0, false);
     }
   }
@@ -345,8 +380,10 @@ struct EpiGrad {
     void* out;
     float* acc;
     int64_t slot;
-    ScaleRef scale;
-    int M, N, dtype, with_w, by_map;
+    ScaleRef scale;            // without planes: of G
+    const int* exps;           // with planes: a power of two of the product's rows, of 2^exp_shift of them from row exp_first on
+    int exp_first, exp_shift, exp_parts;       // exp_parts: exps are the parts' largest
+    int M, N, dtype, by_map;
     int read, write;           // acc is added to the product; the sum goes to acc instead of the result
   };
   template <int kPart>
@@ -356,7 +393,14 @@ struct EpiGrad {
   template <int kPlanes, int kPart, class Stage, class Sums, class Done>
   static __device__ __forceinline__ void run(const Params& p, const Gemm16Args&, const Tile16& w, int row0, int col0, int, Stage& st,
                                              const Sums& sums, Done done) {
-    const Pow2 scale = grad_scale(p.scale, p.with_w);
+    int e = 0;
+    if constexpr (kPlanes == 1) {
+      e = -p.scale.get();
+    } else if (row0 + st.lane < p.M) {
+      e = p.exps[(p.exp_first + row0 + st.lane) >> p.exp_shift];
+      if (p.exp_parts) e = part_scale(e);
+    }
+    const Pow2 scale(e);
 #pragma unroll 1
     for (int k = 0; k < kPart; k += 32) {
       float v[32];
@@ -435,6 +479,14 @@ __device__ __forceinline__ float2 join_row(const float2* part, int parts, int ln
   return a;
 }
 
+// What the gradients of fp32 operands need of a row: the maximum and the rest of its log-sum-exp, softmax less 1 at its label;
+// its coefficient as mant · 2^e, less the scale of x where e is used: G_ij 2^{-kx_i} = mant 2^to_w (softmax ...), and mant · 2^{..}
+// of a_i in to_x: G_ij 2^{-a_i} = to_x (softmax ...).
+struct RowStat {
+  float top, rest, at_label, mant, to_x;
+  int to_w, pad[2];
+};
+
 struct JoinArgs {
   const float2* part;
   const float* target;
@@ -450,8 +502,15 @@ struct JoinArgs {
   ScaleRef scale;
   int n, V, d, parts, shift, keep, dtype;    // 2^shift: classes of a part
   uint32_t* status;
+  // fp32
+  const float2* widest;
+  const float *fx, *fw;
+  RowStat* stat;               // null: the losses alone
+  int *row_exp, *largest;      // a_i; of a part's scale
+  uint16_t* g2;                // g becomes G for gx, this is G for gw
+  int v0, len;                 // the classes that g holds
 };
-// A row's log-sum-exp (log2) and loss and, in place, its kept exponentials to G.  kLanes threads a row; blockIdx.y shares
+// 16-bit operands: a row's log-sum-exp (log2) and loss and, in place, its kept exponentials to G.  kLanes threads a row; blockIdx.y shares
 // the classes of a row where there are few rows.  Bound by reading and writing G.
 template <int kLanes>
 __global__ void __launch_bounds__(256)
@@ -489,21 +548,20 @@ k_loss_rows(const __grid_constant__ JoinArgs p) {
       *reinterpret_cast<uint4*>(p.x_out + row * p.ldxo + i) = v;
     }
   }
-  const int kg = p.scale.get().g;
+  const int kg = p.scale.get();
   const float cg = c * pow2i(kg), at_label = cg * (ex2((target - a.x) - l2) - 1.f);
   const float shift = (float)kExpScale + l2;
   uint16_t* g = p.g + (int64_t)row * p.ldg;
   // four eights a thread at a time: their loads do not wait for one another
   const int step = gridDim.y * kLanes * 8;
   for (int first = (blockIdx.y * kLanes + ln) * 8; first < p.keep; first += 4 * step) {
-    uint4 h[4], l[4];
+    uint4 h[4];
     float f[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int col = first + k * step;
       if (col >= p.keep) break;
       h[k] = *reinterpret_cast<const uint4*>(g + col);
-      if (p.dtype == kF32) l[k] = *reinterpret_cast<const uint4*>(g + p.plane + col);
       f[k] = part[col >> p.shift].x;
     }
 #pragma unroll
@@ -512,25 +570,134 @@ k_loss_rows(const __grid_constant__ JoinArgs p) {
       if (col >= p.keep) break;
       const float scale = cg * ex2((f[k] - a.x) - shift);
       const int at = lab >= col && lab < col + 8 ? (int)(lab - col) : -1;
-      uint32_t hs[4] = {h[k].x, h[k].y, h[k].z, h[k].w}, ls[4] = {l[k].x, l[k].y, l[k].z, l[k].w};
+      uint32_t hs[4] = {h[k].x, h[k].y, h[k].z, h[k].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hs[i]));
-        if (p.dtype == kF32) {
-          const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&ls[i]));
-          v.x += u.x; v.y += u.y;
-        }
         v.x = ok ? (at == 2 * i ? at_label : v.x * scale) : 0.f;
         v.y = ok ? (at == 2 * i + 1 ? at_label : v.y * scale) : 0.f;
-        if (p.dtype == kBF16) {
-          hs[i] = pair16<kFmtBF16>(v.x, v.y, false);
-        } else {
-          hs[i] = pair16<kFmtPlanes>(v.x, v.y, false);
-          if (p.dtype == kF32) ls[i] = pair16<kFmtPlanes>(v.x, v.y, true);
-        }
+        hs[i] = p.dtype == kBF16 ? pair16<kFmtBF16>(v.x, v.y, false) : pair16<kFmtF16>(v.x, v.y, false);
       }
       *reinterpret_cast<uint4*>(g + col) = make_uint4(hs[0], hs[1], hs[2], hs[3]);
-      if (p.dtype == kF32) *reinterpret_cast<uint4*>(g + p.plane + col) = make_uint4(ls[0], ls[1], ls[2], ls[3]);
+    }
+  }
+}
+
+// fp32 operands: a row's log-sum-exp and loss, the scale of its G for gx, and its part in the scales of G for gw.
+template <int kLanes>
+__global__ void __launch_bounds__(256)
+k_loss_join(const __grid_constant__ JoinArgs p) {
+  pdl_wait();
+  const int ln = threadIdx.x % kLanes, row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  if (kLanes == 32 && row >= p.n) return;
+  const float2* part = p.part + (int64_t)row * p.parts;
+  const float2 a = join_row<kLanes>(part, p.parts, ln);
+  const float rest = log2f(a.y);
+  const int64_t lab = p.y[row];
+  const bool ok = has_class(lab, p.V);
+  const float c = ok ? (p.coef != nullptr ? p.coef[row] : 1.f) : 0.f;
+  const float target = ok ? p.target[row] : 0.f;
+  if (ln == 0) {
+    if (lab != -1 && !ok) set_status(p.status, kBadIndex, (uint32_t)row, (uint32_t)lab);
+    p.loss[row] = ok ? c * (kLn2 * ((a.x - target) + rest)) : 0.f;
+  }
+  if (p.stat == nullptr) return;
+  // NaN compares as false and is left out of the maxima
+  const float at_label = ok ? ex2((target - a.x) - rest) - 1.f : 0.f, at_log = log2f(fabsf(at_label)), c_log = log2f(fabsf(c));
+  const int fx = exponent(p.fx[row]);
+  auto offer = [&](int t, float v) {
+    v += c_log + (float)fx;
+    if (!(v > -1000.f)) return;
+    const int e = (int)floorf(v < 1000.f ? v : 1000.f);
+    if (e > *reinterpret_cast<volatile int*>(p.largest + t)) atomicMax(p.largest + t, e);
+  };
+  float top = -INFINITY;
+  const float2* widest = p.widest + (int64_t)row * p.parts;
+  if (ok)
+    for (int t = ln; t < p.parts; t += kLanes) {
+      const float v = (part[t].x - a.x) - rest;
+      top = fmaxf(top, v + log2f(widest[t].x));
+      offer(t, v + log2f(widest[t].y));
+    }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (kLanes > 32) {
+    __shared__ float sh[8];
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = sh[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, sh[i]);
+  }
+  if (ln != 0) return;
+  if (ok) {
+    offer((int)(lab >> p.shift), at_log);
+    top = fmaxf(top, at_log + (float)exponent(p.fw[lab]));
+  }
+  // c = mant · 2^e; zeros, infinities and NaN are their own mant
+  float mant = c;
+  int e = 0;
+  if (finite_bits(c) != 0) mant = frexpf(c, &e);
+  // the row's largest |softmax − 1[label]| 2^{-kw}, below 2^floor(top) · 2; a factor below 2^120, so that nothing is multiplied by an infinity
+  int to = top > -1000.f ? (int)floorf(top < 1000.f ? top : 1000.f) - kScaleTop : -120;
+  to = to < -120 ? -120 : to > 120 ? 120 : to;
+  p.row_exp[row] = e + to;
+  p.stat[row] = RowStat{a.x, rest, at_label, mant, mant * pow2i(-to), e + fx, {}};
+}
+
+// fp32 operands: kept exponentials of a row to G for gx, in place, and to G for gw, beside it.  kLanes threads a row; blockIdx.y
+// shares the classes of a row where there are few rows.  Bound by memory.
+template <int kLanes>
+__global__ void __launch_bounds__(256)
+k_loss_grad(const __grid_constant__ JoinArgs p) {
+  pdl_wait();
+  const int ln = threadIdx.x % kLanes, row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  if (kLanes == 32 && row >= p.n) return;
+  const float2* part = p.part + (int64_t)row * p.parts;
+  const RowStat r = p.stat[row];
+  const bool ok = has_class(p.y[row], p.V);
+  const int64_t lab = ok ? p.y[row] - p.v0 : -1;
+  uint16_t *g = p.g + (int64_t)row * p.ldg, *g2 = p.g2 + (int64_t)row * p.ldg;
+  // two eights a thread at a time: their loads do not wait for one another
+  const int step = gridDim.y * kLanes * 8;
+  for (int first = (blockIdx.y * kLanes + ln) * 8; first < p.len; first += 2 * step) {
+    uint4 h[2], l[2];
+    float4 f[2][2];
+    float top[2];
+    int to_w[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int col = first + k * step;
+      if (col >= p.len) break;
+      h[k] = *reinterpret_cast<const uint4*>(g + col);
+      l[k] = *reinterpret_cast<const uint4*>(g + p.plane + col);
+      f[k][0] = *reinterpret_cast<const float4*>(p.fw + p.v0 + col);
+      f[k][1] = *reinterpret_cast<const float4*>(p.fw + p.v0 + col + 4);
+      const int t = (p.v0 + col) >> p.shift;
+      top[k] = part[t].x;
+      to_w[k] = r.to_w - part_scale(p.largest[t]);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int col = first + k * step;
+      if (col >= p.len) break;
+      const float scale = ex2((top[k] - r.top) - r.rest) * pow2i(-kExpScale), w = r.mant * pow2i(to_w[k] < 126 ? to_w[k] : 126);
+      const int at = lab >= col && lab < col + 8 ? (int)(lab - col) : -1;
+      const uint32_t hs[4] = {h[k].x, h[k].y, h[k].z, h[k].w}, ls[4] = {l[k].x, l[k].y, l[k].z, l[k].w};
+      const float fs[8] = {f[k][0].x, f[k][0].y, f[k][0].z, f[k][0].w, f[k][1].x, f[k][1].y, f[k][1].z, f[k][1].w};
+      uint32_t o[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&hs[i])), v = __half22float2(*reinterpret_cast<const __half2*>(&ls[i]));
+        const float a = at == 2 * i ? r.at_label : (u.x + v.x) * scale, b = at == 2 * i + 1 ? r.at_label : (u.y + v.y) * scale;
+        const float ax = ok ? a * fs[2 * i] * r.to_x : 0.f, bx = ok ? b * fs[2 * i + 1] * r.to_x : 0.f, aw = ok ? a * w : 0.f, bw = ok ? b * w : 0.f;
+        o[0][i] = pair16<kFmtPlanes>(ax, bx, false); o[1][i] = pair16<kFmtPlanes>(ax, bx, true);
+        o[2][i] = pair16<kFmtPlanes>(aw, bw, false); o[3][i] = pair16<kFmtPlanes>(aw, bw, true);
+      }
+      *reinterpret_cast<uint4*>(g + col) = make_uint4(o[0][0], o[0][1], o[0][2], o[0][3]);
+      *reinterpret_cast<uint4*>(g + p.plane + col) = make_uint4(o[1][0], o[1][1], o[1][2], o[1][3]);
+      *reinterpret_cast<uint4*>(g2 + col) = make_uint4(o[2][0], o[2][1], o[2][2], o[2][3]);
+      *reinterpret_cast<uint4*>(g2 + p.plane + col) = make_uint4(o[3][0], o[3][1], o[3][2], o[3][3]);
     }
   }
 }
@@ -752,15 +919,14 @@ using namespace psb;
 
 namespace {
 
-constexpr int kMaxBlocks = 148 * 8;           // of the pass that finds the largest magnitudes, for either operand
-
 // where things lie in the workspace; everything is 256-byte aligned
 struct LossPlan {
   int planes, pack_x, pack_w, parts, per_tile, keep, piece, together;
   int tiny, tiny_ld, tiny_ldg, tiny_smem;     // CTAs of k_loss_tiny, 0: the general way
   Tiling score, gx, gw;                       // gx, gw: of the kept classes, or of a piece
   int64_t dp, ldg, x_plane, w_plane, g_plane;
-  int64_t scales, maxima, lse, target, x, w, part, g, gx_acc, gw_acc, total;
+  int64_t scale, lse, target, x, w, part, g, gx_acc, gw_acc, total;
+  int64_t fx, fw, widest, stat, row_exp, largest, g2;       // fp32
 };
 
 // what a plan depends on: sizes, types and alignment
@@ -804,8 +970,7 @@ LossPlan make_loss_plan(const LossKey& a) {
   p.parts = p.per_tile * ((a.V + cols - 1) / cols);
   int64_t at = 0;
   auto take = [&](int64_t bytes) { const int64_t o = at; at += (bytes + 255) / 256 * 256; return o; };
-  p.scales = take(sizeof(Scales));
-  p.maxima = take(2 * kMaxBlocks * 4);
+  p.scale = take(4);
   p.lse = take((int64_t)a.n * 4);
   p.target = take((int64_t)a.n * 4);
   p.x_plane = (int64_t)a.n * p.dp;
@@ -813,13 +978,24 @@ LossPlan make_loss_plan(const LossKey& a) {
   p.w_plane = (int64_t)a.V * p.dp;
   if (p.pack_w) p.w = take(p.w_plane * 2 * p.planes);
   p.part = take((int64_t)p.parts * a.n * 8);
+  if (p.planes == 2) {
+    p.fx = take((int64_t)a.n * 4);
+    p.fw = take(((int64_t)a.V + 256) * 4);          // a tile reads all of its columns' factors
+    if (a.want_grad) {
+      p.widest = take((int64_t)p.parts * a.n * 8);
+      p.stat = take((int64_t)a.n * sizeof(RowStat));
+      p.row_exp = take((int64_t)a.n * 4);
+      p.largest = take((int64_t)p.parts * 4);
+    }
+  }
   if (a.want_grad) {
-    int64_t len = ((int64_t)a.keep_mb << 20) / ((int64_t)a.n * 2 * p.planes) / 256 * 256;
+    int64_t len = ((int64_t)a.keep_mb << 20) / ((int64_t)a.n * (p.planes == 2 ? 8 : 2)) / 256 * 256;
     if (len < 256) len = 256;
     p.keep = p.piece = (int)(len < a.V ? len : a.V);
     p.ldg = ((int64_t)p.piece + 7) / 8 * 8;
     p.g_plane = (int64_t)a.n * p.ldg;
     p.g = take(p.g_plane * 2 * p.planes);
+    if (p.planes == 2) p.g2 = take(p.g_plane * 4);
     const bool pieces = p.piece < a.V;
     p.gw = choose_tiling(1, p.piece, a.d, a.n, p.planes, false, pieces ? 1 : 16);
     p.gx = choose_tiling(1, a.n, a.d, p.piece, p.planes, false, pieces ? 1 : 64);
@@ -923,32 +1099,38 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
   }
   if (p.total > a.ws_bytes || (reinterpret_cast<uintptr_t>(a.ws) & 255)) return (int)cudaErrorInvalidValue;
   uint8_t* ws = reinterpret_cast<uint8_t*>(a.ws);
-  Scales* found = reinterpret_cast<Scales*>(ws + p.scales);
-  uint32_t* maxima = reinterpret_cast<uint32_t*>(ws + p.maxima);
+  int* found = reinterpret_cast<int*>(ws + p.scale);
   float *lse = reinterpret_cast<float*>(ws + p.lse), *target = reinterpret_cast<float*>(ws + p.target);
   uint16_t *xb = reinterpret_cast<uint16_t*>(ws + p.x), *wb = reinterpret_cast<uint16_t*>(ws + p.w), *gb = reinterpret_cast<uint16_t*>(ws + p.g);
   float2* part = reinterpret_cast<float2*>(ws + p.part);
+  const bool f32 = p.planes == 2;
+  float *fx = reinterpret_cast<float*>(ws + p.fx), *fw = reinterpret_cast<float*>(ws + p.fw);
+  float2* widest = reinterpret_cast<float2*>(ws + p.widest);
+  int *row_exp = reinterpret_cast<int*>(ws + p.row_exp), *largest = reinterpret_cast<int*>(ws + p.largest);
+  uint16_t* g2 = reinterpret_cast<uint16_t*>(ws + p.g2);
   Chain chain{s};
   int r = 0;
 
-  ScaleRef scale{{0, 0, a.dtype == kBF16 ? 0 : 13}, nullptr};       // without coefficients the largest is 1
-  if (a.dtype == kF32 || (a.dtype == kF16 && a.coef != nullptr && a.want_grad)) scale.found = found;
-  if (scale.found != nullptr && a.dtype == kF16) r = chain.launch(k_loss_coef, dim3(1), 256, 0, 1, a.coef, a.y, a.n, a.V, found);
-  unsigned mx = 0, mw = 0;
-  const bool small = ((int64_t)a.n + a.V) * a.d <= 32768;      // 128 KB: 32 values a thread, less than a launch
-  if (a.dtype == kF32 && !small) {
-    mx = blocks_for((int64_t)a.n * ((a.d + 3) / 4), kMaxBlocks);
-    mw = blocks_for((int64_t)a.V * ((a.d + 3) / 4), kMaxBlocks);
-    r = chain.launch(k_loss_absmax, dim3(mx + mw), 256, 0, 1, (const float*)a.x, a.ldx, (const float*)a.w, a.ldw, a.n, a.V, a.d, a.y, (int)mx, maxima);
+  ScaleRef scale{a.dtype == kF16 ? 13 : 0, nullptr};       // without coefficients the largest is 1
+  if (a.dtype == kF16 && a.coef != nullptr && a.want_grad) {
+    scale.found = found;
+    if ((r = chain.launch(k_loss_coef, dim3(1), 256, 0, 1, a.coef, a.y, a.n, a.V, found)) != 0) return r;
   }
-  if (r) return r;
   if (p.pack_x || p.pack_w) {
     const PackArgs px{a.x, a.n, a.ldx, xb, p.dp, p.x_plane}, pw{a.w, a.V, a.ldw, wb, p.dp, p.w_plane};
-    const unsigned bx = p.pack_x ? blocks_for((int64_t)a.n * (p.dp / 8), 148 * 8) : 0, bw = p.pack_w ? blocks_for((int64_t)a.V * (p.dp / 8), 148 * 8) : 0;
-    auto pack = [&](auto kernel) {
-      return chain.launch(kernel, dim3(bx + bw), 256, 0, 1, px, pw, a.d, a.y, a.n, a.V, a.coef, (int)bx, small ? nullptr : maxima, (int)mx, (int)mw, found);
-    };
-    r = a.dtype == kF32 ? pack(k_loss_pack<float>) : a.dtype == kBF16 ? pack(k_loss_pack<__nv_bfloat16>) : pack(k_loss_pack<__half>);
+    if (f32) {
+      // a warp takes a row up to 1024 columns, and the block one above
+      const int64_t rows = (int64_t)a.n + a.V;
+      auto planes = [&](auto kernel, int lanes) {
+        return chain.launch(kernel, dim3(blocks_for(rows * lanes, 148 * 8)), 256, 0, 1, px, pw, a.d, a.y, a.n, a.V, fx, fw, largest,
+                            a.want_grad ? p.parts : 0);
+      };
+      r = a.d <= 1024 ? planes(k_loss_planes<32>, 32) : planes(k_loss_planes<256>, 256);
+    } else {
+      const unsigned bx = p.pack_x ? blocks_for((int64_t)a.n * (p.dp / 8), 148 * 8) : 0, bw = p.pack_w ? blocks_for((int64_t)a.V * (p.dp / 8), 148 * 8) : 0;
+      auto pack = [&](auto kernel) { return chain.launch(kernel, dim3(bx + bw), 256, 0, 1, px, pw, a.d, a.y, a.V, (int)bx); };
+      r = a.dtype == kBF16 ? pack(k_loss_pack<__nv_bfloat16>) : pack(k_loss_pack<__half>);
+    }
     if (r) return r;
   }
 
@@ -960,7 +1142,8 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
   g.M = a.n; g.N = a.V; g.K = a.d;
   g.kb_split = (a.d + kG16K - 1) / kG16K;
   EpiScore::Params es = {};
-  es.part = part; es.target = target; es.y = a.y; es.scale = scale; es.n = a.n; es.V = a.V; es.parts = p.parts; es.per_tile = p.per_tile; es.keep = p.keep;
+  es.part = part; es.target = target; es.y = a.y; es.n = a.n; es.V = a.V; es.parts = p.parts; es.per_tile = p.per_tile; es.keep = p.keep;
+  es.fx = fx; es.fw = fw; es.widest = a.want_grad ? widest : nullptr;
   if (a.want_grad && (r = make_out_map(&es.e, Operand16{gb, a.n, p.keep, p.ldg, p.g_plane, p.planes}, 0)) != 0) return r;
   if ((r = product16<EpiScore>(chain, p.planes, p.score.kind, g, x, w, es)) != 0) return r;
 
@@ -972,12 +1155,16 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
     j.g = gb; j.ldg = p.ldg; j.plane = p.g_plane;
     if (!p.pack_x) { j.x = reinterpret_cast<const uint16_t*>(a.x); j.x_out = xb; j.ldx = a.ldx; j.ldxo = p.dp; }
   }
-  if (p.parts <= 64 && a.V <= 2048) {           // a warp a row; with and without gradients alike, so that losses are the same
-    r = chain.launch(k_loss_rows<32>, dim3((unsigned)(a.n + 7) / 8, 1), 256, 0, 1, j);
+  int64_t share = a.want_grad ? (148 * 6 + a.n - 1) / a.n : 1, most = ((int64_t)p.keep + 8191) / 8192;
+  if (share > most) share = most < 1 ? 1 : most;
+  const bool warp_rows = p.parts <= 64 && a.V <= 2048;      // a warp a row; with and without gradients alike, so that losses are the same
+  const dim3 by_warps((unsigned)(a.n + 7) / 8), by_blocks((unsigned)a.n), shared((unsigned)a.n, (unsigned)share);
+  if (f32) {
+    j.widest = widest; j.fx = fx; j.fw = fw; j.row_exp = row_exp; j.largest = largest; j.g2 = g2;
+    if (a.want_grad) j.stat = reinterpret_cast<RowStat*>(ws + p.stat);
+    r = warp_rows ? chain.launch(k_loss_join<32>, by_warps, 256, 0, 1, j) : chain.launch(k_loss_join<256>, by_blocks, 256, 0, 1, j);
   } else {
-    int64_t share = a.want_grad ? (148 * 6 + a.n - 1) / a.n : 1, most = ((int64_t)p.keep + 8191) / 8192;
-    if (share > most) share = most < 1 ? 1 : most;
-    r = chain.launch(k_loss_rows<256>, dim3((unsigned)a.n, (unsigned)share), 256, 0, 1, j);
+    r = warp_rows ? chain.launch(k_loss_rows<32>, by_warps, 256, 0, 1, j) : chain.launch(k_loss_rows<256>, shared, 256, 0, 1, j);
   }
   if (r || !a.want_grad) return r;
 
@@ -985,22 +1172,34 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
   const int64_t es_out = a.dtype == kF32 ? 4 : 2;
   for (int v0 = 0; v0 < a.V; v0 += p.piece) {
     const int len = a.V - v0 < p.piece ? a.V - v0 : p.piece;
-    const Operand16 gop{gb, a.n, len, p.ldg, p.g_plane, p.planes};
-    if (v0 > 0) {                              // beyond the kept classes: scores once more
-      Gemm16Args gs = g;
-      gs.N = len; gs.b_n0 = v0;
+    const Operand16 gop{gb, a.n, len, p.ldg, p.g_plane, p.planes}, gop_w{f32 ? g2 : gb, a.n, len, p.ldg, p.g_plane, p.planes};
+    Gemm16Args gs = g;
+    gs.N = len; gs.b_n0 = v0;
+    if (f32) {
+      if (v0 > 0) {                            // beyond the kept classes: scores and exponentials once more
+        EpiScore::Params again = es;
+        if ((r = make_out_map(&again.e, gop, 0)) != 0) return r;
+        again.part = nullptr; again.widest = nullptr; again.keep = len; again.v0 = v0;
+        if ((r = product16<EpiScore>(chain, p.planes, p.score.kind, gs, x, w, again)) != 0) return r;
+      }
+      j.v0 = v0; j.len = len;
+      r = warp_rows ? chain.launch(k_loss_grad<32>, by_warps, 256, 0, 1, j) : chain.launch(k_loss_grad<256>, shared, 256, 0, 1, j);
+      if (r) return r;
+    } else if (v0 > 0) {                       // scores once more
       EpiG::Params eg = {};
       if ((r = make_out_map(&eg.g, gop, a.dtype == kBF16)) != 0) return r;
       eg.lse = lse; eg.coef = a.coef; eg.y = a.y; eg.scale = scale; eg.n = a.n; eg.V = a.V; eg.len = len; eg.v0 = v0; eg.dtype = a.dtype;
-      if ((r = product16<EpiG>(chain, p.planes, choose_tiling(1, a.n, len, a.d, p.planes, false, 1).kind, gs, x, w, eg)) != 0) return r;
+      Launch16<EpiG, 1> l = {{gs}, {eg}};
+      if ((r = launch_tiled<1, EpiG>(chain, choose_tiling(1, a.n, len, a.d, 1, false, 1).kind, l, x, w)) != 0) return r;
     }
     EpiGrad::Params e = {};
     e.scale = scale; e.dtype = a.dtype;
     Gradient q[2];
     // gw[v0.., :] = Gᵀ x
-    q[0] = Gradient{g, gop, xz, e};
+    q[0] = Gradient{g, gop_w, xz, e};
     q[0].g.M = len; q[0].g.N = a.d; q[0].g.K = a.n; q[0].g.a_mn = q[0].g.b_mn = 1;
     q[0].e.out = reinterpret_cast<uint8_t*>(a.gw) + (int64_t)v0 * a.d * es_out;
+    q[0].e.exps = largest; q[0].e.exp_parts = 1; q[0].e.exp_first = v0; q[0].e.exp_shift = j.shift;
     if (p.gw.splits > 1) q[0].e.acc = reinterpret_cast<float*>(ws + p.gw_acc);
     if ((r = prepare(q[0], p.gw)) != 0) return r;
     if (!p.together && (r = gradient(chain, p.planes, p.gw.kind, q[0])) != 0) return r;
@@ -1008,7 +1207,7 @@ int psb_softmax_loss(const LossArgs* ap, cudaStream_t s) {
     // gx += G w[v0.., :]
     q[1] = Gradient{g, gop, w, e};
     q[1].g.M = a.n; q[1].g.N = a.d; q[1].g.K = len; q[1].g.b_k0 = v0; q[1].g.b_mn = 1;
-    q[1].e.out = a.gx; q[1].e.with_w = 1;
+    q[1].e.out = a.gx; q[1].e.exps = row_exp;
     if (p.gx.splits > 1 || p.piece < a.V) q[1].e.acc = reinterpret_cast<float*>(ws + p.gx_acc);
     if (p.piece < a.V) { q[1].e.read = v0 > 0; q[1].e.write = v0 + len < a.V; }
     if ((r = prepare(q[1], p.gx)) != 0) return r;

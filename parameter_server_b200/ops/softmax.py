@@ -30,10 +30,12 @@ def softmax_loss(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, coef: Option
 
     ``y``: int64 [n], 0 ≤ y < classes; -1 is a row without a class: whatever x and coef hold there, its loss is 0 and it has
     no part in the gradients.  Another label counts as -1 and is reported by :func:`dense.check_status`.  ``coef``: fp32 [n]
-    (None: ones).  Rows of x and w are contiguous, their strides are free.  fp32 operands are multiplied with 22 bits
-    (three fp16 products) relative to the largest of x, of w and of coef: what is below 2^-17 of it keeps fewer.  16-bit
-    operands are multiplied as they are; sums are fp32.  A small call is one launch, in fp32 throughout.  The gradients need a workspace of 2 bytes (fp32: 4) for each row and
-    class, at most 2 GB (or 256 classes): beyond it the classes come in pieces, whose scores are made twice, and n·d floats."""
+    (None: ones).  Rows of x and w are contiguous, their strides are free.  fp32 operands are multiplied with 22 bits (three
+    fp16 products) relative to the largest of their own row or class: elements below 2^-17 of it keep fewer, below 2^-39 none.
+    In the gradients the same holds for a term beside the largest of its row (gx), or of its and up to 127 neighbouring classes
+    (gw).  16-bit operands are multiplied as they are; sums are fp32.  A small call is one launch, in fp32 throughout.  The
+    gradients need a workspace of 2 bytes (fp32: 8) for each row and class, at most 2 GB (or 256 classes): beyond it the classes
+    come in pieces, whose scores are made twice, and n·d floats."""
     gpu = x.get_device()
     for name, t in (("x", x), ("w", w), ("y", y), ("coef", coef)):
         if t is not None and (t.get_device() != gpu or gpu < 0):

@@ -406,3 +406,94 @@ def test_gradients_far_from_one(dtype, coef, x_size, w_size):
     """Coefficients, rows and classes whose product is a normal fp32 number, whatever their powers of two add up to."""
     x, w, y = _data(150, 333, 56, dtype, 13)
     _check(x * x_size, w * w_size, y, (torch.rand(150, device="cuda") + 0.5) * coef)
+
+
+def _check_each(x, w, y, coef=None):
+    """fp32, with a bound for every element that knows its own row and class alone.  A score is off by the steps of its own terms and
+    by 2^-38 of the largest |x_i| times Σ|w_j| (and the other way round), where planes end; a log-sum-exp by its scores' errors,
+    weighted by softmax.  Exponentials end at 2^-39 of the largest among 128 neighbouring classes, G at 2^-38 of the row's largest
+    |G_ij| max|w_j| for gx, and of the largest |G_ij| max|x_i| among 128 neighbouring classes for gw."""
+    from parameter_server_b200.ops import dense, softmax
+
+    loss, gx, gw = softmax.softmax_loss(x, w, y, coef)
+    only = softmax.softmax_loss(x, w, y, coef, want_grad=False)[0]
+    torch.cuda.synchronize()
+    dense.check_status(x.device)
+    assert torch.equal(only, loss)
+    n, d = x.shape
+    V = w.shape[0]
+    X, W, c = x.double(), w.double(), torch.ones(n, dtype=torch.float64, device=x.device) if coef is None else coef.double()
+    rows = torch.arange(n, device=x.device)
+    s, mag = X @ W.T, X.abs() @ W.abs().T
+    lse = torch.logsumexp(s, 1)
+    p = torch.exp(s - lse[:, None])
+    xm, wm = X.abs().max(1).values, W.abs().max(1).values
+    e_s = _steps(d, torch.float32) * mag + 2.0 ** -22 * s.abs() + 2.0 ** -38 * (xm[:, None] * W.abs().sum(1) + X.abs().sum(1)[:, None] * wm)
+    e_lse = (p * e_s).sum(1) + 2.0 ** -20
+    ref, tol = c * (lse - s[rows, y]), c.abs() * (e_s[rows, y] + e_lse + 2.0 ** -20)
+    off = ((loss.double() - ref).abs() / (tol + 2.0 ** -22 * ref.abs() + 1e-37))
+    assert bool((off <= 1).all()), ("loss", off.max().item())
+    G = c[:, None] * p
+
+    def blocks(t):                                  # the largest of 128 neighbouring classes
+        top = torch.nn.functional.pad(t, (0, -V % 128)).reshape(n, -1, 128).max(2).values
+        return top.repeat_interleave(128, 1)[:, :V]
+
+    eG = G.abs() * (e_s + e_lse[:, None] + 2.0 ** -20 + 2.0 ** -21) + 2.0 ** -39 * blocks(G.abs())
+    G[rows, y] -= c
+    eG += G.abs() * 2.0 ** -22
+    unit_x = 2.0 ** -38 * ((G.abs() * wm).max(1).values[:, None] / wm)
+    unit_w = 2.0 ** -38 * (blocks(G.abs() * xm[:, None]).max(0).values / xm[:, None])
+    for name, got, A, eA, B, bm, k in (("gx", gx, G, eG + unit_x, W, wm, V), ("gw", gw, G.T, (eG + unit_w).T, X, xm, n)):
+        want = A @ B
+        tol = (eA + _steps(k, torch.float32) * A.abs()) @ B.abs() + (A.abs() + eA) @ (2.0 ** -38 * bm)[:, None] + 2.0 ** -23 * want.abs() + 1e-37
+        off = (got.double() - want).abs() / tol
+        assert bool((off <= 1).all()), (name, off.max().item())
+
+
+@pytest.mark.parametrize("size", [1e-12, 1e-3, 1e5, 1e8, 1e12])
+@pytest.mark.parametrize("n,V,d", [(64, 2000, 64), (700, 900, 130), (40, 3001, 1030), (2, 5000, 96)])
+def test_rows_and_classes_keep_their_bits_beside_larger_ones(n, V, d, size):
+    """One row of another magnitude (its class certain, or not), one class, coefficients, all of them, in fp32."""
+    x, w, y = _data(n, V, d, torch.float32, 14, scale=1.0)
+    x2, w2, y2 = x.clone(), w.clone(), y.clone()
+    x2[0] *= size
+    y2[0] = (x2[0].double() @ w.double().T).argmax()
+    _check_each(x2, w, y2)
+    w2[V // 2] *= size
+    _check_each(x, w2, y)
+    coef = torch.rand(n, device="cuda") + 0.5
+    coef[-1] *= size
+    _check_each(x, w, y, coef)
+    x3 = x * size ** torch.linspace(-0.5, 0.5, n, device="cuda")[:, None]
+    w3 = w * size ** torch.linspace(-0.5, 0.0, V, device="cuda")[:, None]
+    _check_each(x3, w3, (x3.double() @ w3.double().T).argmax(1), coef)
+
+
+def test_rows_and_classes_of_different_sizes_in_pieces(monkeypatch):
+    from parameter_server_b200.ops import softmax
+
+    monkeypatch.setattr(softmax, "KEEP_MB", 0)
+    x, w, y = _data(200, 1500, 80, torch.float32, 15, scale=1.0)
+    x[3] *= 1e6
+    y[3] = (x[3].double() @ w.double().T).argmax()
+    w[7] *= 1e-6
+    w[700:720] *= 1e4
+    _check_each(x, w, y, torch.rand(200, device="cuda") + 0.5)
+
+
+def test_zero_rows_and_classes_beside_small_ones():
+    """A row or class of zeros has no magnitude that others are measured by."""
+    for size in (1e-12, 1.0, 1e12):
+        x, w, y = _data(90, 1200, 48, torch.float32, 16, scale=1.0)
+        x[5], w[11] = 0, 0
+        x, w = x * size, w / size
+        from parameter_server_b200.ops import softmax
+
+        _, gx, gw = softmax.softmax_loss(x, w, y)
+        X, W = x.double(), w.double()
+        G = torch.softmax(X @ W.T, 1)
+        G[torch.arange(90, device="cuda"), y] -= 1
+        # 22-bit operands and cut sums of 1200 and 90 terms: far below 2^-16 of a gradient's terms
+        for got, A, B in ((gx, G, W), (gw, G.T, X)):
+            assert bool(((got.double() - A @ B).abs() <= 2.0 ** -16 * (A.abs() @ B.abs())).all())
