@@ -239,3 +239,21 @@ def test_update_captured_and_on_another_stream():
 def test_short_sides_that_end_inside_a_warp(shape):
     """Rounded up to 16 they are 48, 80 or 112: of the warp that holds the last 16 rows, half has none."""
     _check(_data(shape, 10))
+
+
+@pytest.mark.parametrize("shape", [(1, 7), (5, 72), (700, 9), (16, 5000), (3, 40, 12), (16385, 16), (200, 2, 3)])
+@pytest.mark.parametrize("gtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_update_of_thin_matrices(shape, gtype, nesterov):
+    """A short side of at most 16, either way round, batched, on one CTA and on several, against the definition."""
+    test_update(shape, gtype, nesterov)
+
+
+@pytest.mark.parametrize("shape", [(2, 264, 520), (130, 136), (203, 301), (300, 8000), (64, 64), (96, 700), (5, 72), (3, 40, 12)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("offset", [0, 1, 2, 4, 8])
+def test_matrix_at_any_address(shape, dtype, offset):
+    """Wide and single loads of all types, each against the definition: a bound relative to the result, matrix by matrix."""
+    numel = torch.Size(shape).numel()
+    x = (_data(shape, 11) * 1e-2).to(dtype)
+    _check(torch.zeros(numel + 16, dtype=dtype, device="cuda")[offset: offset + numel].view(shape).copy_(x))

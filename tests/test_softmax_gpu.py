@@ -497,3 +497,74 @@ def test_zero_rows_and_classes_beside_small_ones():
         # 22-bit operands and cut sums of 1200 and 90 terms: far below 2^-16 of a gradient's terms
         for got, A, B in ((gx, G, W), (gw, G.T, X)):
             assert bool(((got.double() - A @ B).abs() <= 2.0 ** -16 * (A.abs() @ B.abs())).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V,d", [(2500, 9000, 640), (2305, 6000, 600), (4096, 8200, 800), (3001, 8001, 1001), (2500, 20_000, 1030)])
+def test_tiles_of_pairs_256_wide(n, V, d, dtype):
+    """Sizes of large nets: scores and both gradients in the largest tiles, with two and (16 bits, d up to 768) four epilogue warps for
+    32 rows, whole and with split sums, results by boxes and by rows."""
+    x, w, y = _data(n, V, d, dtype, 17)
+    y[::11] = -1
+    _check(x, w, y, torch.rand(n, device="cuda") + 0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V,d", [(2500, 20_011, 640), (2500, 13_000, 1001)])
+def test_large_pieces(n, V, d, dtype, monkeypatch):
+    """Pieces of some thousand classes, whose scores are made again in the largest tiles."""
+    from parameter_server_b200.ops import softmax
+
+    x, w, y = _data(n, V, d, dtype, 18)
+    coef = torch.rand(n, device="cuda") + 0.5
+    whole = softmax.softmax_loss(x, w, y, coef)
+    monkeypatch.setattr(softmax, "KEEP_MB", 80 if dtype == torch.float32 else 20)
+    assert torch.equal(_check(x, w, y, coef)[0], whole[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V,d", [(1000, 3, 200), (2000, 40, 64), (3000, 17, 64), (6000, 8, 500)])
+def test_infinity_stays_in_its_row_where_classes_are_few(n, V, d, dtype):
+    """Beyond the single launch, where a step on the tensor cores multiplies 16 to 48 classes."""
+    test_infinity_in_a_row_stays_in_its_row(n, V, d, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,V,d", [(500, 700, 32), (3000, 40, 64)])
+def test_nan_and_bad_labels_beyond_the_single_launch(n, V, d, dtype):
+    from parameter_server_b200.ops import dense, softmax
+
+    x, w, y = _data(n, V, d, dtype, 19)
+    x[4, 5], x[9, 1] = float("nan"), float("inf")
+    loss, gx, _ = softmax.softmax_loss(x, w, y)
+    bad = torch.zeros(n, dtype=torch.bool, device="cuda")
+    bad[4] = bad[9] = True
+    assert bool(torch.isnan(loss[bad]).all()) and bool(torch.isfinite(loss[~bad]).all())
+    assert bool(torch.isnan(gx[bad]).any(1).all()) and bool(torch.isfinite(gx[~bad]).all())
+    x, w, y = _data(n, V, d, dtype, 19)
+    dense.check_status(x.device)
+    wrong = y.clone()
+    wrong[3], wrong[7], wrong[11] = V, -2, 1 << 40
+    got = softmax.softmax_loss(x, w, wrong)
+    with pytest.raises(RuntimeError):
+        dense.check_status(x.device)
+    wrong[[3, 7, 11]] = -1
+    for a, b in zip(got, softmax.softmax_loss(x, w, wrong)):
+        assert torch.equal(a, b)
+    dense.check_status(x.device)
+
+
+def test_gradients_against_differences_beyond_the_single_launch():
+    """As for small calls: with h = 2^-3 and directions of length 1 the difference is off by less than h²/6 of a third derivative
+    below |direction·w|³ < 1e-2 of it, and the sum of 300 fp32 losses by 300 · 2^-20 at most, over 2h."""
+    from parameter_server_b200.ops import softmax
+
+    x, w, y = _data(300, 400, 40, torch.float32, 20)
+    coef = torch.rand(300, device="cuda") + 0.5
+    _, gx, gw = softmax.softmax_loss(x, w, y, coef)
+    h = 2.0 ** -3
+    for t, g in ((x, gx), (w, gw)):
+        u = torch.randn_like(t)
+        u = u / u.norm()
+        f = [softmax.softmax_loss(*(a + s * h * u if a is t else a for a in (x, w)), y, coef, want_grad=False)[0].double().sum() for s in (1, -1)]
+        assert abs(((f[0] - f[1]) / (2 * h)).item() - (g.double() * u.double()).sum().item()) < 4e-3
