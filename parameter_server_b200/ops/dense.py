@@ -15,10 +15,16 @@ _status = {}
 
 
 def _status_for(dev) -> torch.Tensor:
+    """The status words of a device, one tensor for as long as the process runs: kernels in flight hold its address.  Threads that
+    ask for it at once get the same."""
     k = (dev.type, dev.index)
-    if k not in _status:
-        _status[k] = torch.zeros(8, dtype=torch.int32, device=dev)
-    return _status[k]
+    st = _status.get(k)
+    if st is None:
+        st = torch.zeros(8, dtype=torch.int32, device=dev)
+        if dev.type == "cuda" and not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(dev).synchronize()        # zeroed before a kernel on another stream writes to them
+        st = _status.setdefault(k, st)
+    return st
 
 
 def status_ptr(dev) -> int:
