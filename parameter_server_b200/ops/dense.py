@@ -14,10 +14,15 @@ ACT = {"IDENTITY": 0, "RELU": 1, "SCALED_TANH": 2, "SIGMOID": 3}
 _status = {}
 
 
+def _key(dev) -> tuple:
+    """A device without an index is the current GPU, as everywhere in PyTorch."""
+    return dev.type, torch.cuda.current_device() if dev.type == "cuda" and dev.index is None else dev.index
+
+
 def _status_for(dev) -> torch.Tensor:
     """The status words of a device, one tensor for as long as the process runs: kernels in flight hold its address.  Threads that
     ask for it at once get the same."""
-    k = (dev.type, dev.index)
+    k = _key(dev)
     st = _status.get(k)
     if st is None:
         st = torch.zeros(8, dtype=torch.int32, device=dev)
@@ -30,7 +35,7 @@ def _status_for(dev) -> torch.Tensor:
 def status_ptr(dev) -> int:
     """Address of the status words of a GPU for operators that may be captured: the words are made and zeroed outside of a
     graph, whose replays would zero them again."""
-    st = _status.get((dev.type, dev.index))
+    st = _status.get(_key(dev))
     if st is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("run the operator, or dense.check_status(device), once on this GPU before it is captured")
