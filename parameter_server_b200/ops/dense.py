@@ -35,7 +35,9 @@ def _status_for(dev) -> torch.Tensor:
 def status_ptr(dev) -> int:
     """Address of the status words of a GPU for operators that may be captured: the words are made and zeroed outside of a
     graph, whose replays would zero them again."""
-    st = _status.get(_key(dev))
+    st = _status.get((dev.type, dev.index))          # as tensors have it
+    if st is None:
+        st = _status.get(_key(dev))
     if st is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("run the operator, or dense.check_status(device), once on this GPU before it is captured")
