@@ -648,9 +648,9 @@ k_loss_join(const __grid_constant__ JoinArgs p) {
     float mant = c;
     int e = 0;
     if (finite_bits(c) != 0) mant = frexpf(c, &e);
-    // the row's largest |softmax − 1[label]| 2^{-kw}, below 2^floor(top) · 2; a factor below 2^120, so that nothing is multiplied by an infinity
-    int to = top > -1000.f ? (int)floorf(top < 1000.f ? top : 1000.f) - kScaleTop : -120;
-    to = to < -120 ? -120 : to > 120 ? 120 : to;
+    // the row's largest |softmax − 1[label]| 2^{-kw}, below 2^floor(top) · 2; a finite factor, so that nothing is multiplied by an infinity
+    int to = top > -1000.f ? (int)floorf(top < 1000.f ? top : 1000.f) - kScaleTop : -126;
+    to = to < -126 ? -126 : to > 126 ? 126 : to;
     p.row_exp[row] = e + to;
     p.stat[row] = RowStat{a.x, rest, at_label, mant, mant * pow2i(-to), e + fx, {}};
   }
@@ -686,7 +686,7 @@ k_loss_grad(const __grid_constant__ JoinArgs p) {
     for (int i = 0; i < 4; ++i) {
       const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&hs[i])), v = __half22float2(*reinterpret_cast<const __half2*>(&ls[i]));
       const float a = at == 2 * i ? r.at_label : (u.x + v.x) * scale, b = at == 2 * i + 1 ? r.at_label : (u.y + v.y) * scale;
-      const float ax = ok ? a * fs[2 * i] * r.to_x : 0.f, bx = ok ? b * fs[2 * i + 1] * r.to_x : 0.f, aw = ok ? a * w : 0.f, bw = ok ? b * w : 0.f;
+      const float ax = ok ? a * r.to_x * fs[2 * i] : 0.f, bx = ok ? b * r.to_x * fs[2 * i + 1] : 0.f, aw = ok ? a * w : 0.f, bw = ok ? b * w : 0.f;
       o[0][i] = pair16<kFmtPlanes>(ax, bx, false); o[1][i] = pair16<kFmtPlanes>(ax, bx, true);
       o[2][i] = pair16<kFmtPlanes>(aw, bw, false); o[3][i] = pair16<kFmtPlanes>(aw, bw, true);
     }

@@ -568,3 +568,25 @@ def test_gradients_against_differences_beyond_the_single_launch():
         u = u / u.norm()
         f = [softmax.softmax_loss(*(a + s * h * u if a is t else a for a in (x, w)), y, coef, want_grad=False)[0].double().sum() for s in (1, -1)]
         assert abs(((f[0] - f[1]) / (2 * h)).item() - (g.double() * u.double()).sum().item()) < 4e-3
+
+
+@pytest.mark.parametrize("x_size,w_size", [(1e26, 1e-26), (1e-26, 1e26), (1e30, 1e-30), (1e-30, 1e30), (1e36, 1e-36), (1e-36, 1e36), (1e-20, 1e-12)])
+def test_rows_and_classes_at_the_ends_of_fp32(x_size, w_size):
+    """Every power of two on the way to scores and gradients stays in fp32.  Classes or rows of 1e-30 and below cannot be brought to
+    2^14 by a scale that fp32 can undo: gradients are held to 2^-16 of their terms."""
+    from parameter_server_b200.ops import softmax
+
+    x, w, y = _data(120, 1500, 72, torch.float32, 21, scale=1.0)
+    x, w = x * x_size, w * w_size
+    if x_size in (1e26, 1e-26):
+        _check_each(x, w, y)
+    loss, gx, gw = softmax.softmax_loss(x, w, y)
+    X, W = x.double(), w.double()
+    s = X @ W.T
+    G = torch.softmax(s, 1)
+    want = torch.logsumexp(s, 1) - s.gather(1, y[:, None])[:, 0]
+    # 2^-18 of scores' terms: 22-bit operands, cut sums of 72 terms
+    assert bool(((loss.double() - want).abs() <= 2.0 ** -17 * ((X.abs() @ W.abs().T).max(1).values + want)).all())
+    G[torch.arange(120, device="cuda"), y] -= 1
+    for got, A, B in ((gx, G, W), (gw, G.T, X)):
+        assert bool(((got.double() - A @ B).abs() <= 2.0 ** -16 * (A.abs() @ B.abs()) + 2.0 ** -140).all())
