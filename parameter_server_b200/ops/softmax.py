@@ -33,9 +33,17 @@ def softmax_loss(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, coef: Option
     (None: ones).  Rows of x and w are contiguous, their strides are free.  fp32 operands are multiplied with 22 bits (three
     fp16 products) relative to the largest of their own row or class: elements below 2^-17 of it keep fewer, below 2^-39 none.
     In the gradients the same holds for a term beside the largest of its row (gx), or of its and up to 127 neighbouring classes
-    (gw).  16-bit operands are multiplied as they are; sums are fp32.  A small call is one launch, in fp32 throughout.  The
-    gradients need a workspace of 2 bytes (fp32: 8) for each row and class, at most 2 GB (or 256 classes): beyond it the classes
-    come in pieces, whose scores are made twice, and n·d floats."""
+    (gw).  A small call is one launch, in fp32 throughout.
+
+    16-bit operands are multiplied as they are, and summed in fp32 on the tensor cores, which cut a sum at every 16 elements (scores
+    of 1024 columns: 3e-7 of the loss).  The gradient of the scores is rounded to the operands' type before its two products (bf16
+    gradients are off by 0.17 to 0.25 % instead of the 0.17 % that their own rounding takes); fp16 keeps it relative to the call's
+    largest coefficient, in units of 2^-38 of that.
+
+    Workspace: 8 bytes (fp32 with gradients: 16) for each row and 32 to 128 classes, for losses alone too; fp32 operands once more,
+    and 16-bit ones whose rows do not start at 16 bytes; for gradients x once more, 2 bytes (fp32: 8) for each row and class, at most
+    2 GB (or 256 classes; beyond that the classes come in pieces, whose scores are made twice), and fp32 copies of gx, and of either
+    gradient where its product is split."""
     gpu = x.get_device()
     for name, t in (("x", x), ("w", w), ("y", y), ("coef", coef)):
         if t is not None and (t.get_device() != gpu or gpu < 0):
