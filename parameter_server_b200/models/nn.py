@@ -98,6 +98,7 @@ class DataLayer(Layer):
         self.set_data(X, torch.from_numpy(labels.astype(np.float32)))
 
     def set_data(self, X: torch.Tensor, y: torch.Tensor, normalize: bool = True) -> None:
+        self._check_labels(y)
         self.X = X.to(self.net.device).contiguous().float()
         self.y = y.to(self.net.device).float()
         if normalize:
@@ -106,10 +107,19 @@ class DataLayer(Layer):
     def set_sparse_data(self, off: torch.Tensor, idx: torch.Tensor, vals: Optional[torch.Tensor], y: torch.Tensor,
                         in_dim: int) -> None:
         """Keep the examples as CSR rows (for a SPARSE_FULLY_CONNECTED consumer): minibatches are row subsets."""
+        self._check_labels(y)
         d = self.net.device
         self.X = None
         self.csr = (off.to(d).long(), idx.to(d).int(), None if vals is None else vals.to(d).float(), int(in_dim))
         self.y = y.to(d).float()
+
+    def _check_labels(self, y: torch.Tensor) -> None:
+        """A softmax loss that takes this layer's labels counts every other number as a row without a class."""
+        for lc in self.net.conf.layer:
+            if lc.type == "SOFTMAX_LOSS" and any(name in list(lc.get("in")) for name in list(self.conf.out)[1:]):
+                bad = (y != y.floor() if y.is_floating_point() else torch.zeros_like(y, dtype=torch.bool)) | ~((y >= -1) & (y < lc.size))
+                if bool(bad.any()):
+                    raise ValueError(f"layer {lc.name}: labels are class numbers from 0 to {lc.size - 1}, or -1: got {y[bad].reshape(-1)[0].item()}")
 
     def _sparse_minibatch(self):
         off, idx, vals, in_dim = self.csr
@@ -250,7 +260,8 @@ class LogisticLossLayer(Layer):
 
 class SoftmaxLossLayer(Layer):
     """Softmax cross entropy over ``size`` classes: the layer holds the classes' weights [size, in], so that the scores
-    need not be kept.  Labels are class numbers from 0 on, as floats or integers; -1 is a row without a class."""
+    need not be kept.  Labels are class numbers from 0 on, as floats or integers; -1 is a row without a class, which counts as a
+    row of loss 0 in the mean that is reported."""
 
     def init(self) -> None:
         self.classes = int(self.conf.size)

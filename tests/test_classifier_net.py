@@ -197,3 +197,19 @@ def test_a_job_from_files(tmp_path):
     conf = cfg.parse_app_config(NET % dict(batch=64, hidden=32, classes=7, update="ORTHOGONAL", iters=3, valid=3, data=data))
     out = nn.run_nn_job(conf, None, PeerGroup.single(torch.device("cuda", 0)))
     assert len(out["history"]) == 3 and out["history"][-1]["test_loss"] > 0
+
+
+@pytest.mark.parametrize("bad", [10.0, 2.5, -2.0, float("nan"), float("inf")])
+def test_labels_that_are_no_classes_are_refused(bad):
+    """They would count as rows without a class, and the job would learn of it at its end only."""
+    X, y = _data(30)
+    sol = nn.SGDSolver(_conf(), PeerGroup.single(torch.device("cpu")))
+    sol.train.layer("data").set_data(X, y, normalize=False)
+    wrong = y.clone()
+    wrong[4] = bad
+    with pytest.raises(ValueError, match="class numbers"):
+        sol.train.layer("data").set_data(X, wrong, normalize=False)
+    with pytest.raises(ValueError, match="class numbers"):
+        sol.train.layer("data").set_sparse_data(torch.arange(31), torch.zeros(30), None, wrong, 5)
+    assert torch.equal(sol.train.layer("data").y, y)
+    sol.train.layer("data").set_data(X, y.long(), normalize=False)
