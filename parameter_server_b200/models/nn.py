@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import math
 import sys
+import warnings
 import zlib
 from dataclasses import dataclass
 from typing import Dict, List, Optional
@@ -95,6 +96,8 @@ class DataLayer(Layer):
         labels = r.value(0)
         if not any(lc.type == "SOFTMAX_LOSS" for lc in self.net.conf.layer):      # whose labels are the numbers of classes
             labels = np.where(labels > 0, 1.0, -1.0)
+        elif set(np.unique(labels).tolist()) == {-1.0, 1.0}:
+            warnings.warn(f"layer {self.name}: labels are -1 and 1; to a softmax loss -1 is a row without a class, and classes are numbered from 0")
         self.set_data(X, torch.from_numpy(labels.astype(np.float32)))
 
     def set_data(self, X: torch.Tensor, y: torch.Tensor, normalize: bool = True) -> None:

@@ -213,3 +213,10 @@ def test_labels_that_are_no_classes_are_refused(bad):
         sol.train.layer("data").set_sparse_data(torch.arange(31), torch.zeros(30), None, wrong, 5)
     assert torch.equal(sol.train.layer("data").y, y)
     sol.train.layer("data").set_data(X, y.long(), normalize=False)
+
+
+def test_files_of_signs_are_pointed_out(tmp_path, cpu_ops):
+    X, y = _data(30, classes=2)
+    _write_libsvm(tmp_path / "part", X, torch.where(y > 0, 1.0, -1.0))
+    with pytest.warns(UserWarning, match="numbered from 0"):
+        nn.SGDSolver(_conf(data=f'data {{ format: TEXT text: LIBSVM file: "{tmp_path}/part" }}'), PeerGroup.single(torch.device("cpu")))
