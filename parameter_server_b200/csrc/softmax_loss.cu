@@ -8,14 +8,14 @@
 // kernel joins the parts of a row to its log-sum-exp.
 //
 // For the gradients the epilogue also writes e^{s−m} · 2^15 in fp16 (relative to the part's own maximum, which is all that
-// is known then), for as many classes as the workspace holds; the second kernel turns it into G in place, with one
-// factor a part.  Making the scores once costs 6nVd operations instead of 8nVd, for a pass over 2 bytes an element
+// is known then), for as many classes as the workspace holds; the second kernel (a third for fp32) turns it into G in place, with
+// one factor a part.  Making the scores once costs 6nVd operations instead of 8nVd, for a pass over 2 bytes an element
 // (8192 rows, 131,072 classes, 2048 wide: 3.2 ms less for 0.85).  Classes beyond the workspace come in pieces, whose scores
 // are made again.  gw of a piece is complete, gx is summed over the pieces in fp32.  Sums have a fixed order: results do not
 // vary from run to run.
 //
-// Bound by the tensor cores: bf16 scores of 4096 rows against 131,072 classes, 1024 wide, take 785 us, 0.83 of the rate of a plain
-// cuBLAS product; 8192 x 131,072 x 2048 with gradients takes 10.4 ms where the products alone, at its sustained rate, take 9.5.
+// Bound by the tensor cores: bf16 scores of 4096 rows against 131,072 classes, 1024 wide, take 785 to 810 us, 0.8 of the rate of a
+// plain cuBLAS product; 8192 x 131,072 x 2048 with gradients takes 10.4 to 10.9 ms where the products alone, at its sustained rate, take 9.5.
 //
 // Scores, maxima, sums and losses are fp32 (in units of log2 e: 2^x is the hardware's exponential).  The exponentials keep 11
 // bits (two planes for fp32: 22); the label's entry of G, where they would cancel, is made from the label's score in fp32.
@@ -480,9 +480,8 @@ __device__ __forceinline__ float2 join_row(const float2* part, int parts, int ln
   return a;
 }
 
-// What the gradients of fp32 operands need of a row: the maximum and the rest of its log-sum-exp, softmax less 1 at its label;
-// its coefficient as mant · 2^e, less the scale of x where e is used: G_ij 2^{-kx_i} = mant 2^to_w (softmax ...), and mant · 2^{..}
-// of a_i in to_x: G_ij 2^{-a_i} = to_x (softmax ...).
+// What the gradients of fp32 operands need of a row: the maximum and the rest of its log-sum-exp (log2), p − 1 of its label's
+// softmax p, and its coefficient c = mant · 2^e with the scales that G takes:  c 2^{-a_i} = to_x,  c 2^{-kx_i} = mant · 2^to_w.
 struct RowStat {
   float top, rest, at_label, mant, to_x;
   int to_w, pad[2];
