@@ -590,3 +590,11 @@ def test_rows_and_classes_at_the_ends_of_fp32(x_size, w_size):
     G[torch.arange(120, device="cuda"), y] -= 1
     for got, A, B in ((gx, G, W), (gw, G.T, X)):
         assert bool(((got.double() - A @ B).abs() <= 2.0 ** -16 * (A.abs() @ B.abs()) + 2.0 ** -140).all())
+
+
+@pytest.mark.parametrize("n,V,d", [(3, 200_000, 16), (700, 70_003, 40), (5, 1_000_003, 8), (1300, 40_000, 24)])
+def test_many_parts_of_many_classes(n, V, d):
+    """fp32: more parts of a row than a block keeps, rows that a block takes one after the other, by warps and by blocks."""
+    x, w, y = _data(n, V, d, torch.float32, 22)
+    y[1] = -1
+    _check(x, w, y, torch.rand(n, device="cuda") + 0.5)
