@@ -997,7 +997,7 @@ LossPlan make_loss_plan(const LossKey& a) {
     if (a.want_gx && !pieces && (p.gw.kind == kOne128 || p.gw.kind == kOne64)) {
       const Tiling t = choose_tiling(1, a.n, a.d, p.piece, p.planes, false, 64, 1, p.gw.kind);
       auto tiles = [&](const Tiling& u, int64_t M) { return (M + 127) / 128 * ((a.d + tiling_cols(u.kind) - 1) / tiling_cols(u.kind)) * u.splits; };
-      if (tiles(p.gw, a.V) + tiles(t, a.n) <= 148) {
+      if (t.kind == p.gw.kind && tiles(p.gw, a.V) + tiles(t, a.n) <= 148) {
         p.together = 1;
         p.gx = t;
       }

@@ -598,3 +598,43 @@ def test_many_parts_of_many_classes(n, V, d):
     x, w, y = _data(n, V, d, torch.float32, 22)
     y[1] = -1
     _check(x, w, y, torch.rand(n, device="cuda") + 0.5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradients_of_millions_of_rows(dtype, monkeypatch):
+    """A sum over 6,000,001 rows on the tensor cores, a cut for each 16 of them, would be 0.8 % short.  Added up every 32,768 rows it is
+    cut by 2^-23 2048 times, 2^-12 at worst; the roundings of G are independent and fall by the root of the rows (2^-12 is far above);
+    the result is rounded."""
+    from parameter_server_b200.ops import dense, softmax
+
+    monkeypatch.setattr(softmax, "KEEP_MB", 0)           # 256 classes at a time, so that the rows are one piece
+    n, V, d = 6_000_001, 300, 8
+    x, w, y = _data(n, V, d, dtype, 23)
+    c = torch.full((n,), 2.0 ** -8, device="cuda")       # within fp16
+    _, gx, gw = softmax.softmax_loss(x, w, y, c)
+    dense.check_status(x.device)
+    W, ref = w.double(), torch.zeros(V, d, dtype=torch.float64, device="cuda")
+    for a in range(0, n, 500_000):
+        X, Y = x[a: a + 500_000].double(), y[a: a + 500_000]
+        p = torch.softmax(X @ W.T, 1)
+        p[torch.arange(len(Y), device="cuda"), Y] -= 1
+        ref += 2.0 ** -8 * (p.T @ X)
+    assert ((gw.double() - ref).norm() / ref.norm()).item() <= HALF_STEP[dtype] + 2 * 2.0 ** -12
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scores_of_very_wide_rows(dtype):
+    """Sums of a million products that have one sign, in fp32 results: added up every 32,768 columns, a score is off by 2^-12 of itself at
+    worst, and by 32 roundings of fp32; one sum of 65,536 cuts would be 0.3 % short."""
+    from parameter_server_b200.ops import softmax
+
+    n, V, d = 5, 40, 1 << 20
+    g = torch.Generator(device="cuda").manual_seed(24)
+    x, w = torch.rand(n, d, generator=g, device="cuda").to(dtype), (torch.rand(V, d, generator=g, device="cuda") * 2.0 ** -14).to(dtype)
+    y = torch.randint(0, V, (n,), generator=g, device="cuda")
+    w[y.unique()] *= 0.25                                # labels' scores are far below the others': they do not cancel
+    loss = softmax.softmax_loss(x, w, y, want_grad=False)[0]
+    s = x.double() @ w.double().T
+    ref = torch.logsumexp(s, 1) - s.gather(1, y[:, None])[:, 0]
+    assert bool(((loss.double() - ref).abs() <= 2 * (2.0 ** -12 + 2.0 ** -18) * s.max(1).values).all())
+    assert bool(((loss.double() - ref).abs() <= 2.0 ** -10 * ref).all())
