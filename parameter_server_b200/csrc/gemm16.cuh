@@ -7,9 +7,9 @@
 // where three tf32 products (11 bits as well) would cost six.  The tensor cores cut a sum to fp32 at every step of 16
 // elements instead of rounding it, an error that grows with the number of steps (K = 60,000: 6e-5 of a gradient); products
 // of planes are therefore summed in TMEM for 128 elements of K at a time (24 steps) and added up in the epilogue's
-// registers.  (64 elements: 25 % slower; 256: 4 % faster, twice the error.)  Products of 16-bit operands are summed in TMEM
-// for kLongK elements at a time: that is cut by 2^-13 of a sum of one sign, on average, which fp16 results do not show (6,000,000
-// elements in one sum: 0.8 %).  An operand may lie either way round in memory: K-major
+// registers.  (64 elements: 25 % slower; 256: 4 % faster, twice the error.)  Products of 16-bit operands are summed in
+// TMEM for as many elements at a time as the epilogue says (kLongK): 32,768 where results are of 16 bits (a sum of one sign comes out
+// 2^-14 short; 6,000,000 elements in one sum: 1 %), 4096 for scores, which are fp32 (2^-17).  An operand may lie either way round in memory: K-major
 // ([rows][k], k contiguous) or MN-major ([k][rows], rows contiguous); nothing is transposed in memory.
 //
 // Shape.  Persistent CTAs, or CTA pairs (cta_group::2) where the problem has enough tiles:
@@ -37,9 +37,9 @@ constexpr int kG16Epi = 4;                         // first warp of the epilogue
 constexpr int kG16Smem = 225 * 1024;              // of the stages and of what leaves
 constexpr int kBoxBytes = 2048;                   // 32 x 32 values of 16 bits
 
-constexpr int kLongK = 32768;
 
-template <int kCtas_, int kN_, int kPlanes_, int kParts_ = 2, bool kLong = false>
+// kLong: blocks of K that 16-bit operands are summed over in TMEM, 0: all
+template <int kCtas_, int kN_, int kPlanes_, int kParts_ = 2, int kLong = 0>
 struct Cfg16 {
   static constexpr int kCtas = kCtas_, kN = kN_, kPlanes = kPlanes_;
   static constexpr int kM = 128 * kCtas, kBRows = kN / kCtas;
@@ -51,8 +51,8 @@ struct Cfg16 {
   static constexpr int kFit = (kG16Smem - 4 * kParts * kBoxes * kBoxBytes) / kStageBytes, kStages = kFit > 8 ? 8 : kFit;
   static constexpr int kSmemBytes = kStages * kStageBytes + 4 * kParts * kBoxes * kBoxBytes + 1024 + 512;
   static constexpr int kBufs = 512 / kN;           // accumulators in TMEM: products run ahead of the epilogue by so many less one
-  static constexpr bool kPromote = kPlanes == 2 || kLong;       // sums of kChunk blocks of K are added up in registers
-  static constexpr int kChunk = kPlanes == 2 ? 2 : kLong ? kLongK / kG16K : 1 << 30;
+  static constexpr bool kPromote = kPlanes == 2 || kLong > 0;   // sums of kChunk blocks of K are added up in registers
+  static constexpr int kChunk = kPlanes == 2 ? 2 : kLong > 0 ? kLong : 1 << 30;
   static_assert(kStages >= 3 && kBRows % 64 == 0 && kBufs >= 2 && kSmemBytes <= 232448, "shape of a tile");
 };
 
@@ -644,12 +644,12 @@ int launch16(Chain& chain, psb::Launch16<Epi, kCount>& launch, const Operand16* 
 }
 
 // ---- which tiles, and in how many pieces K is taken
-// 256x256 on a pair, with two or four epilogue warps for 32 rows or for long sums, 256x128 on a pair, 128x128, 128x64
-enum : int { kPair256 = 0, kPair128 = 1, kOne128 = 2, kOne64 = 3, kKinds = 4, kPair256Wide = 4, kPair256Long = 5 };
+// 256x256 on a pair, with two or four epilogue warps for 32 rows, 256x128 on a pair, 128x128, 128x64
+enum : int { kPair256 = 0, kPair128 = 1, kOne128 = 2, kOne64 = 3, kKinds = 4, kPair256Wide = 4 };
 struct Tiling { int kind, splits, kb_split, sym; };
 
-inline int tiling_rows(int kind) { return kind <= kPair128 || kind >= kPair256Wide ? 256 : 128; }
-inline int tiling_cols(int kind) { return kind == kPair256 || kind >= kPair256Wide ? 256 : kind == kOne64 ? 64 : 128; }
+inline int tiling_rows(int kind) { return kind <= kPair128 || kind == kPair256Wide ? 256 : 128; }
+inline int tiling_cols(int kind) { return kind == kPair256 || kind == kPair256Wide ? 256 : kind == kOne64 ? 64 : 128; }
 inline int tiling_parts(int kind) { return kind == kPair256Wide ? 4 : 2; }
 
 // The cheapest by this estimate, in cycles of an SM.  A round of tiles costs its blocks of K, at the slower of the tensor
@@ -687,27 +687,33 @@ inline Tiling choose_tiling(int64_t batch, int64_t M, int64_t N, int64_t K, int 
   // One plane: up to K = 768 a tile's products take less time than its epilogue, where two warps wait out each other's loads
   // and exponentials (4096 x 65,536 scores, K = 512: 296 -> 208 us; K = 1024, 2 % slower: a stage less, more power).
   if (best.kind == kPair256 && planes == 1 && best.kb_split <= 12) best.kind = kPair256Wide;
-  if (planes == 1 && best.kb_split > psb::kLongK / psb::kG16K) best.kind = kPair256Long;
   return best;
 }
 
+template <int kPlanes, int kLong, class Epi>
+int launch_kind(Chain& chain, int kind, psb::Launch16<Epi, 1>& l, const Operand16& a, const Operand16& b) {
+  if (kind == kPair256) return launch16<psb::Cfg16<2, 256, kPlanes, 2, kLong>, Epi, 1>(chain, l, &a, &b);
+  if constexpr (kPlanes == 1 && kLong == 0) {
+    if (kind == kPair256Wide) return launch16<psb::Cfg16<2, 256, 1, 4>, Epi, 1>(chain, l, &a, &b);
+  }
+  if (kind == kPair128) return launch16<psb::Cfg16<2, 128, kPlanes, 2, kLong>, Epi, 1>(chain, l, &a, &b);
+  if (kind == kOne128) return launch16<psb::Cfg16<1, 128, kPlanes, 2, kLong>, Epi, 1>(chain, l, &a, &b);
+  return launch16<psb::Cfg16<1, 64, kPlanes, 2, kLong>, Epi, 1>(chain, l, &a, &b);
+}
 template <int kPlanes, class Epi>
 int launch_tiled(Chain& chain, int kind, psb::Launch16<Epi, 1>& l, const Operand16& a, const Operand16& b) {
-  if (kind == kPair256) return launch16<psb::Cfg16<2, 256, kPlanes>, Epi, 1>(chain, l, &a, &b);
+  constexpr int kLong = Epi::kLongK / psb::kG16K;
   if constexpr (kPlanes == 1) {
-    if (kind == kPair256Wide) return launch16<psb::Cfg16<2, 256, 1, 4>, Epi, 1>(chain, l, &a, &b);
-    if (kind == kPair256Long) return launch16<psb::Cfg16<2, 256, 1, 2, true>, Epi, 1>(chain, l, &a, &b);
+    if (l.g[0].kb_split > kLong) return launch_kind<1, kLong, Epi>(chain, kind, l, a, b);
   }
-  if (kind == kPair128) return launch16<psb::Cfg16<2, 128, kPlanes>, Epi, 1>(chain, l, &a, &b);
-  if (kind == kOne128) return launch16<psb::Cfg16<1, 128, kPlanes>, Epi, 1>(chain, l, &a, &b);
-  return launch16<psb::Cfg16<1, 64, kPlanes>, Epi, 1>(chain, l, &a, &b);
+  return launch_kind<kPlanes, 0, Epi>(chain, kind, l, a, b);
 }
 template <class Epi>
 int product16(Chain& chain, int planes, int kind, const psb::Gemm16Args& g, const Operand16& a, const Operand16& b, const typename Epi::Params& ep) {
   psb::Launch16<Epi, 1> l = {{g}, {ep}};
   return planes == 2 ? launch_tiled<2, Epi>(chain, kind, l, a, b) : launch_tiled<1, Epi>(chain, kind, l, a, b);
 }
-// two at once, in tiles of 128x128 or 128x64
+// two at once, in tiles of 128x128 or 128x64; sums of up to kLongK
 template <class Epi>
 int products16(Chain& chain, int planes, int kind, psb::Launch16<Epi, 2>& l, const Operand16* a, const Operand16* b) {
   if (planes == 2)

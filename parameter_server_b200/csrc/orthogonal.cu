@@ -203,6 +203,7 @@ k_orth_pack(const void* __restrict__ x, const float* m, int rows, int cols, int 
 // b A + c A² + a I = A (b I + c A) + a I and the new X = (a I + b A + c A²) X are plain products.
 __host__ __device__ __forceinline__ int up4(int n) { return (n + 3) & ~3; }
 struct EpiNs {
+  static constexpr int kLongK = 32768;
   struct Params {
     CUtensorMap out[2];
     float* slots;              // not null: raw sums, [split][batch][M][N rounded up to fours]

@@ -219,6 +219,7 @@ k_loss_planes(PackArgs px, PackArgs pw, int cols, const int64_t* __restrict__ y,
 // exponentials that are kept.  With planes, the largest 2^(s−m) 2^{-kw} and the largest 2^(s−m) of the part as well, both without
 // the label's class: where its softmax is near 1, its G is near 0.
 struct EpiScore {
+  static constexpr int kLongK = 4096;
   struct Params {
     CUtensorMap e;             // exponentials [plane][n][keep]
     float2* part;              // [n][per_tile · class tiles]; null: the exponentials alone, of classes from v0 on
@@ -329,6 +330,7 @@ struct EpiScore {
 
 // G of a piece of the classes, in the operands' 16-bit type, from scores made again
 struct EpiG {
+  static constexpr int kLongK = EpiScore::kLongK;
   struct Params {
     CUtensorMap g;             // [n][len]
     const float* lse;          // [n], log2
@@ -375,6 +377,7 @@ __device__ __forceinline__ void store_as(void* out, int64_t at, float v, int dty
 
 // A gradient: to the result, or as fp32 sums to `acc` (piece by piece, or one slot per split of K)
 struct EpiGrad {
+  static constexpr int kLongK = 32768;
   struct Params {
     CUtensorMap map;           // of the result, where it is 16-bit and aligned
     void* out;
@@ -997,7 +1000,7 @@ LossPlan make_loss_plan(const LossKey& a) {
     if (a.want_gx && !pieces && (p.gw.kind == kOne128 || p.gw.kind == kOne64)) {
       const Tiling t = choose_tiling(1, a.n, a.d, p.piece, p.planes, false, 64, 1, p.gw.kind);
       auto tiles = [&](const Tiling& u, int64_t M) { return (M + 127) / 128 * ((a.d + tiling_cols(u.kind) - 1) / tiling_cols(u.kind)) * u.splits; };
-      if (t.kind == p.gw.kind && tiles(p.gw, a.V) + tiles(t, a.n) <= 148) {
+      if ((p.gw.kb_split > t.kb_split ? p.gw.kb_split : t.kb_split) <= EpiGrad::kLongK / kG16K && tiles(p.gw, a.V) + tiles(t, a.n) <= 148) {
         p.together = 1;
         p.gx = t;
       }
