@@ -68,9 +68,9 @@ def orthogonalize(x: torch.Tensor, steps: int = 5) -> torch.Tensor:
     """``steps`` Newton-Schulz steps on a contiguous matrix [rows, cols] or a batch [batch, rows, cols], fp32, bf16 or
     fp16: ``X = x / (|x|_F + 1e-7)``, then ``X ← 3.4445 X − 4.7750 (X Xᵀ) X + 2.0315 (X Xᵀ)² X`` each, which brings singular
     values into about [0.7, 1.2].  The result has the type of x; fp32 and fp16 results are computed with 22-bit operands, bf16 ones
-    with 22 bits up to the last step and 11 bits in that (off by 0.18 to 0.21 % instead of the 0.17 % of their rounding); a short side of at most 16 is computed in fp32.  The workspace takes
-    8 bytes an element of x and 12 bytes or more an element of the smaller square, none where a short side of at most 128
-    keeps the matrix on the SMs."""
+    with 22 bits up to the last step and 11 bits in that (off by 0.18 to 0.21 % instead of the 0.17 % of their rounding); a short
+    side of at most 16 is computed in fp32.  The workspace takes 8 bytes an element of x and 12 bytes or more an element of the
+    smaller square, none where a short side of at most 128 keeps the matrix on the SMs."""
     gpu, shape = x.get_device(), x.shape
     _check("orthogonalize: x", x, gpu, shape, DTYPES)
     out = torch.empty_like(x)

@@ -36,9 +36,9 @@ def softmax_loss(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, coef: Option
     (gw).  A small call is one launch, in fp32 throughout.
 
     16-bit operands are multiplied as they are, and summed in fp32 on the tensor cores, which cut a sum at every 16 elements (scores
-    of 1024 columns: 3e-7 of the loss) and are left 4096 columns of scores, or 32,768 terms of gradients, at a time.  The gradient of the scores is rounded to the operands' type before its two products (bf16
-    gradients are off by 0.17 to 0.25 % instead of the 0.17 % that their own rounding takes); fp16 keeps it relative to the call's
-    largest coefficient, in units of 2^-38 of that.
+    of 1024 columns: 3e-7 of the loss) and are left 4096 columns of scores, or 32,768 terms of gradients, at a time.  The gradient
+    of the scores is rounded to the operands' type before its two products (bf16 gradients are off by 0.17 to 0.25 % instead of the
+    0.17 % that their own rounding takes); fp16 keeps it relative to the call's largest coefficient, in units of 2^-38 of that.
 
     Workspace: 8 bytes (fp32 with gradients: 16) for each row and 32 to 128 classes, for losses alone too; fp32 operands once more,
     and 16-bit ones whose rows do not start at 16 bytes; for gradients x once more, 2 bytes (fp32: 8) for each row and class, at most

@@ -257,3 +257,13 @@ def test_matrix_at_any_address(shape, dtype, offset):
     numel = torch.Size(shape).numel()
     x = (_data(shape, 11) * 1e-2).to(dtype)
     _check(torch.zeros(numel + 16, dtype=dtype, device="cuda")[offset: offset + numel].view(shape).copy_(x))
+
+
+@pytest.mark.parametrize("shape", [(20, 2_000_000), (1_500_000, 24)])
+def test_millions_of_columns(shape):
+    """bf16, whose last step sums one plane of up to 32,768 columns at a time: its own rounding (1.7e-3 on average) and that of the
+    operands of the last step (1.2e-3) are what is left."""
+    x = _data(shape, 12).bfloat16()
+    got = _check(x)
+    ref, _ = _reference(x, 5, torch.bfloat16)
+    assert ((got.double() - ref).norm() / ref.norm()).item() < 4e-3
